@@ -6,9 +6,13 @@ graph-sharded data-parallel helpers, and the two steps that feed the path (``dat
 device-side batch construction, ``utils.py:11-85``; ``rwconv`` / ``rw_gnn``: the row-normalised propagation
 layer and the per-hidden-node model of ``rwgnn_pyg.py:19-170`` on the same kernels).
 """
+from .attention import hop_buckets, packed_attention, packed_segments, pair_buckets, relative_buckets
 from .model import RW_NN
 from .structure import GraphStructure, clear_structure_cache, get_structure
 from .function import rw_kernel_layer
-from .optim import Adam
+from .layer_norm import LayerNorm, layer_norm
+from .optim import Adam, AdamW
 
-__all__ = ["RW_NN", "Adam", "GraphStructure", "get_structure", "clear_structure_cache", "rw_kernel_layer"]
+__all__ = ["RW_NN", "Adam", "AdamW", "GraphStructure", "LayerNorm", "clear_structure_cache", "get_structure",
+           "hop_buckets", "layer_norm", "packed_attention", "packed_segments", "pair_buckets", "relative_buckets",
+           "rw_kernel_layer"]

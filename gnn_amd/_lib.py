@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librwk.so")
@@ -142,6 +142,18 @@ SIGNATURES = {
     "rwk_model_train_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rwk_model_train_pass_plan": (c_int, [_P, _P, _I64, _P, _I64, _P, _P]),
     "rwk_model_train_pass": (c_int, [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int]),
+    "rwk_layer_norm_forward": (c_int, [_P, _I64, _P, _P, _I64, _I64, c_int32, c_int32, c_float, _P, _P, _P, _P]),
+    "rwk_layer_norm_backward_blocks": (_I64, [_I64, _I64, c_int32]),
+    "rwk_layer_norm_backward": (c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, c_int32, c_int32, _P, _P, _P, _P,
+                                        _P]),
+    "rwk_adamw_chunk_size": (_I64, []),
+    "rwk_adamw_step": (c_int, [_P, _P, _I64, _I64, _P, _I64, c_int32, c_int32, _P, c_double, c_double, c_double,
+                               c_double, c_uint64, _P, _P]),
+    "rwk_attention_forward": (c_int, [_P, _P]),
+    "rwk_attention_backward": (c_int, [_P, _P]),
+    "rwk_pair_buckets_dense": (c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P]),
+    "rwk_pair_buckets_relative": (c_int, [_P, _I64, _P, _P, _I64, _I64, _P, _P]),
+    "rwk_pair_buckets_hops": (c_int, [_P, _P, _P, c_int32, _P, _P, _I64, _I64, _P, _P]),
 }
 
 _lib = None
@@ -173,6 +185,15 @@ def check(code: int, what: str):
     if code != 0:
         msg = load().rwk_error_string(code).decode()
         raise RwkError(f"{what} failed: {msg} (code {code})")
+
+
+def element_type(dtype):
+    """``RWK_F32`` / ``RWK_F16`` / ``RWK_BF16`` of a torch dtype; ``TypeError`` for any other."""
+    import torch
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    if code is None:
+        raise TypeError("expected float32, float16 or bfloat16, got %s" % dtype)
+    return code
 
 
 def ptr(t):

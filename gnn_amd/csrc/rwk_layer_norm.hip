@@ -1,0 +1,438 @@
+// Layer norm over the last dimension of a (rows, width) matrix and its backward pass:
+//
+//   h = (x - mean) * rstd,  y = h * w + b,      mean, var of the row, rstd = 1 / sqrt(var + eps)
+//   dx = rstd * (t - mean(t) - h * mean(t * h)),  t = dy * w;      dw = sum_rows dy * h,  db = sum_rows dy
+//
+// Both passes are bound by memory: the forward reads and writes each element once, the backward reads x and dy and
+// writes dx.  A row stays in the registers of the lanes that share it between its statistics and its output (the
+// variance is the mean of squared distances from the mean, not a difference of two large sums).  All arithmetic is
+// fp32, one rounding to the element type at the store.
+#include "rwk_vec.h"
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / RWK_WAVE;
+
+// Sum over the TPR threads that share a row (a part of a wavefront, a wavefront or the workgroup), to all of them.
+// `red` holds kWaves floats and is used by workgroup-wide rows only; two alternating buffers save a barrier.
+template <int TPR>
+__device__ inline float row_sum(float v, float *red) {
+    if (TPR <= RWK_WAVE) return rwk_group_sum(v, TPR);
+    v = rwk_wave_sum(v);
+    if ((threadIdx.x & (RWK_WAVE - 1)) == 0) red[threadIdx.x / RWK_WAVE] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += red[w];
+    return s;
+}
+
+// The V * IT elements of a row that thread t of TPR holds: vectors t, t + TPR, ...  Beyond the row: zeros.
+template <typename T, int TPR, int V, int IT>
+__device__ inline void load_row(const T *__restrict__ row, int width, int t, float (&out)[IT * V]) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (t + i * TPR) * V;
+        if (c + V <= width) {
+            const auto v = rwk_load<T, V>(row + c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[i * V + j] = (float)v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[i * V + j] = c + j < width ? (float)row[c + j] : 0.f;
+        }
+    }
+}
+
+template <typename T, int TPR, int V, int IT>
+__device__ inline void store_row(T *__restrict__ row, int width, int t, const float (&in)[IT * V]) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (t + i * TPR) * V;
+        if (c + V <= width) {
+            typename RwkPack<T, V>::type v;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = (T)in[i * V + j];
+            rwk_store<T, V>(row + c, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < width) row[c + j] = (T)in[i * V + j];
+        }
+    }
+}
+
+template <typename T, typename W, int TPR, int V, int IT>
+__global__ void __launch_bounds__(kBlock)
+norm_forward_kernel(const T *__restrict__ x, long long x_stride, const W *__restrict__ weight,
+                    const W *__restrict__ bias, long long rows, int width, float eps, T *__restrict__ y,
+                    float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+    __shared__ float red[2][kWaves];
+    constexpr int kRows = kBlock / TPR;
+    const int t = threadIdx.x % TPR;
+    for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows) {
+        const long long r = r0 + threadIdx.x / TPR;
+        const bool there = r < rows;                  // the whole workgroup takes part in the sums
+        float v[IT * V];
+        load_row<T, TPR, V, IT>(x + (there ? r : rows - 1) * x_stride, width, t, v);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT * V; ++i) s += v[i];
+        const float mean = row_sum<TPR>(s, red[0]) / (float)width;    // exact for constant rows
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = (t + i * TPR) * V + j < width ? v[i * V + j] - mean : 0.f;
+                v[i * V + j] = d;
+                q = fmaf(d, d, q);
+            }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / (float)width + eps);
+        float w[IT * V], b[IT * V];
+        load_row<W, TPR, V, IT>(weight, width, t, w);
+        if (bias != nullptr) load_row<W, TPR, V, IT>(bias, width, t, b);
+#pragma unroll
+        for (int i = 0; i < IT * V; ++i) v[i] = bias != nullptr ? fmaf(v[i] * rstd, w[i], b[i]) : v[i] * rstd * w[i];
+        if (!there) continue;
+        store_row<T, TPR, V, IT>(y + r * width, width, t, v);
+        if (t == 0 && mean_out != nullptr) {
+            mean_out[r] = mean;
+            rstd_out[r] = rstd;
+        }
+    }
+}
+
+// dx of the workgroup's rows and its sums of dy * h and dy over them: one row [dw | db] of `partials` per workgroup.
+template <typename T, typename W, int TPR, int V, int IT>
+__global__ void __launch_bounds__(kBlock)
+norm_backward_kernel(const T *__restrict__ x, long long x_stride, const T *__restrict__ dy, long long dy_stride,
+                     const W *__restrict__ weight, const float *__restrict__ mean_in,
+                     const float *__restrict__ rstd_in, long long rows, int width, T *__restrict__ dx,
+                     float *__restrict__ partials) {
+    constexpr int kRows = kBlock / TPR;
+    __shared__ float red[2][2][kWaves];
+    const int t = threadIdx.x % TPR;
+    const float inv = 1.f / (float)width;
+    float w[IT * V], dw[IT * V], db[IT * V];
+    load_row<W, TPR, V, IT>(weight, width, t, w);
+#pragma unroll
+    for (int i = 0; i < IT * V; ++i) dw[i] = db[i] = 0.f;
+    int turn = 0;
+    for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows, turn ^= 1) {
+        const long long r = r0 + threadIdx.x / TPR;
+        const bool there = r < rows;
+        const long long rc = there ? r : rows - 1;
+        float h[IT * V], g[IT * V];
+        load_row<T, TPR, V, IT>(x + rc * x_stride, width, t, h);
+        load_row<T, TPR, V, IT>(dy + rc * dy_stride, width, t, g);
+        const float mean = mean_in[rc], rstd = rstd_in[rc];
+        float a = 0.f, c = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT * V; ++i) {
+            h[i] = (h[i] - mean) * rstd;              // beyond the row: dy = 0 and w = 0 take it out
+            if (there) {
+                dw[i] = fmaf(g[i], h[i], dw[i]);
+                db[i] += g[i];
+            }
+            g[i] *= w[i];
+            a += g[i];
+            c = fmaf(g[i], h[i], c);
+        }
+        a = row_sum<TPR>(a, red[turn][0]) * inv;
+        c = row_sum<TPR>(c, red[turn][1]) * inv;
+#pragma unroll
+        for (int i = 0; i < IT * V; ++i) h[i] = rstd * (g[i] - a - h[i] * c);
+        if (there) store_row<T, TPR, V, IT>(dx + r * width, width, t, h);
+    }
+    float *out = partials + (long long)blockIdx.x * 2 * width;
+    if (TPR == kBlock) {
+        store_row<float, TPR, V, IT>(out, width, t, dw);
+        store_row<float, TPR, V, IT>(out + width, width, t, db);
+    } else {
+        // the workgroup's kRows row slots in slot order
+        __shared__ float sums[kBlock * V];
+#pragma unroll
+        for (int k = 0; k < 2 * IT; ++k) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                sums[threadIdx.x * V + j] = k < IT ? dw[(k % IT) * V + j] : db[(k % IT) * V + j];
+            __syncthreads();
+            for (int e = threadIdx.x; e < TPR * V; e += kBlock) {
+                float s = 0.f;
+                for (int q = 0; q < kRows; ++q) s += sums[q * TPR * V + e];
+                const int col = (k % IT) * TPR * V + e;
+                if (col < width) out[(k < IT ? 0 : width) + col] = s;
+            }
+        }
+    }
+}
+
+// Rows too wide for registers: the same sums in three passes over the row, which the second and third find in the
+// cache of the compute unit's die.
+template <typename T, typename W>
+__global__ void __launch_bounds__(kBlock)
+norm_forward_wide_kernel(const T *__restrict__ x, long long x_stride, const W *__restrict__ weight,
+                         const W *__restrict__ bias, int width, float eps, T *__restrict__ y,
+                         float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+    __shared__ float red[2][kWaves];
+    const long long r = blockIdx.x;
+    const T *row = x + r * x_stride;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < width; c += kBlock) s += (float)row[c];
+    const float mean = row_sum<kBlock>(s, red[0]) / (float)width;
+    float q = 0.f;
+    for (int c = threadIdx.x; c < width; c += kBlock) {
+        const float d = (float)row[c] - mean;
+        q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<kBlock>(q, red[1]) / (float)width + eps);
+    for (int c = threadIdx.x; c < width; c += kBlock)
+        y[r * width + c] = (T)fmaf(((float)row[c] - mean) * rstd, (float)weight[c],
+                                   bias != nullptr ? (float)bias[c] : 0.f);
+    if (threadIdx.x == 0 && mean_out != nullptr) {
+        mean_out[r] = mean;
+        rstd_out[r] = rstd;
+    }
+}
+
+template <typename T, typename W>
+__global__ void __launch_bounds__(kBlock)
+norm_backward_wide_kernel(const T *__restrict__ x, long long x_stride, const T *__restrict__ dy, long long dy_stride,
+                          const W *__restrict__ weight, const float *__restrict__ mean_in,
+                          const float *__restrict__ rstd_in, int width, T *__restrict__ dx) {
+    __shared__ float red[2][kWaves];
+    const long long r = blockIdx.x;
+    const T *row = x + r * x_stride, *grad = dy + r * dy_stride;
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    float a = 0.f, c = 0.f;
+    for (int i = threadIdx.x; i < width; i += kBlock) {
+        const float t = (float)grad[i] * (float)weight[i];
+        a += t;
+        c = fmaf(t, ((float)row[i] - mean) * rstd, c);
+    }
+    a = row_sum<kBlock>(a, red[0]) / (float)width;
+    c = row_sum<kBlock>(c, red[1]) / (float)width;
+    for (int i = threadIdx.x; i < width; i += kBlock)
+        dx[r * width + i] = (T)(rstd * ((float)grad[i] * (float)weight[i] - a - ((float)row[i] - mean) * rstd * c));
+}
+
+// [dw | db] partials of wide rows: workgroup (column block, row split)
+template <typename T>
+__global__ void __launch_bounds__(kBlock)
+norm_weight_wide_kernel(const T *__restrict__ x, long long x_stride, const T *__restrict__ dy, long long dy_stride,
+                        const float *__restrict__ mean_in, const float *__restrict__ rstd_in, long long rows,
+                        int width, float *__restrict__ partials) {
+    const int c = blockIdx.x * kBlock + threadIdx.x;
+    if (c >= width) return;
+    float dw = 0.f, db = 0.f;
+    for (long long r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float g = (float)dy[r * dy_stride + c];
+        dw = fmaf(g, ((float)x[r * x_stride + c] - mean_in[r]) * rstd_in[r], dw);
+        db += g;
+    }
+    float *out = partials + (long long)blockIdx.y * 2 * width;
+    out[c] = dw;
+    out[width + c] = db;
+}
+
+// dw, db = column sums of the partial rows [dw | db], in row order within 16 fixed groups, then in group order
+constexpr int kSumCols = 64, kSumGroups = 16;
+template <typename W>
+__global__ void __launch_bounds__(kSumCols * kSumGroups)
+norm_weight_sum_kernel(const float *__restrict__ partials, int n_partials, int width, W *__restrict__ dw,
+                       W *__restrict__ db) {
+    __shared__ float part[kSumGroups][kSumCols];
+    const int lane = threadIdx.x % kSumCols, group = threadIdx.x / kSumCols;
+    const long long c = (long long)blockIdx.x * kSumCols + lane;
+    float s = 0.f;
+    if (c < 2ll * width)
+        for (int p = group; p < n_partials; p += kSumGroups) s += partials[(long long)p * 2 * width + c];
+    part[group][lane] = s;
+    __syncthreads();
+    if (group != 0 || c >= 2ll * width) return;
+    for (int g = 1; g < kSumGroups; ++g) s += part[g][lane];
+    if (c < width) {
+        dw[c] = (W)s;
+    } else if (db != nullptr) {
+        db[c - width] = (W)s;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Launch shapes.  Threads per row: as few as hold the row in one vector each up to a wavefront, so that narrow rows
+// (node features of a few channels) still fill every lane; wider rows give each lane of a wavefront, then of a
+// workgroup, more vectors.  The backward pass keeps two column sums per element besides the row and turns to the
+// workgroup earlier.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kMaxGrid = 4096;
+constexpr int kBackwardGrid = 1024;     // workgroups of the backward pass, each with one row of partial sums
+constexpr int kWideSplit = 64;
+
+constexpr int kRegisterWidth = 8192;    // wider rows do not fit a workgroup's registers
+
+int rows_per_block(int64_t width, int vec) {
+    const int64_t vectors = rwk_ceil_div(width, vec);
+    if (vectors <= 4) return kBlock / 4;
+    if (vectors <= 16) return kBlock / 16;
+    if (vectors <= 128) return kBlock / 64;
+    return 1;
+}
+
+int64_t backward_blocks(int64_t rows, int64_t width, int vec) {
+    if (width > kRegisterWidth) return rows < kWideSplit ? rows : kWideSplit;
+    const int64_t blocks = rwk_ceil_div(rows, rows_per_block(width, vec));
+    return blocks < kBackwardGrid ? blocks : kBackwardGrid;
+}
+
+struct NormArgs {
+    const void *x, *dy, *weight, *bias;
+    long long x_stride, dy_stride, rows;
+    int width;
+    float eps;
+    void *out;                    // y or dx
+    float *mean, *rstd, *partials;
+    void *dw, *db;
+    hipStream_t stream;
+};
+
+template <typename T, typename W, int TPR, int IT>
+int launch_forward(const NormArgs &a) {
+    constexpr int V = RwkVecOf<T>::n;
+    long long grid = rwk_ceil_div(a.rows, kBlock / TPR);
+    if (grid > kMaxGrid) grid = kMaxGrid;
+    hipLaunchKernelGGL((norm_forward_kernel<T, W, TPR, V, IT>), dim3((unsigned)grid), dim3(kBlock), 0, a.stream,
+                       (const T *)a.x, a.x_stride, (const W *)a.weight, (const W *)a.bias, a.rows, a.width, a.eps,
+                       (T *)a.out, a.mean, a.rstd);
+    RWK_LAUNCH_CHECK();
+    return RWK_OK;
+}
+
+template <typename T, typename W>
+int forward(const NormArgs &a) {
+    constexpr int V = RwkVecOf<T>::n;
+    const int64_t vectors = rwk_ceil_div(a.width, V);
+    if (vectors <= 4) return launch_forward<T, W, 4, 1>(a);
+    if (vectors <= 16) return launch_forward<T, W, 16, 1>(a);
+    if (vectors <= 64) return launch_forward<T, W, 64, 1>(a);
+    if (vectors <= 128) return launch_forward<T, W, 64, 2>(a);
+    if (vectors <= 256) return launch_forward<T, W, 256, 1>(a);
+    if (vectors <= 512) return launch_forward<T, W, 256, 2>(a);
+    if (vectors <= 1024) return launch_forward<T, W, 256, 4>(a);
+    if (vectors <= 2048 && V == 4) return launch_forward<T, W, 256, 8>(a);
+    if (a.rows > 0x7FFFFFFFll) return RWK_E_SIZE;
+    hipLaunchKernelGGL((norm_forward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(kBlock), 0, a.stream,
+                       (const T *)a.x, a.x_stride, (const W *)a.weight, (const W *)a.bias, a.width, a.eps, (T *)a.out,
+                       a.mean, a.rstd);
+    RWK_LAUNCH_CHECK();
+    return RWK_OK;
+}
+
+template <typename T, typename W, int TPR, int IT>
+int launch_backward(const NormArgs &a, int64_t blocks) {
+    constexpr int V = RwkVecOf<T>::n;
+    hipLaunchKernelGGL((norm_backward_kernel<T, W, TPR, V, IT>), dim3((unsigned)blocks), dim3(kBlock), 0, a.stream,
+                       (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, (const W *)a.weight, a.mean, a.rstd,
+                       a.rows, a.width, (T *)a.out, a.partials);
+    RWK_LAUNCH_CHECK();
+    return RWK_OK;
+}
+
+template <typename T, typename W>
+int backward(const NormArgs &a) {
+    constexpr int V = RwkVecOf<T>::n;
+    const int64_t vectors = rwk_ceil_div(a.width, V);
+    const int64_t blocks = backward_blocks(a.rows, a.width, V);
+    int code = RWK_OK;
+    if (a.width > kRegisterWidth) {
+        if (a.rows > 0x7FFFFFFFll) return RWK_E_SIZE;
+        hipLaunchKernelGGL((norm_backward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(kBlock), 0, a.stream,
+                           (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, (const W *)a.weight, a.mean,
+                           a.rstd, a.width, (T *)a.out);
+        RWK_LAUNCH_CHECK();
+        hipLaunchKernelGGL((norm_weight_wide_kernel<T>), dim3((unsigned)rwk_ceil_div(a.width, kBlock), (unsigned)blocks),
+                           dim3(kBlock), 0, a.stream, (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, a.mean,
+                           a.rstd, a.rows, a.width, a.partials);
+        RWK_LAUNCH_CHECK();
+    } else if (vectors <= 4) {
+        code = launch_backward<T, W, 4, 1>(a, blocks);
+    } else if (vectors <= 16) {
+        code = launch_backward<T, W, 16, 1>(a, blocks);
+    } else if (vectors <= 64) {
+        code = launch_backward<T, W, 64, 1>(a, blocks);
+    } else if (vectors <= 128) {
+        code = launch_backward<T, W, 64, 2>(a, blocks);
+    } else if (vectors <= 256) {
+        code = launch_backward<T, W, 256, 1>(a, blocks);
+    } else if (vectors <= 512) {
+        code = launch_backward<T, W, 256, 2>(a, blocks);
+    } else if (vectors <= 1024) {
+        code = launch_backward<T, W, 256, 4>(a, blocks);
+    } else {
+        code = launch_backward<T, W, 256, V == 4 ? 8 : 4>(a, blocks);     // fp32 rows of 4097 to 8192
+    }
+    if (code != RWK_OK) return code;
+    hipLaunchKernelGGL((norm_weight_sum_kernel<W>), dim3((unsigned)rwk_ceil_div(2ll * a.width, kSumCols)),
+                       dim3(kSumCols * kSumGroups), 0, a.stream, a.partials, (int)blocks, a.width, (W *)a.dw,
+                       (W *)a.db);
+    RWK_LAUNCH_CHECK();
+    return RWK_OK;
+}
+
+int check(const NormArgs &a, int32_t type, int32_t weight_type) {
+    RWK_REQUIRE_PTR(a.x);
+    RWK_REQUIRE_PTR(a.weight);
+    RWK_REQUIRE_PTR(a.out);
+    if (type < RWK_F32 || type > RWK_BF16 || (weight_type != type && weight_type != RWK_F32)) return RWK_E_UNSUPPORTED;
+    if (a.rows <= 0 || a.width <= 0 || a.x_stride < a.width) return RWK_E_SIZE;
+    return RWK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t rwk_layer_norm_backward_blocks(int64_t rows, int64_t width, int32_t type) {
+    if (rows <= 0 || width <= 0 || width > 0x3FFFFFFF) return 0;
+    return backward_blocks(rows, width, type == RWK_F32 ? 4 : 8);
+}
+
+int rwk_layer_norm_forward(const void *x, int64_t x_stride, const void *weight, const void *bias, int64_t rows,
+                           int64_t width, int32_t type, int32_t weight_type, float eps, void *y, float *mean,
+                           float *rstd, rwk_stream_t stream) {
+    if (width > 0x3FFFFFFF) return RWK_E_SIZE;
+    NormArgs a{};
+    a.x = x; a.weight = weight; a.bias = bias; a.x_stride = x_stride; a.rows = rows; a.width = (int)width; a.eps = eps;
+    a.out = y; a.mean = mean; a.rstd = rstd; a.stream = (hipStream_t)stream;
+    const int code = check(a, type, weight_type);
+    if (code != RWK_OK) return code;
+    if ((mean == nullptr) != (rstd == nullptr)) return RWK_E_NULL;
+    if (type == RWK_F32) return forward<float, float>(a);
+    if (type == RWK_F16) return weight_type == RWK_F32 ? forward<rwk_f16, float>(a) : forward<rwk_f16, rwk_f16>(a);
+    return weight_type == RWK_F32 ? forward<rwk_bf16, float>(a) : forward<rwk_bf16, rwk_bf16>(a);
+}
+
+int rwk_layer_norm_backward(const void *x, int64_t x_stride, const void *dy, int64_t dy_stride, const void *weight,
+                            const float *mean, const float *rstd, int64_t rows, int64_t width, int32_t type,
+                            int32_t weight_type, void *dx, float *partials, void *dw, void *db, rwk_stream_t stream) {
+    if (width > 0x3FFFFFFF) return RWK_E_SIZE;
+    NormArgs a{};
+    a.x = x; a.dy = dy; a.weight = weight; a.x_stride = x_stride; a.dy_stride = dy_stride; a.rows = rows;
+    a.width = (int)width; a.out = dx; a.mean = (float *)mean; a.rstd = (float *)rstd; a.partials = partials;
+    a.dw = dw; a.db = db; a.stream = (hipStream_t)stream;
+    const int code = check(a, type, weight_type);
+    if (code != RWK_OK) return code;
+    RWK_REQUIRE_PTR(dy);
+    RWK_REQUIRE_PTR(mean);
+    RWK_REQUIRE_PTR(rstd);
+    RWK_REQUIRE_PTR(partials);
+    RWK_REQUIRE_PTR(dw);
+    if (dy_stride < width) return RWK_E_SIZE;
+    if (type == RWK_F32) return backward<float, float>(a);
+    if (type == RWK_F16) return weight_type == RWK_F32 ? backward<rwk_f16, float>(a) : backward<rwk_f16, rwk_f16>(a);
+    return weight_type == RWK_F32 ? backward<rwk_bf16, float>(a) : backward<rwk_bf16, rwk_bf16>(a);
+}
+
+}  // extern "C"

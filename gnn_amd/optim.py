@@ -8,12 +8,13 @@ device, so the update can be captured in a HIP graph and a scheduler can change 
 """
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from . import _lib
 from .dp import FlatGradBucket
 
-__all__ = ["FlatAdam", "StepTail", "Adam"]
+__all__ = ["FlatAdam", "StepTail", "Adam", "AdamW"]
 
 
 class FlatAdam:
@@ -312,3 +313,227 @@ class StepTail:
             o.betas[1], o.eps, o.weight_decay, upd(self.counters), _lib.ptr(self.corr_slot), stream),
             "rwk_hidden_backward_reduce_adam")
         self.done = True
+
+
+class _AdamWTable:
+    """Device tables of one launch shape: the parameters of one group with one type on one device."""
+
+    def __init__(self, opt: "AdamW", group: dict, params, ids):
+        self.group, self.params = group, params
+        self.dtype, self.device = params[0].dtype, params[0].device
+        self.type = _lib.element_type(self.dtype)
+        size = int(_lib.load().rwk_adamw_chunk_size())
+        fields, steps = [], []
+        for i, (p, pid) in enumerate(zip(params, ids)):
+            st = opt.state[p]
+            fields += [p.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
+                       st["exp_avg_scale"].data_ptr() if opt.state_bits == 8 else 0,
+                       st["exp_avg_sq_scale"].data_ptr() if opt.state_bits == 8 else 0, p.numel(), pid - i]
+            steps.append(int(st["step"]))
+        n_chunks = -(-np.array([p.numel() for p in params], dtype=np.int64) // size)
+        ends = np.cumsum(n_chunks)
+        self.first_chunk = [0] + ends.tolist()
+        chunks = np.empty((int(ends[-1]), 2), dtype=np.int64)                          # rwk_adamw_chunk[]
+        chunks[:, 0] = np.repeat(np.arange(len(params)), n_chunks)
+        chunks[:, 1] = (np.arange(len(chunks)) - np.repeat(ends - n_chunks, n_chunks)) * size
+        fields = np.array(fields, dtype=np.int64)                                      # rwk_adamw_tensor[]
+        packed = torch.from_numpy(np.concatenate([fields, chunks.reshape(-1), np.repeat(steps, n_chunks)])).to(
+            self.device)                                                               # one copy to the device
+        self.table, self.chunks, self.steps = packed.split([fields.size, chunks.size, len(chunks)])
+        self.lr = torch.tensor([float(group["lr"])], dtype=torch.float64, device=self.device)
+        self.lr_on_device = float(group["lr"])
+        self.pointers = [p.data_ptr() for p in params]
+
+    def push_lr(self):
+        lr = float(self.group["lr"])
+        if lr != self.lr_on_device:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the learning rate changed: call push_lr() before the capture (a captured step "
+                                   "reads the rate from the device)")
+            with _lib.device_guard(self.device):
+                self.lr.fill_(lr)
+            self.lr_on_device = lr
+
+    def step(self, lib, opt: "AdamW"):
+        import ctypes
+        keep, grads = [], []
+        for p in self.params:
+            g = p.grad
+            if g is not None:
+                if g.layout != torch.strided:
+                    raise RuntimeError("gnn_amd.AdamW does not take sparse gradients")
+                if g.dtype is not self.dtype or g.device != self.device:
+                    raise TypeError("a gradient must have its parameter's type and device")
+                g = g.detach()
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                keep.append(g)
+                g = g.data_ptr()
+            grads.append(g)
+        self.push_lr()
+        group, stream = self.group, _lib.current_stream(self.device)
+        limit = 256                                       # RWK_ADAMW_TENSORS: gradient addresses of one launch
+        with _lib.device_guard(self.device):
+            for base in range(0, len(grads), limit):
+                part = grads[base:base + limit]
+                lo, hi = self.first_chunk[base], self.first_chunk[base + len(part)]
+                if hi == lo or all(g is None for g in part):
+                    continue
+                _lib.check(lib.rwk_adamw_step(
+                    self.table.data_ptr(), self.chunks.data_ptr() + 16 * lo, hi - lo, base,
+                    (ctypes.c_void_p * len(part))(*part), len(part), self.type, opt.state_bits, self.lr.data_ptr(),
+                    float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
+                    float(group["weight_decay"]), opt.seed, self.steps.data_ptr() + 8 * lo, stream),
+                    "rwk_adamw_step")
+        self._keep = keep                                 # the launches read them asynchronously
+
+    def read_steps(self, opt: "AdamW"):
+        steps = self.steps.tolist()
+        for p, lo, hi in zip(self.params, self.first_chunk, self.first_chunk[1:]):
+            if hi > lo:                                   # a tensor without elements has no chunk to count in
+                opt.state[p]["step"] = torch.tensor(float(steps[lo]), dtype=torch.float32)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over any number of tensors with one launch per 256 of them, their moment
+    estimates held in 32 or in 8 bits: ``optimizer = gnn_amd.AdamW(model.parameters(), lr=1e-3, state_bits=8)``.
+
+    A ``torch.optim.Optimizer``: parameter groups with their own rates, betas and decay, schedulers, closures,
+    ``state_dict()`` / ``load_state_dict()``.  Parameters are contiguous float32, float16 or bfloat16 tensors on HIP
+    devices and stay where they are (:class:`Adam` moves them into one flat fp32 buffer).  The update is computed in
+    fp32 and rounded to the parameter's type once; a parameter whose ``.grad`` is ``None`` is skipped and does not
+    age.  The step counts and the learning rate live on the device, so a captured step replays correctly;
+    :meth:`push_lr` hands a changed rate to replays.
+
+    ``state_bits=32``: ``exp_avg`` and ``exp_avg_sq`` are float32, in torch's layout.  ``state_bits=8``: they are
+    float8 (e4m3) tensors with one fp32 scale per 256 consecutive elements (``exp_avg_scale``, ``exp_avg_sq_scale``;
+    a moment is value times scale), a quarter of the memory.  Values are rounded up or down at random in proportion to
+    the distances - ``exp_avg_sq`` moves by a thousandth per step, far less than the spacing of 8-bit values - with
+    bits that follow from ``seed``, the step, the tensor's place and the element, so runs repeat bit by bit.  A
+    gradient that is not finite makes its whole block of 256 moments not finite."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if not 0 <= int(seed) < 2 ** 64:
+            raise ValueError("seed must be in 0 .. 2^64 - 1")
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self._tables = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            if not float(group["lr"]) >= 0.0:
+                raise ValueError("lr must not be negative")
+            if not float(group["eps"]) >= 0.0:
+                raise ValueError("eps must not be negative")
+            if not float(group["weight_decay"]) >= 0.0:
+                raise ValueError("weight_decay must not be negative")
+            if not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
+                raise ValueError("betas must be in [0, 1)")
+            for p in group["params"]:
+                if not p.is_cuda:
+                    raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
+                _lib.element_type(p.dtype)
+                if p.layout != torch.strided or not p.is_contiguous():
+                    raise ValueError("gnn_amd.AdamW takes contiguous parameters")
+        except Exception:
+            self.param_groups.pop()
+            raise
+        for p in group["params"]:
+            self.state[p] = self._new_state(p)
+        self._drop_tables()
+
+    def _new_state(self, p):
+        st = {"step": torch.zeros((), dtype=torch.float32)}
+        n = p.numel()
+        for name in ("exp_avg", "exp_avg_sq"):
+            if self.state_bits == 32:
+                st[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                blocks = (n + 255) // 256
+                flat = torch.zeros(blocks * 256, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                st[name] = flat[:n].view(p.shape)         # the kernel reads and writes whole blocks of 256
+                st[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        return st
+
+    def _drop_tables(self):
+        """The tables describe other tensors from here on: their step counts move to the state."""
+        if self._tables is not None:
+            for t in self._tables:
+                t.read_steps(self)
+        self._tables = None
+
+    def _build_tables(self):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gnn_amd.AdamW builds its tables at its first step and whenever a parameter moved: "
+                               "take one step before the capture")
+        self._drop_tables()
+        tables, pid = [], 0
+        for group in self.param_groups:
+            kinds = {}
+            for p in group["params"]:
+                if not p.is_cuda or p.layout != torch.strided or not p.is_contiguous():
+                    raise ValueError("gnn_amd.AdamW takes contiguous parameters on HIP devices")
+                if any(s.device != p.device for k, s in self.state[p].items() if k != "step"):
+                    raise RuntimeError("a parameter moved to another device after the optimiser was built")
+                kinds.setdefault((p.dtype, p.device), ([], []))
+                kinds[p.dtype, p.device][0].append(p)
+                kinds[p.dtype, p.device][1].append(pid)
+                pid += 1
+            for params, ids in kinds.values():
+                with _lib.device_guard(params[0].device):
+                    tables.append(_AdamWTable(self, group, params, ids))
+        self._tables = tables
+
+    def push_lr(self):
+        """Hand changed learning rates to the device (``step`` does it by itself; replays of a captured step do not)."""
+        for t in self._tables or ():
+            t.push_lr()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if self._tables is None or any([p.data_ptr() for p in t.params] != t.pointers for t in self._tables):
+            self._build_tables()
+        lib = _lib.load()
+        for t in self._tables:
+            t.step(lib, self)
+        return loss
+
+    def state_dict(self):
+        for t in self._tables or ():                      # the step counts live on the device
+            t.read_steps(self)
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        names = ["exp_avg", "exp_avg_sq"]
+        if self.state_bits == 8:
+            names += ["exp_avg_scale", "exp_avg_sq_scale"]
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        new = {}
+        for i, p in zip(saved, params):                   # checked whole before anything is changed
+            st = self._new_state(p)
+            src = state_dict["state"].get(i)
+            if src:
+                for name in names:
+                    if name not in src:
+                        raise ValueError(f"the saved state has no {name}: it was made with other state_bits")
+                    dtype = torch.float8_e4m3fn if self.state_bits == 8 and not name.endswith("_scale") \
+                        else torch.float32
+                    if src[name].dtype != dtype or src[name].shape != st[name].shape:
+                        raise ValueError(f"the saved {name} is {src[name].dtype} of shape {tuple(src[name].shape)}, "
+                                         f"not {dtype} of shape {tuple(st[name].shape)}")
+                    st[name].copy_(src[name])
+                st["step"] = torch.tensor(float(src["step"]), dtype=torch.float32)
+            new[p] = st
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self._tables = None
+        for p, st in new.items():
+            self.state[p] = st

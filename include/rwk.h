@@ -41,6 +41,11 @@ extern "C" {
 #define RWK_E_STATIC_SIZE (-5) /* the input needs more of the library's fixed device scratch than it holds */
 #define RWK_E_DEVICE (-6)      /* the stream's device is not the current device */
 
+/* element types of the entry points that serve more than float32 */
+#define RWK_F32 0
+#define RWK_F16 1
+#define RWK_BF16 2
+
 typedef void *rwk_stream_t;
 
 int rwk_version(void);
@@ -883,6 +888,120 @@ int rwk_distance_bias_combine(const float *x, const float *y, const float *s1, c
 
 /* out[i][c] = x[i][c] * scale[i] */
 int rwk_row_scale(const float *x, const float *scale, int64_t n, int64_t d, float *out, rwk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Layer norm over the last dimension (the per-row counterpart of the head's batch norm, model.py:68).
+ * type: RWK_F32, RWK_F16 or RWK_BF16; weight_type: the same, or RWK_F32 for weights kept in fp32.
+ * ------------------------------------------------------------------------------------- */
+
+/* y (rows, width) contiguous = (x - mean) * rstd * weight + bias; x has rows x_stride >= width elements apart, bias
+ * may be NULL.  mean and rstd (rows, float32) are written when both are given (the backward pass needs them). */
+int rwk_layer_norm_forward(const void *x, int64_t x_stride, const void *weight, const void *bias, int64_t rows,
+                           int64_t width, int32_t type, int32_t weight_type, float eps, void *y, float *mean,
+                           float *rstd, rwk_stream_t stream);
+
+/* Rows of `partials` (float32, 2 * width each) that rwk_layer_norm_backward needs. */
+int64_t rwk_layer_norm_backward_blocks(int64_t rows, int64_t width, int32_t type);
+
+/* dx (rows, width) contiguous, dw and db (width, of weight_type; db may be NULL) from dy (rows dy_stride apart) and
+ * what the forward pass left.  Sums run in a fixed order. */
+int rwk_layer_norm_backward(const void *x, int64_t x_stride, const void *dy, int64_t dy_stride, const void *weight,
+                            const float *mean, const float *rstd, int64_t rows, int64_t width, int32_t type,
+                            int32_t weight_type, void *dx, float *partials, void *dw, void *db, rwk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * AdamW over many tensors in one launch (the optimiser step of main.py:79,87 with decoupled weight decay).
+ * ------------------------------------------------------------------------------------- */
+#define RWK_ADAMW_TENSORS 256   /* gradients of one launch */
+
+/* One parameter tensor; the table of them lies on the device.  32-bit states: exp_avg and exp_avg_sq are float32 of
+ * n elements, the scales are unused.  8-bit states: float8 (e4m3) values, padded to a multiple of 256 and 4-byte
+ * aligned, with one float32 scale per 256 consecutive elements; a moment is value * scale.  id_offset is added to
+ * the tensor's place in the table to name its random stream. */
+typedef struct {
+    void *param;
+    void *exp_avg;
+    void *exp_avg_sq;
+    float *exp_avg_scale;
+    float *exp_avg_sq_scale;
+    int64_t n;
+    int64_t id_offset;
+} rwk_adamw_tensor;
+
+/* Elements [start, start + rwk_adamw_chunk_size()) of a tensor, as far as it reaches. */
+typedef struct {
+    int64_t tensor;
+    int64_t start;
+} rwk_adamw_chunk;
+
+int64_t rwk_adamw_chunk_size(void);
+
+/* One step of the tensors [tensor_base, tensor_base + n_grads) of `tensors`, whose n_chunks chunks `chunks` lists.
+ * grads (host): one device address per tensor, NULL = the tensor is left as it is.  Parameters and gradients are of
+ * `type`, states of state_bits (8 or 32).  lr: float64[1] on the device.  chunk_steps (int64, n_chunks, device): the
+ * steps taken so far per chunk, advanced here.  seed: key of the 8-bit states' rounding bits. */
+int rwk_adamw_step(const rwk_adamw_tensor *tensors, const rwk_adamw_chunk *chunks, int64_t n_chunks,
+                   int64_t tensor_base, const void *const *grads, int64_t n_grads, int32_t type, int32_t state_bits,
+                   const double *lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
+                   int64_t *chunk_steps, rwk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention inside packed segments (the graphs of a block-diagonal batch, walks or prompts laid end to end), causal or
+ * not, with query heads sharing key / value heads and an optional learned bias per head and bucket of a pair: the
+ * trainable form of the distance-biased walk operator (rwgnn_dis_bias6.py:222-250).
+ *
+ *   s_ij = scale * q_i . k_j (+ table[h][code_ij]),  i, j of one segment, j <= i if causal, code_ij < n_buckets
+ *   out_i = sum_j softmax_j(s_ij) v_j;  a row without pairs gives zeros and takes no gradient
+ * ------------------------------------------------------------------------------------- */
+
+/* Element strides count elements; the elements of a head are adjacent.  out, dq (rows, heads, dim) and dk, dv
+ * (rows, kv_heads, dim) are contiguous.  Rows behind the last segment are neither read nor written. */
+typedef struct {
+    const void *q, *k, *v;          /* (rows, heads, dim), (rows, kv_heads, dim) */
+    void *out;
+    const void *d_out;              /* backward only, as are dq, dk, dv, delta, d_table, d_table_partials */
+    void *dq, *dk, *dv;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
+    const int32_t *seg_ptr;         /* n_segments + 1 first rows */
+    int64_t n_segments, rows;
+    int64_t heads, kv_heads, dim;   /* heads a multiple of kv_heads, dim 1 .. 128 */
+    float scale;                    /* positive */
+    int32_t causal;
+    int32_t type;                   /* RWK_F32, RWK_F16, RWK_BF16 */
+    int32_t block_rows;             /* rows of a block: 32 or 128 */
+    float *stats;                   /* (heads, rows, 2): row maximum and 1 / sum; NULL if no backward pass follows */
+    float *delta;                   /* (heads, rows), written by the backward pass */
+    const uint8_t *codes;           /* rwk_pair_buckets_*; NULL without a bias */
+    const int64_t *code_start;      /* first byte of every segment's codes */
+    const void *table;              /* (heads, n_buckets) of `type` */
+    int64_t n_buckets;              /* 0 without a bias, else 1 .. 32 */
+    void *d_table;                  /* (heads, n_buckets) of `type` */
+    float *d_table_partials;        /* (heads, n_buckets, n_items) */
+    /* blocks of block_rows rows, (segment, first row inside it) pairs of int32, together covering every row of every
+     * segment once; the order decides only which block starts first */
+    const int32_t *q_items, *k_items;
+    int64_t n_items;
+} rwk_attention;
+
+int rwk_attention_forward(const rwk_attention *a, rwk_stream_t stream);
+int rwk_attention_backward(const rwk_attention *a, rwk_stream_t stream);
+
+/* Bucket codes of all ordered pairs (query row, key row) of every segment, as rwk_attention reads them: a segment of
+ * n rows has n rows of codes, each padded to a multiple of 32 with 255 (a code that never attends), from byte
+ * code_start[g].  From a dense list (segment after segment, n * n codes each, from byte pair_start[g]), ... */
+int rwk_pair_buckets_dense(const uint8_t *dense, const int64_t *pair_start, const int32_t *seg_ptr,
+                           const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
+                           rwk_stream_t stream);
+/* ... from the difference j - i of the rows' places, clamped to [-reach, reach], through a table of 2 * reach + 1
+ * codes, ... */
+int rwk_pair_buckets_relative(const uint8_t *by_offset, int64_t reach, const int32_t *seg_ptr,
+                              const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
+                              rwk_stream_t stream);
+/* ... or from hop distances as rwk_khop_fill lists them: 0 for a row itself, the distance for the pairs listed,
+ * far_code for the others. */
+int rwk_pair_buckets_hops(const int32_t *row_start, const int32_t *col, const int32_t *dist, int32_t far_code,
+                          const int32_t *seg_ptr, const int64_t *code_start, int64_t n_segments, int64_t rows,
+                          uint8_t *codes, rwk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,300 @@
+"""``gnn_amd.AdamW`` against the formula in 64 bits (32-bit states) and, for the 8-bit states, against their definition
+written out in numpy: every code and scale has to be equal, so a test that plants other rounding would fail."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+E24 = 2.0 ** -24
+HYPER = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.02)
+# chunk borders (4096 elements), block borders (256), vector borders (4), single elements
+SIZES = [1, 3, 4, 255, 256, 257, 1023, 4095, 4096, 4097, 9001]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    return torch.device("cuda:0")
+
+
+def make(dev, dtype, sizes, seed=0):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    params = [torch.nn.Parameter(torch.randn(n, generator=g, device=dev).to(dtype)) for n in sizes]
+    grads = [[(torch.randn(n, generator=g, device=dev) * 10.0 ** (i % 4 - 2)).to(dtype) for i, n in enumerate(sizes)]
+             for _ in range(4)]
+    return params, grads
+
+
+def formula(p, g, m, v, t, hyper):
+    """One step in 64 bits."""
+    b1, b2 = hyper["betas"]
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    up = hyper["lr"] * (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + hyper["eps"])
+    return p * (1 - hyper["lr"] * hyper["weight_decay"]) - up, m, v, up
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_32_bit_states_follow_the_formula(dev, dtype):
+    """Per step from the kernel's own state: p, m and v each within their roundings - m and v three fp32 operations
+    each, p the type's half step and a dozen fp32 operations on the update."""
+    from gnn_amd import AdamW
+    params, grads = make(dev, dtype, SIZES)
+    opt = AdamW(params, **HYPER)
+    u = torch.finfo(dtype).eps / 2
+    for t, gs in enumerate(grads, 1):
+        before = [(p.detach().double().clone(), opt.state[p]["exp_avg"].double().clone(),
+                   opt.state[p]["exp_avg_sq"].double().clone()) for p in params]
+        for p, g in zip(params, gs):
+            p.grad = g
+        opt.step()
+        for p, g, (p0, m0, v0) in zip(params, gs, before):
+            g = g.double()
+            want, m, v, up = formula(p0, g, m0, v0, t, HYPER)
+            got_m, got_v = opt.state[p]["exp_avg"].double(), opt.state[p]["exp_avg_sq"].double()
+            assert ((got_m - m).abs() <= E24 * 4 * (m0.abs() + g.abs())).all()
+            assert ((got_v - v).abs() <= E24 * 5 * v).all()
+            bound = u * want.abs() + E24 * 4 * p0.abs() + E24 * 24 * up.abs() \
+                + HYPER["lr"] * E24 * 8 * (m0.abs() + g.abs()) / (torch.sqrt(v) + 1e-8) + torch.finfo(dtype).tiny
+            assert ((p.detach().double() - want).abs() <= bound * (1 + u)).all()
+    assert float(opt.state_dict()["state"][0]["step"]) == 4
+
+
+# --- 8-bit states: the definition in numpy ------------------------------------------------------------------------
+def philox(n, tensor, step, seed):
+    c = [np.arange(-(-n // 4), dtype=np.uint64), np.uint64(tensor), np.uint64(step), np.uint64(0)]
+    c = [np.broadcast_to(x, c[0].shape).copy() for x in c]
+    k0, k1 = seed & 0xFFFFFFFF, seed >> 32
+    low = np.uint64(0xFFFFFFFF)
+    for _ in range(7):
+        p0, p1 = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = [(p1 >> np.uint64(32)) ^ c[1] ^ np.uint64(k0), p1 & low, (p0 >> np.uint64(32)) ^ c[3] ^ np.uint64(k1), p0 & low]
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    return np.stack(c, 1).reshape(-1)[:n].astype(np.uint32)
+
+
+def encode(x, bits, positive):
+    """fp32 values in blocks of 256 -> (codes, scales), each operation rounded to fp32."""
+    n = x.size
+    f = np.float32
+    blocks = np.zeros(-(-n // 256) * 256, f)
+    blocks[:n] = np.abs(x)
+    blocks = blocks.reshape(-1, 256)
+    scale = blocks.max(1) * (f(1) / f(448))
+    scale[scale < np.finfo(f).tiny] = 0
+    with np.errstate(divide="ignore"):
+        inverse = np.where(scale == 0, f(0), f(1) / scale)
+    y = np.minimum(blocks * inverse[:, None], f(448)).reshape(-1)[:n]
+    add = bits.astype(np.int64) << 4
+    normal = ((y.view(np.uint32).astype(np.int64) + add) >> 20) - (120 << 3)
+    small = ((y.astype(np.float64) * 2.0 ** 29).astype(np.int64) + add) >> 20
+    code = np.where(y >= 2.0 ** -6, normal, small)
+    if positive:
+        code = np.where((code == 0) & (x > 0), 1, code)
+    return (code | (np.signbit(x).astype(np.int64) << 7)).astype(np.uint8), scale
+
+
+def decode(codes, scale):
+    value = torch.from_numpy(codes.copy()).view(torch.float8_e4m3fn).float().numpy()
+    return value * np.repeat(scale, 256)[:codes.size]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_8_bit_states_are_the_defined_numbers(dev, dtype):
+    from gnn_amd import AdamW
+    params, grads = make(dev, dtype, SIZES, seed=1)
+    seed = (7 << 32) + 12345
+    opt = AdamW(params, state_bits=8, seed=seed, **HYPER)
+    b1, b2 = HYPER["betas"]
+    f = np.float32
+    state = [[np.zeros(n, np.uint8), np.zeros(-(-n // 256), f), np.zeros(n, np.uint8), np.zeros(-(-n // 256), f)]
+             for n in SIZES]
+    u = torch.finfo(dtype).eps / 2
+    for t, gs in enumerate(grads, 1):
+        before = [p.detach().double().clone() for p in params]
+        for p, g in zip(params, gs):
+            p.grad = g
+        opt.step()
+        for i, (p, g, s) in enumerate(zip(params, gs, state)):
+            gn = g.float().cpu().numpy()
+            m = decode(s[0], s[1]) * f(b1) + gn * f(1 - b1)
+            v = decode(s[2], s[3]) * f(b2) + (gn * f(1 - b2)) * gn
+            bits = philox(gn.size, i, t, seed)
+            s[0], s[1] = encode(m, bits & 0xFFFF, False)
+            s[2], s[3] = encode(v, bits >> 16, True)
+            st = opt.state[p]
+            for name, mine in zip(("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"), s):
+                theirs = st[name].view(torch.uint8) if st[name].dtype == torch.float8_e4m3fn else st[name]
+                assert np.array_equal(theirs.cpu().numpy(), mine), (name, gn.size, t)
+            md, vd = (torch.from_numpy(z).double().to(dev) for z in (m, v))
+            c1, c2 = 1 - b1 ** t, 1 - b2 ** t
+            up = HYPER["lr"] * (md / c1) / (torch.sqrt(vd / c2) + HYPER["eps"])
+            want = before[i] * (1 - HYPER["lr"] * HYPER["weight_decay"]) - up
+            bound = u * want.abs() + E24 * (4 * before[i].abs() + 24 * up.abs()) + torch.finfo(dtype).tiny
+            assert ((p.detach().double() - want).abs() <= bound * (1 + u)).all()
+
+
+def test_8_bit_second_moment_keeps_moving(dev):
+    """v of a gradient whose size drops a hundredfold follows the fp32 state down: its mean over many elements stays
+    within the noise of the rounding (an eighth per value at most, averaged over 2^14 of them), where rounding to
+    nearest would leave it where it was; and no positive v becomes zero."""
+    from gnn_amd import AdamW
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    n = 1 << 14
+    p8, p32 = (torch.nn.Parameter(torch.zeros(n, device=dev)) for _ in range(2))
+    o8, o32 = AdamW([p8], state_bits=8, betas=(0.9, 0.999)), AdamW([p32], betas=(0.9, 0.999))
+    for t in range(1500):
+        grad = torch.randn(n, generator=g, device=dev) * (1.0 if t < 500 else 0.01)
+        p8.grad = p32.grad = grad
+        o8.step()
+        o32.step()
+    st = o8.state[p8]
+    v8 = st["exp_avg_sq"].float() * st["exp_avg_sq_scale"].repeat_interleave(256)
+    v32 = o32.state[p32]["exp_avg_sq"]
+    assert (st["exp_avg_sq"].float() > 0).all()
+    # standard deviation of one value: about a quarter; of the mean: 0.25 / 128; five of them
+    assert abs(float(v8.mean() / v32.mean()) - 1) < 0.01
+    rms = float((p8 - p32).detach().square().mean().sqrt() / p32.detach().square().mean().sqrt())
+    assert rms < 0.25
+
+
+def test_zero_gradients_tiny_and_not_finite_values(dev):
+    from gnn_amd import AdamW
+    for bits in (8, 32):
+        p = torch.nn.Parameter(torch.ones(1024, device=dev))
+        opt = AdamW([p], lr=0.1, weight_decay=0.0, state_bits=bits)
+        p.grad = torch.zeros(1024, device=dev)
+        opt.step()
+        assert torch.equal(p.detach(), torch.ones(1024, device=dev))          # 0 / (0 + eps)
+        p.grad = torch.full((1024,), 1e-30, device=dev)                       # squares below the smallest number
+        opt.step()
+        assert p.isfinite().all()
+        p.grad = torch.zeros(1024, device=dev)
+        p.grad[300], p.grad[700] = float("inf"), float("nan")
+        opt.step()
+        opt.step()
+        bad = ~p.isfinite()
+        if bits == 32:
+            assert bad.nonzero().flatten().tolist() == [300, 700]
+        else:                                                                 # their blocks of 256
+            assert bad[256:768].all() and not bad[:256].any() and not bad[768:].any()
+
+
+def test_none_gradients_groups_and_unaligned_tensors(dev):
+    """Two groups with their own rates, a tensor without gradient at one step (it does not age), tensors that begin at
+    odd elements of a buffer, an empty one, more tensors than one launch holds; types mixed in a group."""
+    from gnn_amd import AdamW
+    base = torch.randn(30000, device=dev)
+    at, ps = 1, []
+    for i in range(300):
+        n = 1 + (37 * i) % 91
+        ps.append(torch.nn.Parameter(base[at:at + n]))
+        at += n
+    ps += [torch.nn.Parameter(torch.randn(513, device=dev).bfloat16()), torch.nn.Parameter(torch.empty(0, device=dev))]
+    ref = [torch.nn.Parameter(p.detach().double()) for p in ps]
+    groups = lambda q: [dict(params=q[:150], lr=1e-2), dict(params=q[150:], lr=3e-3, betas=(0.8, 0.95), weight_decay=0.1)]
+    mine, theirs = AdamW(groups(ps)), torch.optim.AdamW(groups(ref), foreach=False)
+    for t in range(3):
+        for i, (p, r) in enumerate(zip(ps, ref)):
+            skip = t == 1 and i % 7 == 0
+            p.grad = None if skip else torch.randn_like(p)
+            r.grad = None if skip else p.grad.double()
+        if t == 2:
+            for o in (mine, theirs):
+                o.param_groups[0]["lr"] = 5e-3
+        mine.step()
+        theirs.step()
+    for i, (p, r) in enumerate(zip(ps, ref)):
+        # three steps: the type's half step each, and fp32 arithmetic on updates of at most a few rates
+        tol = 3 * torch.finfo(p.dtype).eps / 2 * 4 + 1e-6
+        assert ((p.detach().double() - r.detach()).abs() <= tol * (1 + r.detach().abs())).all(), i
+    saved = mine.state_dict()["state"]
+    assert float(saved[0]["step"]) == 2 and float(saved[1]["step"]) == 3
+    rest = base[at:].clone()
+    mine.step()
+    assert torch.equal(base[at:], rest)                                       # nothing behind the last tensor
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint_continues_bit_for_bit(dev, bits):
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.bfloat16, [700, 33], seed=5)
+
+    def go(opt, ps, gs):
+        for p, g in zip(ps, gs):
+            p.grad = g
+        opt.step()
+    opt = AdamW(params, state_bits=bits, seed=9, **HYPER)
+    for gs in grads[:2]:
+        go(opt, params, gs)
+    saved, weights = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in params]
+    for gs in grads[2:]:
+        go(opt, params, gs)
+    fresh = [torch.nn.Parameter(w) for w in weights]
+    other = AdamW(fresh, state_bits=bits, seed=9)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["lr"] == HYPER["lr"]
+    for gs in grads[2:]:
+        go(other, fresh, gs)
+    for a, b in zip(params, fresh):
+        assert torch.equal(a, b)
+        for name, t in opt.state[a].items():
+            if name != "step":
+                assert torch.equal(t.view(torch.uint8) if t.dtype.itemsize == 1 else t,
+                                   other.state[b][name].view(torch.uint8) if t.dtype.itemsize == 1 else other.state[b][name])
+    assert all(t["exp_avg"].dtype == (torch.float8_e4m3fn if bits == 8 else torch.float32)
+               for t in other.state_dict()["state"].values())
+    with pytest.raises(ValueError):
+        AdamW(fresh, state_bits=40 - bits).load_state_dict(saved)
+
+
+def test_captured_step_replays_with_a_new_rate(dev):
+    from gnn_amd import AdamW
+    for bits in (8, 32):
+        params, grads = make(dev, torch.float32, [5000, 77], seed=6)
+        twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        a, b = AdamW(params, state_bits=bits, seed=2), AdamW(twin, state_bits=bits, seed=2)
+        for q in (params, twin):
+            for p, g in zip(q, grads[0]):
+                p.grad = g.clone()
+        a.step()                                                 # tables; the capture needs them
+        b.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a.step()
+        for k in range(4):
+            if k == 2:
+                for o in (a, b):
+                    o.param_groups[0]["lr"] = 4e-4
+                a.push_lr()
+            for q in (params, twin):
+                for p, g in zip(q, grads[k % 4]):
+                    p.grad.copy_(g)
+            graph.replay()
+            torch.cuda.synchronize()
+            b.step()
+            for p, q in zip(params, twin):
+                assert torch.equal(p, q), (bits, k)
+        assert float(a.state_dict()["state"][0]["step"]) == 5
+
+
+def test_parameters_that_move_and_strided_gradients(dev):
+    from gnn_amd import AdamW
+    p = torch.nn.Parameter(torch.randn(40, 30, device=dev))
+    q = torch.nn.Parameter(p.detach().clone())
+    a, b = AdamW([p]), AdamW([q])
+    for t in range(3):
+        g = torch.randn(30, 40, device=dev)
+        p.grad, q.grad = g.t(), g.t().contiguous()
+        a.step()
+        b.step()
+        if t == 0:
+            p.data = p.data.clone()                              # another address: the tables follow
+    assert torch.equal(p, q) and float(a.state_dict()["state"][0]["step"]) == 3
