@@ -64,14 +64,17 @@ __device__ inline Frag<T> pack(const float (&x)[16], int s) {
 // row (of the transposed index) that register i of lane half h holds in a 32x32 result
 __device__ inline int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// D elements padded to KS * 16 for the first product's sum and to DT * 32 rows of the second's result
+// D elements padded to KS * 16 for the first product's sum and to DT * 32 rows of the second's result.  The second
+// product of KS = 1 reads past a row's 16 elements into the next: rows of the result that nobody stores.
 template <typename T, int KS>
 struct Shape {
     static constexpr int DT = (KS + 1) / 2;
-    static constexpr int W = 32 * DT;                             // elements of a row in LDS
+    static constexpr int W = 16 * KS;                             // elements of a row in LDS
     static constexpr int E = 16 / (int)sizeof(T);                 // elements of a chunk
-    static constexpr int C = W / E;                               // chunks of a row: 4, 8, 16 or 32
-    __device__ static int swizzle(int row) { return C == 4 ? (row >> 1) & 3 : row & (C - 1); }
+    static constexpr int C = W / E;                               // chunks of a row: a power of two, 2 .. 32
+    __device__ static int swizzle(int row) {
+        return C == 2 ? (row >> 2) & 1 : C == 4 ? (row >> 1) & 3 : row & (C - 1);
+    }
     // place of chunk c of a row
     __device__ static int at(int row, int c) { return row * W + ((c ^ swizzle(row)) * E); }
 };
@@ -98,31 +101,102 @@ __device__ inline Frag<T> load_global(const T *row, int first, int dim) {
     return f;
 }
 
-// ROWS rows from `first` of a (rows, dim) matrix into LDS; rows from `rows` on and elements from `dim` on are zeros
-template <typename T, int KS, int ROWS, int NT>
-__device__ inline void load_tile(const T *base, long long stride, int first, int rows, int dim, T *lds) {
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ inline uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+
+// ROWS rows at a time of a (rows, dim) matrix of a segment into LDS; rows from `rows` on and elements from `dim` on are
+// zeros.  issue() starts the tile that begins at row `first`, commit() finishes it; in between, the workgroup computes
+// on the other buffer.
+//   ASYNC: the loads write LDS by themselves, 16 bytes a lane, and the buffer's bounds give the zeros; finish() waits.
+//     Written as asm: for the builtin the compiler waits for all of them before any read of LDS.
+//   otherwise (elements that are not whole 16-byte chunks, or unaligned rows): through registers, element by element
+//     where a chunk is not whole.
+template <typename T, int KS, int ROWS, int NT, bool ASYNC>
+struct TileLoader {
     using S = Shape<T, KS>;
+    static constexpr int N = (ROWS * S::C + NT - 1) / NT;
+    typedef typename RwkPack<T, S::E>::type Chunk;
+    const T *base;
+    long long stride;
+    int rows, dim;
+    uint32_t offset[ASYNC ? N : 1];
+    Chunk held[ASYNC ? 1 : N];
+
+    __device__ TileLoader(const T *base_, long long stride_, int rows_, int dim_)
+        : base(base_), stride(stride_), rows(rows_), dim(dim_) {
+        if constexpr (ASYNC) {
 #pragma unroll
-    for (int i = 0; i < (ROWS * S::C + NT - 1) / NT; ++i) {
-        const int k = (int)threadIdx.x + i * NT;
-        if (ROWS * S::C % NT != 0 && k >= ROWS * S::C) break;
-        const int row = k / S::C, c = k % S::C;
-        typename RwkPack<T, S::E>::type v;
-#pragma unroll
-        for (int e = 0; e < S::E; ++e) v[e] = (T)0.f;
-        if (first + row < rows) {
-            const T *p = base + (long long)(first + row) * stride + c * S::E;
-            if ((c + 1) * S::E <= dim) {
-                v = rwk_load<T, S::E>(p);
-            } else {
-#pragma unroll
-                for (int e = 0; e < S::E; ++e)
-                    if (c * S::E + e < dim) v[e] = p[e];
+            for (int i = 0; i < N; ++i) {
+                const int k = (int)threadIdx.x + i * NT, row = k / S::C, c = (k % S::C) ^ S::swizzle(row);
+                // a chunk behind the row's elements: an offset that no buffer reaches
+                offset[i] = c * S::E < dim ? (uint32_t)(row * (int)stride * (int)sizeof(T) + c * 16) : 0xFFFFFF00u;
             }
         }
-        *reinterpret_cast<typename RwkPack<T, S::E>::type *>(lds + S::at(row, c)) = v;
     }
+
+    __device__ void issue(int first, T *lds) {
+        if constexpr (ASYNC) {
+            const uint64_t at = (uint64_t)(base + (long long)first * stride);
+            const int left = min(rows - first, ROWS);
+            i32x4 rsrc;
+            rsrc[0] = __builtin_amdgcn_readfirstlane((int)at);
+            rsrc[1] = __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xFFFFu));
+            rsrc[2] = __builtin_amdgcn_readfirstlane(
+                left > 0 ? ((left - 1) * (int)stride + dim) * (int)sizeof(T) : 0);
+            rsrc[3] = 0x00027000;
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (threadIdx.x & ~63u) * 16);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (ROWS * S::C % NT != 0 && (int)(threadIdx.x & ~63u) + i * NT >= ROWS * S::C) break;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                             :
+                             : "s"(to + i * NT * 16), "v"(offset[i]), "s"(rsrc)
+                             : "memory");          // m0 is set right before every use by the compiler too
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int k = (int)threadIdx.x + i * NT, row = k / S::C, c = k % S::C;
+                Chunk v;
+#pragma unroll
+                for (int e = 0; e < S::E; ++e) v[e] = (T)0.f;
+                if (first + row < rows && row < ROWS) {
+                    const T *p = base + (long long)(first + row) * stride + c * S::E;
+                    if ((c + 1) * S::E <= dim) {
+                        v = rwk_load<T, S::E>(p);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < S::E; ++e) v[e] = c * S::E + e < dim ? p[e] : (T)0.f;
+                    }
+                }
+                held[i] = v;
+            }
+        }
+    }
+
+    __device__ void commit(T *lds) {
+        if constexpr (!ASYNC) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int k = (int)threadIdx.x + i * NT, row = k / S::C, c = k % S::C;
+                if (ROWS * S::C % NT != 0 && k >= ROWS * S::C) break;
+                *reinterpret_cast<Chunk *>(lds + S::at(row, c)) = held[i];
+            }
+        }
+    }
+};
+
+// everything this workgroup's loads and writes put into LDS is there, and nobody reads the buffer before it any more
+template <bool ASYNC>
+__device__ inline void tile_ready() {
+    if (ASYNC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
 }
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }     // one instruction
 
 // operand whose 32 rows are rows of the tile and whose summed index is the element: step ks
 template <typename T, int KS>
@@ -242,14 +316,27 @@ __device__ inline void load_table(const RwkAttnArgs &p, int head, float *table) 
         table[b] = b < p.a.n_buckets ? (float)((const T *)p.a.table)[(long long)head * p.a.n_buckets + b] : -INFINITY;
 }
 
-template <typename T, int KS, int NW, bool BIAS>
-__global__ void __launch_bounds__(64 * NW)
+// Bytes of LDS in front of the bias table: two buffers of two tiles, and the elements that the second product of
+// KS = 1 reads past the last row.
+template <typename T, int KS, int ROWS> constexpr int tile_bytes() { return ROWS * 16 * KS * (int)sizeof(T); }
+template <typename T, int KS, int ROWS> constexpr int tiles_bytes() {
+    return 4 * tile_bytes<T, KS, ROWS>() + (KS == 1 ? 32 * (int)sizeof(T) : 0);
+}
+template <typename T, int NW> constexpr int tile_rows() { return sizeof(T) == 2 && NW > 1 ? 64 : 32; }
+
+// Scores below the reference by this much or less (in powers of two) leave it as it is: the sums and the output are
+// rescaled only when a row's maximum has grown by a factor of 2^8 in its exponential, and stay far inside fp32's (and
+// the probabilities inside fp16's) range.
+constexpr float kSlack = 8.f;
+
+template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC ? 2 : 1)
 attention_forward_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
-    constexpr int NT = 64 * NW, DT = S::DT, BN = sizeof(T) == 2 ? 64 : 32, TN = BN / 32;
+    constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
-    T *k_tile = (T *)attn_lds, *v_tile = k_tile + BN * S::W;
-    float *table = (float *)(v_tile + BN * S::W);
+    T *tiles = (T *)attn_lds;                                       // buffer b: keys at 2 b, values at 2 b + 1
+    float *table = (float *)(attn_lds + tiles_bytes<T, KS, BN>());
     const Place at = query_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int q0 = at.first + 32 * (int)(threadIdx.x >> 6), q = q0 + (lane & 31), qc = q < n ? q : n - 1;
@@ -257,92 +344,108 @@ attention_forward_kernel(const RwkAttnArgs p) {
     const int nb = (int)p.a.n_buckets;
     if (BIAS) load_table<T, NT>(p, at.head, table);
 
+    TileLoader<T, KS, BN, NT, ASYNC> keys((const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head, p.a.k_row, n, dim);
+    TileLoader<T, KS, BN, NT, ASYNC> values((const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head, p.a.v_row, n, dim);
+    keys.issue(0, tiles);
+    values.issue(0, tiles + BN * S::W);
     Frag<T> qf[KS];
     const T *q_row = (const T *)p.a.q + (at.base + qc) * p.a.q_row + at.head * p.a.q_head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = load_global<T>(q_row, 16 * ks + 8 * h, dim);
-    const T *k_base = (const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head;
-    const T *v_base = (const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head;
     const uint8_t *code_row = nullptr;
     if (BIAS) code_row = p.a.codes + p.a.code_start[at.seg] + (long long)qc * ((n + 31) / 32 * 32);
 
     // without a bias the maximum is taken over q . k and the scale meets it in the exponent; with one the scores are
     // the sum, and the difference is formed before the change of base, so that a bias of the type's lowest value
     // stays finite
-    const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
+    const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e, slack = kSlack / c;
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
-    float top = -INFINITY, sum = 0.f;
+    float ref = -INFINITY, sum = 0.f;           // ref: what the exponentials are taken relative to
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
-    for (int k0 = 0; k0 < end; k0 += BN) {
-        __syncthreads();
-        load_tile<T, KS, BN, NT>(k_base, p.a.k_row, k0, n, dim, k_tile);
-        load_tile<T, KS, BN, NT>(v_base, p.a.v_row, k0, n, dim, v_tile);
-        __syncthreads();
-        if (q0 >= n || (causal && k0 > q0 + 31)) continue;
-        float s[TN][16];
-#pragma unroll
-        for (int t = 0; t < TN; ++t) {
-            f32x16 x = f32x16{};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) x = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], x);
-            unpack(x, s[t]);
+    keys.commit(tiles);
+    values.commit(tiles + BN * S::W);
+    for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
+        const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
+        T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
+        tile_ready<ASYNC>();
+        if (k0 + BN < end) {
+            keys.issue(k0 + BN, next);
+            values.issue(k0 + BN, next + BN * S::W);
         }
-        if (BIAS) {
+        if (q0 < n && !(causal && k0 > q0 + 31)) {
+            float s[TN][16];
 #pragma unroll
-            for (int t = 0; t < TN; ++t)
+            for (int t = 0; t < TN; ++t) {
+                f32x16 x = f32x16{};
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    // columns from n on are padded with codes that do not attend
-                    const uint32_t codes = k0 + 32 * t < n
-                        ? *(const uint32_t *)(code_row + k0 + 32 * t + 8 * g + 4 * h) : 0xFFFFFFFFu;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int b = min((int)((codes >> (8 * e)) & 255u), nb);
-                        const float x = fmaf(s[t][4 * g + e], scale, table[b]);
-                        s[t][4 * g + e] = b < nb ? x : -INFINITY;
-                    }
-                }
-        }
-        if (k0 + BN > n || (causal && k0 + BN - 1 > q0)) {
-            const int last = causal ? min(q, n - 1) : n - 1;
-#pragma unroll
-            for (int t = 0; t < TN; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] = k0 + 32 * t + reg_row(i, h) <= last ? s[t][i] : -INFINITY;
-        }
-        float here = s[0][0];
-#pragma unroll
-        for (int t = 0; t < TN; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) here = fmaxf(here, s[t][i]);
-        here = fmaxf(here, __shfl_xor(here, 32, 64));
-        const float now = fmaxf(top, here), ref = now == -INFINITY ? 0.f : now;
-        const float shrink = exp2f((top - ref) * c);
-        top = now;
-        float part = 0.f;
-#pragma unroll
-        for (int t = 0; t < TN; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2f(BIAS ? (s[t][i] - ref) * c : fmaf(s[t][i], c, -ref * c));
-                part += s[t][i];
+                for (int ks = 0; ks < KS; ++ks)
+                    x = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], x);
+                unpack(x, s[t]);
             }
-        sum = fmaf(sum, shrink, part);
+            if (BIAS) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+                for (int t = 0; t < TN; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
+                    for (int g = 0; g < 4; ++g) {
+                        // columns from n on are padded with codes that do not attend
+                        const uint32_t codes = k0 + 32 * t < n
+                            ? *(const uint32_t *)(code_row + k0 + 32 * t + 8 * g + 4 * h) : 0xFFFFFFFFu;
 #pragma unroll
-        for (int t = 0; t < TN; ++t)
+                        for (int e = 0; e < 4; ++e) {
+                            const int b = min((int)((codes >> (8 * e)) & 255u), nb);
+                            const float x = fmaf(s[t][4 * g + e], scale, table[b]);
+                            s[t][4 * g + e] = b < nb ? x : -INFINITY;
+                        }
+                    }
+            }
+            if (k0 + BN > n || (causal && k0 + BN - 1 > q0)) {
+                const int last = causal ? min(q, n - 1) : n - 1;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Frag<T> pf = pack<T>(s[t], u);
+                for (int t = 0; t < TN; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[t][i] = k0 + 32 * t + reg_row(i, h) <= last ? s[t][i] : -INFINITY;
+            }
+            float here = s[0][0];
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) here = fmaxf(here, s[t][i]);
+            here = fmaxf(here, __shfl_xor(here, 32, 64));
+            const bool grown = here > ref + slack || (ref == -INFINITY && here > -INFINITY);
+            if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+                const float now = grown ? here : ref;
+                const float shrink = ref == now ? 1.f : exp2_fast((ref - now) * c);
+                ref = now;
+                sum *= shrink;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = mma(column_operand<T, KS>(v_tile, 32 * t + 16 * u, dt, lane), pf, acc[dt]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
             }
+            const float base = ref == -INFINITY ? 0.f : ref, base_c = base * c;
+            float part = 0.f;
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[t][i] = exp2_fast(BIAS ? (s[t][i] - base) * c : fmaf(s[t][i], c, -base_c));
+                    part += s[t][i];
+                }
+            sum += part;
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> pf = pack<T>(s[t], u);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        acc[dt] = mma(column_operand<T, KS>(v_tile, 32 * t + 16 * u, dt, lane), pf, acc[dt]);
+                }
+        }
+        keys.commit(next);
+        values.commit(next + BN * S::W);
     }
     if (q >= n) return;
     sum += __shfl_xor(sum, 32, 64);
@@ -350,19 +453,19 @@ attention_forward_kernel(const RwkAttnArgs p) {
     store_rows<T, DT>((T *)p.a.out + ((at.base + q) * p.a.heads + at.head) * dim, dim, h, acc, inv);
     if (p.a.stats != nullptr && h == 0) {
         float *st = p.a.stats + 2 * (at.head * p.a.rows + at.base + q);
-        st[0] = top == -INFINITY ? 0.f : top;
+        st[0] = ref == -INFINITY ? 0.f : ref;
         st[1] = inv;
     }
 }
 
-template <typename T, int KS, int NW, bool BIAS>
-__global__ void __launch_bounds__(64 * NW)
+template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && !BIAS ? 2 : 1)
 attention_dq_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
-    constexpr int NT = 64 * NW, DT = S::DT, BN = sizeof(T) == 2 ? 64 : 32, TN = BN / 32;
+    constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
-    T *k_tile = (T *)attn_lds, *v_tile = k_tile + BN * S::W;
-    float *table = (float *)(v_tile + BN * S::W), *hist = table + 64;
+    T *tiles = (T *)attn_lds;
+    float *table = (float *)(attn_lds + tiles_bytes<T, KS, BN>()), *hist = table + 64;
     const Place at = query_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int q0 = at.first + 32 * (int)(threadIdx.x >> 6), q = q0 + (lane & 31), qc = q < n ? q : n - 1;
@@ -373,6 +476,10 @@ attention_dq_kernel(const RwkAttnArgs p) {
         for (int b = 0; b <= nb; ++b) hist[b * NT + threadIdx.x] = 0.f;    // a thread's own sums
     }
 
+    TileLoader<T, KS, BN, NT, ASYNC> keys((const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head, p.a.k_row, n, dim);
+    TileLoader<T, KS, BN, NT, ASYNC> values((const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head, p.a.v_row, n, dim);
+    keys.issue(0, tiles);
+    values.issue(0, tiles + BN * S::W);
     Frag<T> qf[KS], of[KS];
     const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
     const T *q_row = (const T *)p.a.q + (at.base + qc) * p.a.q_row + at.head * p.a.q_head;
@@ -390,8 +497,6 @@ attention_dq_kernel(const RwkAttnArgs p) {
     const long long row_at = at.head * p.a.rows + at.base + qc;
     if (q < n && h == 0) p.a.delta[row_at] = delta;
     const float ref = p.a.stats[2 * row_at], inv = p.a.stats[2 * row_at + 1];
-    const T *k_base = (const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head;
-    const T *v_base = (const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head;
     const uint8_t *code_row = nullptr;
     if (BIAS) code_row = p.a.codes + p.a.code_start[at.seg] + (long long)qc * ((n + 31) / 32 * 32);
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
@@ -400,17 +505,27 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
-    for (int k0 = 0; k0 < end; k0 += BN) {
-        __syncthreads();
-        load_tile<T, KS, BN, NT>(k_base, p.a.k_row, k0, n, dim, k_tile);
-        load_tile<T, KS, BN, NT>(v_base, p.a.v_row, k0, n, dim, v_tile);
-        __syncthreads();
-        if (q0 >= n) continue;
+    keys.commit(tiles);
+    values.commit(tiles + BN * S::W);
+    for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
+        const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
+        T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
+        tile_ready<ASYNC>();
+        if (k0 + BN < end) {
+            keys.issue(k0 + BN, next);
+            values.issue(k0 + BN, next + BN * S::W);
+        }
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
             const int kt = k0 + 32 * t;
-            if (kt >= n || (causal && kt > q0 + 31)) break;
-            f32x16 sx = f32x16{}, dx = f32x16{};
+            if (q0 >= n || kt >= n || (causal && kt > q0 + 31)) break;
+            // the products begin at minus the row's reference and minus its delta
+            f32x16 sx, dx;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sx[i] = BIAS ? 0.f : -ref;
+                dx[i] = -delta;
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 sx = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], sx);
@@ -427,23 +542,21 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int b = min((int)((codes[g] >> (8 * e)) & 255u), nb);
-                        const float x = fmaf(s[4 * g + e], scale, table[b]);
+                        const float x = fmaf(s[4 * g + e], scale, table[b]) - ref;
                         s[4 * g + e] = b < nb ? x : -INFINITY;
                     }
                 }
             }
-            const bool masked = kt + 32 > n || (causal && kt + 31 > q0);
-            if (masked) {
+            if (BIAS || kt + 32 > n || (causal && kt + 31 > q0)) {
                 const int last = causal ? min(q, n - 1) : n - 1;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
+                    d[i] = s[i] > -INFINITY ? d[i] : 0.f;        // a masked pair's value may be anything
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool off = (BIAS || masked) && s[i] == -INFINITY;
-                const float pr = exp2f(BIAS ? (s[i] - ref) * c : fmaf(s[i], c, -ref * c)) * inv;
-                s[i] = off ? 0.f : pr * (d[i] - delta);      // a masked pair's value may be anything
-            }
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] * c) * inv * d[i];
             if (BIAS) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -459,6 +572,8 @@ attention_dq_kernel(const RwkAttnArgs p) {
                     acc[dt] = mma(column_operand<T, KS>(k_tile, 32 * t + 16 * u, dt, lane), sf, acc[dt]);
             }
         }
+        keys.commit(next);
+        values.commit(next + BN * S::W);
     }
     if (q < n) store_rows<T, DT>((T *)p.a.dq + o_at, dim, h, acc, scale);
     if (BIAS) {
@@ -474,99 +589,172 @@ attention_dq_kernel(const RwkAttnArgs p) {
     }
 }
 
-template <typename T, int KS, int NW, bool BIAS>
-__global__ void __launch_bounds__(64 * NW)
+// KB blocks of 32 keys per wavefront: with two, every operand read from LDS meets two products.
+template <typename T, int KS, int NW, int KB, bool BIAS, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, 1)
 attention_dkv_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
-    constexpr int NT = 64 * NW, DT = S::DT, BQ = 32;
+    constexpr int NT = 64 * NW, DT = S::DT, BQ = tile_rows<T, NW>(), TQ = BQ / 32;
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
-    T *q_tile = (T *)attn_lds, *o_tile = q_tile + BQ * S::W;
-    float *st = (float *)(o_tile + BQ * S::W), *table = st + 3 * BQ;       // st: maximum, 1 / sum, delta per row
+    T *tiles = (T *)attn_lds;                                       // buffer b: q at 2 b, d_out at 2 b + 1
+    // per buffer and row: - the reference, 1 / sum, - delta
+    float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>()), *table = stats + 6 * BQ;
     const Place at = key_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
-    const int k0 = at.first + 32 * (int)(threadIdx.x >> 6), k = k0 + (lane & 31), kc = k < n ? k : n - 1;
+    const int k0 = at.first + 32 * KB * (int)(threadIdx.x >> 6);
     const bool causal = p.a.causal != 0;
     const int nb = (int)p.a.n_buckets;
 
-    Frag<T> kf[KS], vf[KS];
-    const T *k_row = (const T *)p.a.k + (at.base + kc) * p.a.k_row + at.kv_head * p.a.k_head;
-    const T *v_row = (const T *)p.a.v + (at.base + kc) * p.a.v_row + at.kv_head * p.a.v_head;
+    Frag<T> kf[KB][KS], vf[KB][KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        kf[ks] = load_global<T>(k_row, 16 * ks + 8 * h, dim);
-        vf[ks] = load_global<T>(v_row, 16 * ks + 8 * h, dim);
+    for (int b = 0; b < KB; ++b) {
+        const int k = min(k0 + 32 * b + (lane & 31), n - 1);
+        const T *k_row = (const T *)p.a.k + (at.base + k) * p.a.k_row + at.kv_head * p.a.k_head;
+        const T *v_row = (const T *)p.a.v + (at.base + k) * p.a.v_row + at.kv_head * p.a.v_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            kf[b][ks] = load_global<T>(k_row, 16 * ks + 8 * h, dim);
+            vf[b][ks] = load_global<T>(v_row, 16 * ks + 8 * h, dim);
+        }
     }
     const long long code_stride = (n + 31) / 32 * 32;
-    const uint8_t *code_col = nullptr;
-    if (BIAS) code_col = p.a.codes + p.a.code_start[at.seg] + kc;
+    const uint8_t *code_at = nullptr;
+    if (BIAS) code_at = p.a.codes + p.a.code_start[at.seg];
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
 
-    f32x16 dk[DT], dv[DT];
+    f32x16 dk[KB][DT], dv[KB][DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dk[b][dt] = dv[b][dt] = f32x16{};
+    const int begin = causal ? at.first : 0;
     for (int g = 0; g < p.group; ++g) {
         const int head = at.head + g;
-        const T *q_base = (const T *)p.a.q + at.base * p.a.q_row + head * p.a.q_head;
-        const T *o_base = (const T *)p.a.d_out + at.base * p.a.do_row + head * p.a.do_head;
         const long long row_at = head * p.a.rows + at.base;
-        if (BIAS) {
-            __syncthreads();
-            load_table<T, NT>(p, head, table);
-        }
-        for (int q0 = causal ? at.first : 0; q0 < n; q0 += BQ) {
-            __syncthreads();
-            load_tile<T, KS, BQ, NT>(q_base, p.a.q_row, q0, n, dim, q_tile);
-            load_tile<T, KS, BQ, NT>(o_base, p.a.do_row, q0, n, dim, o_tile);
+        TileLoader<T, KS, BQ, NT, ASYNC> queries((const T *)p.a.q + at.base * p.a.q_row + head * p.a.q_head, p.a.q_row, n, dim);
+        TileLoader<T, KS, BQ, NT, ASYNC> grads((const T *)p.a.d_out + at.base * p.a.do_row + head * p.a.do_head, p.a.do_row, n, dim);
+        __syncthreads();                          // the head before is done with the buffers and the table
+        if (BIAS) load_table<T, NT>(p, head, table);
+        float held[3];
+        const auto start = [&](int q0, int turn) {
+            queries.issue(q0, tiles + 2 * turn * BQ * S::W);
+            grads.issue(q0, tiles + (2 * turn + 1) * BQ * S::W);
+            const int q = q0 + (int)threadIdx.x;
             if (threadIdx.x < BQ) {
-                const int q = q0 + (int)threadIdx.x;
-                st[threadIdx.x] = q < n ? p.a.stats[2 * (row_at + q)] : 0.f;
-                st[BQ + threadIdx.x] = q < n ? p.a.stats[2 * (row_at + q) + 1] : 0.f;     // rows beyond: p = 0
-                st[2 * BQ + threadIdx.x] = q < n ? p.a.delta[row_at + q] : 0.f;
+                const bool there = q < n;         // rows beyond: p = 0
+                held[0] = there ? -p.a.stats[2 * (row_at + q)] : 0.f;
+                held[1] = there ? p.a.stats[2 * (row_at + q) + 1] : 0.f;
+                held[2] = there ? -p.a.delta[row_at + q] : 0.f;
             }
-            __syncthreads();
-            if (k0 >= n || (causal && q0 + BQ - 1 < k0)) continue;
-            f32x16 sx = f32x16{}, dx = f32x16{};
+        };
+        const auto finish = [&](int turn) {
+            queries.commit(tiles + 2 * turn * BQ * S::W);
+            grads.commit(tiles + (2 * turn + 1) * BQ * S::W);
+            if (threadIdx.x < BQ) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                sx = mma(row_operand<T, KS>(q_tile, lane & 31, ks, h), kf[ks], sx);
-                dx = mma(row_operand<T, KS>(o_tile, lane & 31, ks, h), vf[ks], dx);
+                for (int j = 0; j < 3; ++j) stats[(3 * turn + j) * BQ + threadIdx.x] = held[j];
             }
-            float s[16], d[16];
-            unpack(sx, s);
-            unpack(dx, d);
-            const bool masked = causal && q0 < k0 + 31;
+        };
+        start(begin, 0);
+        finish(0);
+        for (int q0 = begin, turn = 0; q0 < n; q0 += BQ, turn ^= 1) {
+            tile_ready<ASYNC>();
+            if (q0 + BQ < n) start(q0 + BQ, turn ^ 1);
+            const T *q_tile = tiles + 2 * turn * BQ * S::W, *o_tile = q_tile + BQ * S::W;
+            const float *st = stats + 3 * turn * BQ;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = reg_row(i, h);
-                const float ref = st[r], inv = st[BQ + r], delta = st[2 * BQ + r];
-                bool off = false;
-                if (BIAS) {
-                    const int b = q0 + r < n ? min((int)code_col[(q0 + r) * code_stride], nb) : nb;
-                    off = b >= nb;
-                    s[i] = fmaf(s[i], scale, table[b]);
+            for (int t = 0; t < TQ; ++t) {
+                const int qt = q0 + 32 * t;
+                if (k0 >= n || qt >= n) break;
+                if (causal && qt + 31 < k0) continue;
+                typedef float f32x4 __attribute__((ext_vector_type(4)));
+                f32x16 sx[KB], dx[KB];
+                float inv[16];
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const f32x4 r = *(const f32x4 *)(st + 32 * t + 8 * g4 + 4 * h);
+                    const f32x4 i = *(const f32x4 *)(st + BQ + 32 * t + 8 * g4 + 4 * h);
+                    const f32x4 d = *(const f32x4 *)(st + 2 * BQ + 32 * t + 8 * g4 + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        inv[4 * g4 + e] = i[e];
+#pragma unroll
+                        for (int b = 0; b < KB; ++b) {
+                            sx[b][4 * g4 + e] = BIAS ? 0.f : r[e];
+                            dx[b][4 * g4 + e] = d[e];
+                        }
+                    }
                 }
-                if (masked) off = off || q0 + r < k;
-                float pr = exp2f(BIAS ? (s[i] - ref) * c : fmaf(s[i], c, -ref * c)) * inv;
-                if (BIAS) off = off || s[i] == -INFINITY;
-                pr = off ? 0.f : pr;
-                d[i] = off ? 0.f : pr * (d[i] - delta);
-                s[i] = pr;
-            }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Frag<T> pf = pack<T>(s, u), sf = pack<T>(d, u);
+                for (int ks = 0; ks < KS; ++ks) {
+                    const Frag<T> qr = row_operand<T, KS>(q_tile, 32 * t + (lane & 31), ks, h);
+                    const Frag<T> gr = row_operand<T, KS>(o_tile, 32 * t + (lane & 31), ks, h);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    dv[dt] = mma(column_operand<T, KS>(o_tile, 16 * u, dt, lane), pf, dv[dt]);
-                    dk[dt] = mma(column_operand<T, KS>(q_tile, 16 * u, dt, lane), sf, dk[dt]);
+                    for (int b = 0; b < KB; ++b) {
+                        sx[b] = mma(qr, kf[b][ks], sx[b]);
+                        dx[b] = mma(gr, vf[b][ks], dx[b]);
+                    }
+                }
+                float s[KB][16], d[KB][16];
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    unpack(sx[b], s[b]);
+                    unpack(dx[b], d[b]);
+                    const int k = k0 + 32 * b + (lane & 31);
+                    if (BIAS) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = qt + reg_row(i, h);
+                            const int code = r < n ? min((int)code_at[r * code_stride + min(k, n - 1)], nb) : nb;
+                            const float x = fmaf(s[b][i], scale, table[code]) + st[32 * t + reg_row(i, h)];
+                            s[b][i] = code < nb ? x : -INFINITY;
+                        }
+                    }
+                    if (BIAS || (causal && qt < k0 + 32 * b + 31)) {
+                        const int least = causal ? k : 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            s[b][i] = qt + reg_row(i, h) >= least ? s[b][i] : -INFINITY;
+                            d[b][i] = s[b][i] > -INFINITY ? d[b][i] : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[b][i] = exp2_fast(s[b][i] * c) * inv[i];
+                        d[b][i] *= s[b][i];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    Frag<T> pf[KB], sf[KB];
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        pf[b] = pack<T>(s[b], u);
+                        sf[b] = pack<T>(d[b], u);
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const Frag<T> gc = column_operand<T, KS>(o_tile, 32 * t + 16 * u, dt, lane);
+                        const Frag<T> qc = column_operand<T, KS>(q_tile, 32 * t + 16 * u, dt, lane);
+#pragma unroll
+                        for (int b = 0; b < KB; ++b) {
+                            dv[b][dt] = mma(gc, pf[b], dv[b][dt]);
+                            dk[b][dt] = mma(qc, sf[b], dk[b][dt]);
+                        }
+                    }
                 }
             }
+            if (q0 + BQ < n) finish(turn ^ 1);
         }
     }
-    if (k >= n) return;
-    const long long to = ((at.base + k) * p.a.kv_heads + at.kv_head) * dim;
-    store_rows<T, DT>((T *)p.a.dk + to, dim, h, dk, scale);
-    store_rows<T, DT>((T *)p.a.dv + to, dim, h, dv, 1.f);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        const int k = k0 + 32 * b + (lane & 31);
+        if (k >= n) continue;
+        const long long to = ((at.base + k) * p.a.kv_heads + at.kv_head) * dim;
+        store_rows<T, DT>((T *)p.a.dk + to, dim, h, dk[b], scale);
+        store_rows<T, DT>((T *)p.a.dv + to, dim, h, dv[b], 1.f);
+    }
 }
 
 template <typename K>
@@ -580,27 +768,48 @@ int launch_kernel(K kernel, long long grid, int threads, size_t lds, const RwkAt
     return RWK_OK;
 }
 
-template <typename T, int KS, int NW, bool BIAS>
+template <typename T, int KS, bool WIDE, bool BIAS, bool ASYNC>
 int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
-    using S = Shape<T, KS>;
-    constexpr int NT = 64 * NW;
-    const size_t row = S::W * sizeof(T), keys = sizeof(T) == 2 ? 64 : 32;
+    constexpr int NW = WIDE ? 4 : 1, NT = 64 * NW, ROWS = tile_rows<T, NW>();
     if (pass == kRwkAttnForward)
-        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS>, p.a.n_items * p.a.heads, NT,
-                             2 * keys * row + 64 * sizeof(float), p, stream);
+        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
+                             tiles_bytes<T, KS, ROWS>() + 64 * sizeof(float), p, stream);
     if (pass == kRwkAttnDq)
-        return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS>, p.a.n_items * p.a.heads, NT,
-                             2 * keys * row + (64 + (BIAS ? (p.a.n_buckets + 1) * NT : 0)) * sizeof(float), p, stream);
-    return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS>, p.a.n_items * p.a.kv_heads, NT,
-                         2 * 32 * row + (3 * 32 + 64) * sizeof(float), p, stream);
+        return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
+                             tiles_bytes<T, KS, ROWS>() + (64 + (BIAS ? (p.a.n_buckets + 1) * NT : 0)) * sizeof(float), p,
+                             stream);
+    // two wavefronts of 64 keys where the registers hold two blocks' keys, values and sums, else four of 32
+    constexpr int KB = WIDE && sizeof(T) == 2 && KS <= 4 ? 2 : 1, KROWS = tile_rows<T, NW / KB>();
+    return launch_kernel(attention_dkv_kernel<T, KS, NW / KB, KB, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT / KB,
+                         tiles_bytes<T, KS, KROWS>() + (6 * KROWS + 64) * sizeof(float), p, stream);
+}
+
+// Rows whose elements are whole 16-byte chunks at 16-byte addresses, not too far apart for 32-bit offsets inside a
+// tile, are loaded straight into LDS.
+template <typename T>
+bool chunked(const RwkAttnArgs &p, bool backward) {
+    const long long e = 16 / (long long)sizeof(T), far = 0x7FFFFFFFll / (64 * (long long)sizeof(T)) - 1;
+    const auto fits = [&](const void *at, long long row, long long head) {
+        return (uintptr_t)at % 16 == 0 && row % e == 0 && head % e == 0 && row >= 0 && row < far;
+    };
+    return p.a.dim % e == 0 && fits(p.a.q, p.a.q_row, p.a.q_head) && fits(p.a.k, p.a.k_row, p.a.k_head) &&
+           fits(p.a.v, p.a.v_row, p.a.v_head) && (!backward || fits(p.a.d_out, p.a.do_row, p.a.do_head));
 }
 
 template <typename T, int KS>
 int launch_width(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
-    const bool bias = p.a.n_buckets > 0;
-    if (p.a.block_rows == 128)
-        return bias ? launch_shape<T, KS, 4, true>(pass, p, stream) : launch_shape<T, KS, 4, false>(pass, p, stream);
-    return bias ? launch_shape<T, KS, 1, true>(pass, p, stream) : launch_shape<T, KS, 1, false>(pass, p, stream);
+    const bool bias = p.a.n_buckets > 0, wide = p.a.block_rows == 128, async = chunked<T>(p, pass != kRwkAttnForward);
+#define RWK_ATTN_CASE(W, B, A) if (wide == W && bias == B && async == A) return launch_shape<T, KS, W, B, A>(pass, p, stream)
+    RWK_ATTN_CASE(true, true, true);
+    RWK_ATTN_CASE(true, true, false);
+    RWK_ATTN_CASE(true, false, true);
+    RWK_ATTN_CASE(true, false, false);
+    RWK_ATTN_CASE(false, true, true);
+    RWK_ATTN_CASE(false, true, false);
+    RWK_ATTN_CASE(false, false, true);
+    RWK_ATTN_CASE(false, false, false);
+#undef RWK_ATTN_CASE
+    return RWK_E_UNSUPPORTED;
 }
 
 template <typename T>
