@@ -72,8 +72,15 @@ struct Shape {
     static constexpr int W = 16 * KS;                             // elements of a row in LDS
     static constexpr int E = 16 / (int)sizeof(T);                 // elements of a chunk
     static constexpr int C = W / E;                               // chunks of a row: a power of two, 2 .. 32
+    // 64 banks of 4 bytes serve 16 lanes of 16 bytes, or 32 of 8, at once.  Row reads: 16 rows at one chunk have to
+    // lie in 16 different places of 256 bytes.  Column reads: 16-bit types four rows of four chunks, fp32 the rows r
+    // and r + 4 of eight chunks each.
     __device__ static int swizzle(int row) {
-        return C == 2 ? (row >> 2) & 1 : C == 4 ? (row >> 1) & 3 : row & (C - 1);
+        if (C == 2) return (row >> 3) & 1;
+        if (C == 4) return (row >> 2) & 3;
+        if (C == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+        if (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+        return ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
     }
     // place of chunk c of a row
     __device__ static int at(int row, int c) { return row * W + ((c ^ swizzle(row)) * E); }
@@ -194,6 +201,26 @@ template <bool ASYNC>
 __device__ inline void tile_ready() {
     if (ASYNC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+}
+
+// Rows and statistics read before the loop are there: without this the compiler waits for them at their first use
+// inside it, and with them for the tiles in flight, again in every round.
+__device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }          // vmcnt(0)
+
+// Order of the LDS reads and products that the compiler has put into one block: AHEAD reads first, then PER reads
+// behind every product.  By itself it reads every operand right before its product and waits.
+template <typename T, int READS, int PRODUCTS, int AHEAD, int PER>
+__device__ inline void interleave() {
+    if constexpr (sizeof(T) == 2) {
+        constexpr int N = (READS - AHEAD + PER - 1) / PER;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - N, 0);
+    }
 }
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }     // one instruction
@@ -366,6 +393,7 @@ attention_forward_kernel(const RwkAttnArgs p) {
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
     keys.commit(tiles);
     values.commit(tiles + BN * S::W);
+    loads_done();
     for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
         const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
         T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
@@ -384,6 +412,7 @@ attention_forward_kernel(const RwkAttnArgs p) {
                     x = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], x);
                 unpack(x, s[t]);
             }
+            interleave<T, TN * KS, TN * KS, TN * KS < 6 ? TN * KS : 6, 1>();
             if (BIAS) {
 #pragma unroll
                 for (int t = 0; t < TN; ++t)
@@ -458,6 +487,10 @@ attention_forward_kernel(const RwkAttnArgs p) {
     }
 }
 
+// What the backward pass adds to a row's scores so that their exponential is the probability: minus the forward
+// pass's reference, and the logarithm of 1 / sum.  -infinity for a row without pairs and for rows that do not exist.
+__device__ inline float reference(float ref, float inv, float c) { return __log2f(inv) / c - ref; }
+
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && !BIAS ? 2 : 1)
 attention_dq_kernel(const RwkAttnArgs p) {
@@ -496,10 +529,10 @@ attention_dq_kernel(const RwkAttnArgs p) {
     delta += __shfl_xor(delta, 32, 64);
     const long long row_at = at.head * p.a.rows + at.base + qc;
     if (q < n && h == 0) p.a.delta[row_at] = delta;
-    const float ref = p.a.stats[2 * row_at], inv = p.a.stats[2 * row_at + 1];
     const uint8_t *code_row = nullptr;
     if (BIAS) code_row = p.a.codes + p.a.code_start[at.seg] + (long long)qc * ((n + 31) / 32 * 32);
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
+    const float ref = reference(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
 
     f32x16 acc[DT];
 #pragma unroll
@@ -507,6 +540,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
     keys.commit(tiles);
     values.commit(tiles + BN * S::W);
+    loads_done();
     for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
         const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
         T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
@@ -519,11 +553,11 @@ attention_dq_kernel(const RwkAttnArgs p) {
         for (int t = 0; t < TN; ++t) {
             const int kt = k0 + 32 * t;
             if (q0 >= n || kt >= n || (causal && kt > q0 + 31)) break;
-            // the products begin at minus the row's reference and minus its delta
+            // the products begin at the row's reference and at minus its delta
             f32x16 sx, dx;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                sx[i] = BIAS ? 0.f : -ref;
+                sx[i] = BIAS ? 0.f : ref;
                 dx[i] = -delta;
             }
 #pragma unroll
@@ -531,6 +565,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 sx = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], sx);
                 dx = mma(row_operand<T, KS>(v_tile, 32 * t + (lane & 31), ks, h), of[ks], dx);
             }
+            interleave<T, 2 * KS, 2 * KS, 2 * KS < 6 ? 2 * KS : 6, 1>();
             float s[16], d[16];
             unpack(sx, s);
             unpack(dx, d);
@@ -542,7 +577,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int b = min((int)((codes[g] >> (8 * e)) & 255u), nb);
-                        const float x = fmaf(s[4 * g + e], scale, table[b]) - ref;
+                        const float x = fmaf(s[4 * g + e], scale, table[b]) + ref;
                         s[4 * g + e] = b < nb ? x : -INFINITY;
                     }
                 }
@@ -556,7 +591,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] * c) * inv * d[i];
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] * c) * d[i];
             if (BIAS) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -589,44 +624,56 @@ attention_dq_kernel(const RwkAttnArgs p) {
     }
 }
 
-// KB blocks of 32 keys per wavefront: with two, every operand read from LDS meets two products.
-template <typename T, int KS, int NW, int KB, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, 1)
+// dK and dV of 32 keys per wavefront.  Two wavefronts per SIMD hide each other's exponentials and LDS reads, which
+// leaves 256 registers each: at 128 elements of 16 bits the sums take 128 and the keys 32 of them, and the values stay
+// in LDS.
+template <typename T, int KS> constexpr bool values_in_lds() { return sizeof(T) == 2 && KS == 8; }
+template <typename T, int KS, int NW> constexpr int dkv_rows() {
+    return values_in_lds<T, KS>() ? 32 : tile_rows<T, NW>();
+}
+template <typename T, int KS, int NW> constexpr int dkv_lds() {
+    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + (4 * dkv_rows<T, KS, NW>() + 64) * (int)sizeof(float) +
+           (values_in_lds<T, KS>() ? tile_bytes<T, KS, 32 * NW>() : 0);
+}
+
+template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, KS == 8 && (sizeof(T) == 4 || !ASYNC) ? 1 : 2)
 attention_dkv_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
-    constexpr int NT = 64 * NW, DT = S::DT, BQ = tile_rows<T, NW>(), TQ = BQ / 32;
+    constexpr int NT = 64 * NW, DT = S::DT, BQ = dkv_rows<T, KS, NW>(), TQ = BQ / 32;
+    constexpr bool VL = values_in_lds<T, KS>();
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;                                       // buffer b: q at 2 b, d_out at 2 b + 1
-    // per buffer and row: - the reference, 1 / sum, - delta
-    float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>()), *table = stats + 6 * BQ;
+    // per buffer and row: the reference, - delta
+    float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>()), *table = stats + 4 * BQ;
+    T *v_tile = (T *)(table + 64);
     const Place at = key_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
-    const int k0 = at.first + 32 * KB * (int)(threadIdx.x >> 6);
+    const int wave = (int)(threadIdx.x >> 6), k0 = at.first + 32 * wave, k = k0 + (lane & 31), kc = min(k, n - 1);
     const bool causal = p.a.causal != 0;
     const int nb = (int)p.a.n_buckets;
 
-    Frag<T> kf[KB][KS], vf[KB][KS];
+    Frag<T> kf[KS], vf[VL ? 1 : KS];
+    const T *k_row = (const T *)p.a.k + (at.base + kc) * p.a.k_row + at.kv_head * p.a.k_head;
+    const T *v_base = (const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head;
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-        const int k = min(k0 + 32 * b + (lane & 31), n - 1);
-        const T *k_row = (const T *)p.a.k + (at.base + k) * p.a.k_row + at.kv_head * p.a.k_head;
-        const T *v_row = (const T *)p.a.v + (at.base + k) * p.a.v_row + at.kv_head * p.a.v_head;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            kf[b][ks] = load_global<T>(k_row, 16 * ks + 8 * h, dim);
-            vf[b][ks] = load_global<T>(v_row, 16 * ks + 8 * h, dim);
-        }
+    for (int ks = 0; ks < KS; ++ks) {
+        kf[ks] = load_global<T>(k_row, 16 * ks + 8 * h, dim);
+        if constexpr (!VL) vf[ks] = load_global<T>(v_base + kc * p.a.v_row, 16 * ks + 8 * h, dim);
+    }
+    if constexpr (VL) {
+        TileLoader<T, KS, 32 * NW, NT, ASYNC> values(v_base, p.a.v_row, n, dim);
+        values.issue(at.first, v_tile);
+        values.commit(v_tile);                    // there with the first tile of queries
     }
     const long long code_stride = (n + 31) / 32 * 32;
     const uint8_t *code_at = nullptr;
     if (BIAS) code_at = p.a.codes + p.a.code_start[at.seg];
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
 
-    f32x16 dk[KB][DT], dv[KB][DT];
+    f32x16 dk[DT], dv[DT];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) dk[b][dt] = dv[b][dt] = f32x16{};
+    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
     const int begin = causal ? at.first : 0;
     for (int g = 0; g < p.group; ++g) {
         const int head = at.head + g;
@@ -635,16 +682,15 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         TileLoader<T, KS, BQ, NT, ASYNC> grads((const T *)p.a.d_out + at.base * p.a.do_row + head * p.a.do_head, p.a.do_row, n, dim);
         __syncthreads();                          // the head before is done with the buffers and the table
         if (BIAS) load_table<T, NT>(p, head, table);
-        float held[3];
+        float held[2];
         const auto start = [&](int q0, int turn) {
             queries.issue(q0, tiles + 2 * turn * BQ * S::W);
             grads.issue(q0, tiles + (2 * turn + 1) * BQ * S::W);
             const int q = q0 + (int)threadIdx.x;
             if (threadIdx.x < BQ) {
-                const bool there = q < n;         // rows beyond: p = 0
-                held[0] = there ? -p.a.stats[2 * (row_at + q)] : 0.f;
-                held[1] = there ? p.a.stats[2 * (row_at + q) + 1] : 0.f;
-                held[2] = there ? -p.a.delta[row_at + q] : 0.f;
+                const bool there = q < n;
+                held[0] = there ? reference(p.a.stats[2 * (row_at + q)], p.a.stats[2 * (row_at + q) + 1], c) : -INFINITY;
+                held[1] = there ? -p.a.delta[row_at + q] : 0.f;
             }
         };
         const auto finish = [&](int turn) {
@@ -652,109 +698,84 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             grads.commit(tiles + (2 * turn + 1) * BQ * S::W);
             if (threadIdx.x < BQ) {
 #pragma unroll
-                for (int j = 0; j < 3; ++j) stats[(3 * turn + j) * BQ + threadIdx.x] = held[j];
+                for (int j = 0; j < 2; ++j) stats[(2 * turn + j) * BQ + threadIdx.x] = held[j];
             }
         };
         start(begin, 0);
         finish(0);
+        loads_done();
         for (int q0 = begin, turn = 0; q0 < n; q0 += BQ, turn ^= 1) {
             tile_ready<ASYNC>();
             if (q0 + BQ < n) start(q0 + BQ, turn ^ 1);
             const T *q_tile = tiles + 2 * turn * BQ * S::W, *o_tile = q_tile + BQ * S::W;
-            const float *st = stats + 3 * turn * BQ;
+            const float *st = stats + 2 * turn * BQ;
 #pragma unroll
             for (int t = 0; t < TQ; ++t) {
                 const int qt = q0 + 32 * t;
                 if (k0 >= n || qt >= n) break;
                 if (causal && qt + 31 < k0) continue;
                 typedef float f32x4 __attribute__((ext_vector_type(4)));
-                f32x16 sx[KB], dx[KB];
-                float inv[16];
+                f32x16 sx, dx;
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
                     const f32x4 r = *(const f32x4 *)(st + 32 * t + 8 * g4 + 4 * h);
-                    const f32x4 i = *(const f32x4 *)(st + BQ + 32 * t + 8 * g4 + 4 * h);
-                    const f32x4 d = *(const f32x4 *)(st + 2 * BQ + 32 * t + 8 * g4 + 4 * h);
+                    const f32x4 d = *(const f32x4 *)(st + BQ + 32 * t + 8 * g4 + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        inv[4 * g4 + e] = i[e];
-#pragma unroll
-                        for (int b = 0; b < KB; ++b) {
-                            sx[b][4 * g4 + e] = BIAS ? 0.f : r[e];
-                            dx[b][4 * g4 + e] = d[e];
-                        }
+                        sx[4 * g4 + e] = BIAS ? 0.f : r[e];
+                        dx[4 * g4 + e] = d[e];
                     }
                 }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const Frag<T> qr = row_operand<T, KS>(q_tile, 32 * t + (lane & 31), ks, h);
-                    const Frag<T> gr = row_operand<T, KS>(o_tile, 32 * t + (lane & 31), ks, h);
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) {
-                        sx[b] = mma(qr, kf[b][ks], sx[b]);
-                        dx[b] = mma(gr, vf[b][ks], dx[b]);
-                    }
+                    sx = mma(row_operand<T, KS>(q_tile, 32 * t + (lane & 31), ks, h), kf[ks], sx);
+                    const Frag<T> o = row_operand<T, KS>(o_tile, 32 * t + (lane & 31), ks, h);
+                    if constexpr (VL) dx = mma(o, row_operand<T, KS>(v_tile, 32 * wave + (lane & 31), ks, h), dx);
+                    else dx = mma(o, vf[ks], dx);
                 }
-                float s[KB][16], d[KB][16];
-#pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    unpack(sx[b], s[b]);
-                    unpack(dx[b], d[b]);
-                    const int k = k0 + 32 * b + (lane & 31);
-                    if (BIAS) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int r = qt + reg_row(i, h);
-                            const int code = r < n ? min((int)code_at[r * code_stride + min(k, n - 1)], nb) : nb;
-                            const float x = fmaf(s[b][i], scale, table[code]) + st[32 * t + reg_row(i, h)];
-                            s[b][i] = code < nb ? x : -INFINITY;
-                        }
-                    }
-                    if (BIAS || (causal && qt < k0 + 32 * b + 31)) {
-                        const int least = causal ? k : 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            s[b][i] = qt + reg_row(i, h) >= least ? s[b][i] : -INFINITY;
-                            d[b][i] = s[b][i] > -INFINITY ? d[b][i] : 0.f;
-                        }
-                    }
+                interleave<T, 8 + (VL ? 3 : 2) * KS, 2 * KS, 8 + (KS < 2 ? 2 : 6), VL ? 2 : 1>();
+                float s[16], d[16];
+                unpack(sx, s);
+                unpack(dx, d);
+                if (BIAS) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[b][i] = exp2_fast(s[b][i] * c) * inv[i];
-                        d[b][i] *= s[b][i];
+                        const int r = qt + reg_row(i, h);
+                        const int code = r < n ? min((int)code_at[r * code_stride + kc], nb) : nb;
+                        const float x = fmaf(s[i], scale, table[code]) + st[32 * t + reg_row(i, h)];
+                        s[i] = code < nb ? x : -INFINITY;
                     }
+                }
+                if (BIAS || (causal && qt < k0 + 31)) {
+                    const int least = causal ? k : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[i] = qt + reg_row(i, h) >= least ? s[i] : -INFINITY;
+                        d[i] = s[i] > -INFINITY ? d[i] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = exp2_fast(s[i] * c);
+                    d[i] *= s[i];
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    Frag<T> pf[KB], sf[KB];
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) {
-                        pf[b] = pack<T>(s[b], u);
-                        sf[b] = pack<T>(d[b], u);
-                    }
+                    const Frag<T> pf = pack<T>(s, u), sf = pack<T>(d, u);
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const Frag<T> gc = column_operand<T, KS>(o_tile, 32 * t + 16 * u, dt, lane);
-                        const Frag<T> qc = column_operand<T, KS>(q_tile, 32 * t + 16 * u, dt, lane);
-#pragma unroll
-                        for (int b = 0; b < KB; ++b) {
-                            dv[b][dt] = mma(gc, pf[b], dv[b][dt]);
-                            dk[b][dt] = mma(qc, sf[b], dk[b][dt]);
-                        }
+                        dv[dt] = mma(column_operand<T, KS>(o_tile, 32 * t + 16 * u, dt, lane), pf, dv[dt]);
+                        dk[dt] = mma(column_operand<T, KS>(q_tile, 32 * t + 16 * u, dt, lane), sf, dk[dt]);
                     }
                 }
             }
             if (q0 + BQ < n) finish(turn ^ 1);
         }
     }
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-        const int k = k0 + 32 * b + (lane & 31);
-        if (k >= n) continue;
-        const long long to = ((at.base + k) * p.a.kv_heads + at.kv_head) * dim;
-        store_rows<T, DT>((T *)p.a.dk + to, dim, h, dk[b], scale);
-        store_rows<T, DT>((T *)p.a.dv + to, dim, h, dv[b], 1.f);
-    }
+    if (k >= n) return;
+    const long long to = ((at.base + k) * p.a.kv_heads + at.kv_head) * dim;
+    store_rows<T, DT>((T *)p.a.dk + to, dim, h, dk, scale);
+    store_rows<T, DT>((T *)p.a.dv + to, dim, h, dv, 1.f);
 }
 
 template <typename K>
@@ -778,10 +799,8 @@ int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
         return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
                              tiles_bytes<T, KS, ROWS>() + (64 + (BIAS ? (p.a.n_buckets + 1) * NT : 0)) * sizeof(float), p,
                              stream);
-    // two wavefronts of 64 keys where the registers hold two blocks' keys, values and sums, else four of 32
-    constexpr int KB = WIDE && sizeof(T) == 2 && KS <= 4 ? 2 : 1, KROWS = tile_rows<T, NW / KB>();
-    return launch_kernel(attention_dkv_kernel<T, KS, NW / KB, KB, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT / KB,
-                         tiles_bytes<T, KS, KROWS>() + (6 * KROWS + 64) * sizeof(float), p, stream);
+    return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT,
+                         dkv_lds<T, KS, NW>(), p, stream);
 }
 
 // Rows whose elements are whole 16-byte chunks at 16-byte addresses, not too far apart for 32-bit offsets inside a
