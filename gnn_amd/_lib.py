@@ -151,9 +151,9 @@ SIGNATURES = {
                                c_double, c_uint64, _P, _P]),
     "rwk_attention_forward": (c_int, [_P, _P]),
     "rwk_attention_backward": (c_int, [_P, _P]),
-    "rwk_pair_buckets_dense": (c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P]),
-    "rwk_pair_buckets_relative": (c_int, [_P, _I64, _P, _P, _I64, _I64, _P, _P]),
-    "rwk_pair_buckets_hops": (c_int, [_P, _P, _P, c_int32, _P, _P, _I64, _I64, _P, _P]),
+    "rwk_pair_buckets_dense": (c_int, [_P, _P, _P, _P, _P, _I64, c_int32, _P, _P, _P]),
+    "rwk_pair_buckets_relative": (c_int, [_P, _I64, _P, _P, _P, _I64, c_int32, _P, _P, _P]),
+    "rwk_pair_buckets_hops": (c_int, [_P, _P, _P, c_int32, _P, _P, _P, _I64, c_int32, _P, _P]),
 }
 
 _lib = None

@@ -35,7 +35,7 @@ class _Args(ctypes.Structure):
                 ("v_head", _I64), ("do_row", _I64), ("do_head", _I64), ("seg_ptr", _P), ("n_segments", _I64),
                 ("rows", _I64), ("heads", _I64), ("kv_heads", _I64), ("dim", _I64), ("scale", c_float),
                 ("causal", c_int32), ("type", c_int32), ("block_rows", c_int32), ("stats", _P), ("delta", _P),
-                ("codes", _P), ("code_start", _P), ("table", _P), ("n_buckets", _I64), ("d_table", _P),
+                ("codes", _P), ("codes_by_key", _P), ("code_start", _P), ("table", _P), ("n_buckets", _I64), ("d_table", _P),
                 ("d_table_partials", _P), ("q_items", _P), ("k_items", _P), ("n_items", _I64)]
 
 
@@ -106,14 +106,16 @@ def packed_segments(lengths, device=None) -> PackedSegments:
 
 
 class PairBuckets:
-    """Bucket codes (uint8) of all pairs of a packed batch, row by row as the kernels read them."""
+    """Bucket codes (uint8) of all pairs of a packed batch as the kernels read them: a row per query, and the same with
+    a row per key for the pass that owns the keys.  Two bytes per pair, one if the codes are symmetric."""
 
-    def __init__(self, segments: PackedSegments):
+    def __init__(self, segments: PackedSegments, symmetric: bool = False):
         self.segments = segments
         padded = -(-segments.lengths // 32) * 32
         sizes = segments.lengths * padded
         self._start = torch.from_numpy(np.concatenate([[0], np.cumsum(sizes)])).to(segments.device)
         self._codes = torch.empty(int(sizes.sum()), dtype=torch.uint8, device=segments.device)
+        self._by_key = self._codes if symmetric else torch.empty_like(self._codes)
 
     def dense(self, segment: int) -> torch.Tensor:
         """Codes of one segment, (n, n): query row, key row."""
@@ -124,12 +126,13 @@ class PairBuckets:
         return self._codes[start:start + n * padded].view(n, padded)[:, :n]
 
 
-def _fill(segments: PackedSegments, entry: str, *args) -> PairBuckets:
-    buckets = PairBuckets(segments)
+def _fill(segments: PackedSegments, entry: str, *args, symmetric: bool = False) -> PairBuckets:
+    buckets = PairBuckets(segments, symmetric)
+    out = (buckets._codes.data_ptr(),) if symmetric else (buckets._codes.data_ptr(), buckets._by_key.data_ptr())
     with _lib.device_guard(segments.device):
         _lib.check(getattr(_lib.load(), entry)(
-            *args, segments._seg_ptr, buckets._start.data_ptr(), segments.n_segments, segments.total,
-            buckets._codes.data_ptr(), _lib.current_stream(segments.device)), entry)
+            *args, segments._seg_ptr, buckets._start.data_ptr(), segments._items, segments.n_items,
+            segments.block_rows, *out, _lib.current_stream(segments.device)), entry)
     return buckets
 
 
@@ -187,7 +190,7 @@ def hop_buckets(adj: torch.Tensor, graph_indicator: torch.Tensor, max_distance: 
     elif not np.array_equal(segments.lengths, st.base.counts.cpu().numpy()):
         raise ValueError("the segments are not the batch's graphs")
     return _fill(segments, "rwk_pair_buckets_hops", st.row_start.data_ptr(), _lib.ptr(st.col), _lib.ptr(st.dist),
-                 st.max_distance + 1 if far == "bucket" else 255)
+                 st.max_distance + 1 if far == "bucket" else 255, symmetric=True)
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -209,7 +212,8 @@ def _describe(q, k, v, segments, causal, scale, table, buckets):
     a.q_items = segments._q_causal if causal else segments._items
     a.k_items = segments._k_causal if causal else segments._items
     if table is not None:
-        a.codes, a.code_start = buckets._codes.data_ptr(), buckets._start.data_ptr()
+        a.codes, a.codes_by_key = buckets._codes.data_ptr(), buckets._by_key.data_ptr()
+        a.code_start = buckets._start.data_ptr()
         a.table, a.n_buckets = table.data_ptr(), table.shape[1]
     return a
 

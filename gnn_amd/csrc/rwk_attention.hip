@@ -61,6 +61,8 @@ int check(const rwk_attention *a, bool backward) {
     if (a->n_buckets > 0) {
         RWK_REQUIRE_PTR(a->codes);
         RWK_REQUIRE_PTR(a->code_start);
+        if (backward) RWK_REQUIRE_PTR(a->codes_by_key);
+        if ((uintptr_t)a->codes % 16 != 0 || (uintptr_t)a->codes_by_key % 16 != 0) return RWK_E_ALIGN;
     }
     if (backward) {
         RWK_REQUIRE_PTR(a->d_out);
@@ -84,75 +86,111 @@ int launch(RwkAttnPass pass, const rwk_attention &a, const int32_t *items, hipSt
     return rwk_attention_launch_bf16(pass, p, stream);
 }
 
-// segment of a row: the last g with seg_ptr[g] <= row (segments without rows are passed over)
-__device__ inline int segment_of(const int *__restrict__ seg_ptr, int n_segments, int row) {
-    int lo = 0, hi = n_segments;                 // seg_ptr[lo] <= row < seg_ptr[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (seg_ptr[mid] <= row) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-struct CodeRow {
-    int g, i, n, padded;
-    uint8_t *out;
+// The workgroups of the kernels below each take one block of rows of a segment.
+struct CodeBlock {
+    int g, first, n, rows, padded;
+    long long start;
 };
-__device__ inline CodeRow code_row(const int *seg_ptr, int n_segments, const int64_t *code_start, uint8_t *codes,
-                                   int row) {
-    CodeRow r;
-    r.g = segment_of(seg_ptr, n_segments, row);
-    r.i = row - seg_ptr[r.g];
-    r.n = seg_ptr[r.g + 1] - seg_ptr[r.g];
-    r.padded = (r.n + 31) / 32 * 32;
-    r.out = codes + code_start[r.g] + (long long)r.i * r.padded;
-    return r;
+__device__ inline CodeBlock code_block(const int *items, const int *seg_ptr, const int64_t *code_start, int block_rows) {
+    CodeBlock b;
+    b.g = items[2 * blockIdx.x];
+    b.first = items[2 * blockIdx.x + 1];
+    b.n = seg_ptr[b.g + 1] - seg_ptr[b.g];
+    b.rows = min(block_rows, b.n - b.first);
+    b.padded = (b.n + 31) / 32 * 32;
+    b.start = code_start[b.g];
+    return b;
 }
 
+// Rows of n bytes at any address to rows of a multiple of 32, four bytes a lane, a wavefront per row; and, by 64 x 64
+// tiles through LDS, to the same with a row per key.
 __global__ void __launch_bounds__(kBlock)
 pair_dense_kernel(const uint8_t *__restrict__ dense, const int64_t *__restrict__ pair_start,
-                  const int *__restrict__ seg_ptr, const int64_t *__restrict__ code_start, int n_segments,
-                  uint8_t *__restrict__ codes) {
-    const CodeRow r = code_row(seg_ptr, n_segments, code_start, codes, (int)blockIdx.x);
-    const uint8_t *in = dense + pair_start[r.g] + (long long)r.i * r.n;
-    for (int j = threadIdx.x; j < r.padded; j += kBlock) r.out[j] = j < r.n ? in[j] : 255;
+                  const int *__restrict__ seg_ptr, const int64_t *__restrict__ code_start,
+                  const int *__restrict__ items, int block_rows, uint8_t *__restrict__ codes,
+                  uint8_t *__restrict__ codes_by_key) {
+    __shared__ uint8_t tile[64][68];
+    const CodeBlock b = code_block(items, seg_ptr, code_start, block_rows);
+    const uint8_t *in = dense + pair_start[b.g];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r = wave; r < b.rows; r += kBlock / 64) {
+        const uint8_t *row = in + (long long)(b.first + r) * b.n;
+        for (int j = 4 * lane; j < b.padded; j += 256) {
+            uint32_t v = 0xFFFFFFFFu;
+            if (j + 4 <= b.n) {
+                __builtin_memcpy(&v, row + j, 4);
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < b.n) v = (v & ~(255u << (8 * e))) | ((uint32_t)row[j + e] << (8 * e));
+            }
+            *(uint32_t *)(codes + b.start + (long long)(b.first + r) * b.padded + j) = v;
+        }
+    }
+    for (int k0 = b.first; k0 < b.first + b.rows; k0 += 64)
+        for (int q0 = 0; q0 < b.padded; q0 += 64) {
+            __syncthreads();
+            for (int i = wave; i < 64; i += kBlock / 64)
+                tile[i][lane] = q0 + i < b.n && k0 + lane < b.n ? in[(long long)(q0 + i) * b.n + k0 + lane] : 255;
+            __syncthreads();
+            for (int i = wave; i < 64; i += kBlock / 64)
+                if (k0 + i < b.first + b.rows && q0 + lane < b.padded)
+                    codes_by_key[b.start + (long long)(k0 + i) * b.padded + q0 + lane] = tile[lane][i];
+        }
 }
 
 __global__ void __launch_bounds__(kBlock)
 pair_relative_kernel(const uint8_t *__restrict__ by_offset, int reach, const int *__restrict__ seg_ptr,
-                     const int64_t *__restrict__ code_start, int n_segments, uint8_t *__restrict__ codes) {
-    const CodeRow r = code_row(seg_ptr, n_segments, code_start, codes, (int)blockIdx.x);
-    for (int j = threadIdx.x; j < r.padded; j += kBlock) {
-        int d = j - r.i;
-        d = d < -reach ? -reach : d > reach ? reach : d;
-        r.out[j] = j < r.n ? by_offset[d + reach] : 255;
+                     const int64_t *__restrict__ code_start, const int *__restrict__ items, int block_rows,
+                     uint8_t *__restrict__ codes, uint8_t *__restrict__ codes_by_key) {
+    const CodeBlock b = code_block(items, seg_ptr, code_start, block_rows);
+    const auto code = [&](int d) { return (uint32_t)by_offset[min(max(d, -reach), reach) + reach]; };
+    for (int r = threadIdx.x >> 6; r < b.rows; r += kBlock / 64) {
+        const int i = b.first + r;
+        const long long at = b.start + (long long)i * b.padded;
+        for (int j = 4 * (threadIdx.x & 63); j < b.padded; j += 256) {
+            uint32_t forward = 0, back = 0;
+            for (int e = 0; e < 4; ++e) {
+                forward |= (j + e < b.n ? code(j + e - i) : 255u) << (8 * e);
+                back |= (j + e < b.n ? code(i - j - e) : 255u) << (8 * e);
+            }
+            *(uint32_t *)(codes + at + j) = forward;
+            *(uint32_t *)(codes_by_key + at + j) = back;
+        }
     }
 }
 
 __global__ void __launch_bounds__(kBlock)
 pair_hops_kernel(const int *__restrict__ row_start, const int *__restrict__ col, const int *__restrict__ dist,
                  int far_code, const int *__restrict__ seg_ptr, const int64_t *__restrict__ code_start,
-                 int n_segments, uint8_t *__restrict__ codes) {
-    const int row = (int)blockIdx.x;
-    const CodeRow r = code_row(seg_ptr, n_segments, code_start, codes, row);
-    for (int j = threadIdx.x; j < r.padded; j += kBlock)
-        r.out[j] = j == r.i ? 0 : j < r.n ? (uint8_t)far_code : 255;
+                 const int *__restrict__ items, int block_rows, uint8_t *__restrict__ codes) {
+    const CodeBlock b = code_block(items, seg_ptr, code_start, block_rows);
+    const int lo = seg_ptr[b.g];
+    for (int r = 0; r < b.rows; ++r) {
+        const int i = b.first + r;
+        uint8_t *out = codes + b.start + (long long)i * b.padded;
+        for (int j = threadIdx.x; j < b.padded; j += kBlock) out[j] = j == i ? 0 : j < b.n ? (uint8_t)far_code : 255;
+    }
     __syncthreads();                              // the listed pairs overwrite what other threads wrote
-    for (int e = row_start[row] + threadIdx.x; e < row_start[row + 1]; e += kBlock) {
-        const int j = col[e] - (row - r.i);
-        if ((unsigned)j < (unsigned)r.n) r.out[j] = (uint8_t)dist[e];
+    for (int r = threadIdx.x >> 6; r < b.rows; r += kBlock / 64) {
+        const int i = b.first + r;
+        uint8_t *out = codes + b.start + (long long)i * b.padded;
+        for (int e = row_start[lo + i] + (int)(threadIdx.x & 63); e < row_start[lo + i + 1]; e += 64) {
+            const int j = col[e] - lo;
+            if ((unsigned)j < (unsigned)b.n) out[j] = (uint8_t)dist[e];
+        }
     }
 }
 
-int check_codes(const int32_t *seg_ptr, const int64_t *code_start, int64_t n_segments, int64_t rows,
-                const uint8_t *codes) {
-    if (n_segments < 0 || n_segments >= 0x7FFFFFFFll || rows < 0 || rows >= 0x7FFFFFFFll) return RWK_E_SIZE;
-    if (rows > 0 && n_segments < 1) return RWK_E_SIZE;
-    if (rows == 0) return RWK_OK;
+int check_codes(const int32_t *seg_ptr, const int64_t *code_start, const int32_t *items, int64_t n_items,
+                int32_t block_rows, const uint8_t *codes) {
+    if (n_items < 0 || n_items > 0x7FFFFFFFll) return RWK_E_SIZE;
+    if (block_rows != 32 && block_rows != 128) return RWK_E_UNSUPPORTED;
+    if (n_items == 0) return RWK_OK;
     RWK_REQUIRE_PTR(seg_ptr);
     RWK_REQUIRE_PTR(code_start);
+    RWK_REQUIRE_PTR(items);
     RWK_REQUIRE_PTR(codes);
-    return RWK_OK;
+    return (uintptr_t)codes % 16 == 0 ? RWK_OK : RWK_E_ALIGN;
 }
 
 }  // namespace
@@ -177,40 +215,42 @@ int rwk_attention_backward(const rwk_attention *a, rwk_stream_t stream) {
 }
 
 int rwk_pair_buckets_dense(const uint8_t *dense, const int64_t *pair_start, const int32_t *seg_ptr,
-                           const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
-                           rwk_stream_t stream) {
-    const int code = check_codes(seg_ptr, code_start, n_segments, rows, codes);
-    if (code != RWK_OK || rows == 0) return code;
+                           const int64_t *code_start, const int32_t *items, int64_t n_items, int32_t block_rows,
+                           uint8_t *codes, uint8_t *codes_by_key, rwk_stream_t stream) {
+    int code = check_codes(seg_ptr, code_start, items, n_items, block_rows, codes);
+    if (code == RWK_OK) code = check_codes(seg_ptr, code_start, items, n_items, block_rows, codes_by_key);
+    if (code != RWK_OK || n_items == 0) return code;
     RWK_REQUIRE_PTR(dense);
     RWK_REQUIRE_PTR(pair_start);
-    hipLaunchKernelGGL(pair_dense_kernel, dim3((unsigned)rows), dim3(kBlock), 0, (hipStream_t)stream, dense,
-                       pair_start, seg_ptr, code_start, (int)n_segments, codes);
+    hipLaunchKernelGGL(pair_dense_kernel, dim3((unsigned)n_items), dim3(kBlock), 0, (hipStream_t)stream, dense,
+                       pair_start, seg_ptr, code_start, items, block_rows, codes, codes_by_key);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }
 
 int rwk_pair_buckets_relative(const uint8_t *by_offset, int64_t reach, const int32_t *seg_ptr,
-                              const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
-                              rwk_stream_t stream) {
-    const int code = check_codes(seg_ptr, code_start, n_segments, rows, codes);
+                              const int64_t *code_start, const int32_t *items, int64_t n_items, int32_t block_rows,
+                              uint8_t *codes, uint8_t *codes_by_key, rwk_stream_t stream) {
     if (reach < 0 || reach > 0x3FFFFFFF) return RWK_E_SIZE;
-    if (code != RWK_OK || rows == 0) return code;
+    int code = check_codes(seg_ptr, code_start, items, n_items, block_rows, codes);
+    if (code == RWK_OK) code = check_codes(seg_ptr, code_start, items, n_items, block_rows, codes_by_key);
+    if (code != RWK_OK || n_items == 0) return code;
     RWK_REQUIRE_PTR(by_offset);
-    hipLaunchKernelGGL(pair_relative_kernel, dim3((unsigned)rows), dim3(kBlock), 0, (hipStream_t)stream, by_offset,
-                       (int)reach, seg_ptr, code_start, (int)n_segments, codes);
+    hipLaunchKernelGGL(pair_relative_kernel, dim3((unsigned)n_items), dim3(kBlock), 0, (hipStream_t)stream, by_offset,
+                       (int)reach, seg_ptr, code_start, items, block_rows, codes, codes_by_key);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }
 
 int rwk_pair_buckets_hops(const int32_t *row_start, const int32_t *col, const int32_t *dist, int32_t far_code,
-                          const int32_t *seg_ptr, const int64_t *code_start, int64_t n_segments, int64_t rows,
-                          uint8_t *codes, rwk_stream_t stream) {
-    const int code = check_codes(seg_ptr, code_start, n_segments, rows, codes);
+                          const int32_t *seg_ptr, const int64_t *code_start, const int32_t *items, int64_t n_items,
+                          int32_t block_rows, uint8_t *codes, rwk_stream_t stream) {
     if (far_code < 0 || far_code > 255) return RWK_E_SIZE;
-    if (code != RWK_OK || rows == 0) return code;
+    const int code = check_codes(seg_ptr, code_start, items, n_items, block_rows, codes);
+    if (code != RWK_OK || n_items == 0) return code;
     RWK_REQUIRE_PTR(row_start);
-    hipLaunchKernelGGL(pair_hops_kernel, dim3((unsigned)rows), dim3(kBlock), 0, (hipStream_t)stream, row_start, col,
-                       dist, far_code, seg_ptr, code_start, (int)n_segments, codes);
+    hipLaunchKernelGGL(pair_hops_kernel, dim3((unsigned)n_items), dim3(kBlock), 0, (hipStream_t)stream, row_start, col,
+                       dist, far_code, seg_ptr, code_start, items, block_rows, codes);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }

@@ -114,6 +114,13 @@ __device__ inline uint32_t lds_address(const void *p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
 }
 
+__device__ inline void load_to_lds(i32x4 rsrc, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to), "v"(offset), "s"(rsrc)
+                 : "memory");          // m0 is set right before every use by the compiler too
+}
+
 // ROWS rows at a time of a (rows, dim) matrix of a segment into LDS; rows from `rows` on and elements from `dim` on are
 // zeros.  issue() starts the tile that begins at row `first`, commit() finishes it; in between, the workgroup computes
 // on the other buffer.
@@ -158,10 +165,7 @@ struct TileLoader {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (ROWS * S::C % NT != 0 && (int)(threadIdx.x & ~63u) + i * NT >= ROWS * S::C) break;
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                             :
-                             : "s"(to + i * NT * 16), "v"(offset[i]), "s"(rsrc)
-                             : "memory");          // m0 is set right before every use by the compiler too
+                load_to_lds(rsrc, offset[i], to + i * NT * 16);
             }
         } else {
 #pragma unroll
@@ -196,10 +200,52 @@ struct TileLoader {
     }
 };
 
+// Bucket codes of ROWS rows (the workgroup's own rows, the last of the segment for those behind it) and COLS columns
+// at a time, straight into LDS.  Columns from the segment's end on hold anything.
+template <int ROWS, int COLS, int NT>
+struct CodeLoader {
+    static constexpr int C = COLS / 16, N = (ROWS * C + NT - 1) / NT;
+    const uint8_t *base;
+    int pitch, records;
+    uint32_t offset[N];
+    __device__ static int at(int row, int chunk) {
+        return row * COLS + (chunk ^ (C == 4 ? (row >> 2) & 3 : (row >> 3) & 1)) * 16;
+    }
+    __device__ CodeLoader(const uint8_t *codes, int first, int n) {
+        pitch = (n + 31) / 32 * 32;
+        base = codes + (long long)first * pitch;
+        const int last = min(ROWS, n - first) - 1;
+        records = (last + 1) * pitch;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = (int)threadIdx.x + i * NT, row = k / C, c = (at(row, k % C) - row * COLS) / 16;
+            offset[i] = (uint32_t)(min(row, last) * pitch + c * 16);
+        }
+    }
+    __device__ void issue(int column, uint8_t *lds) const {
+        const uint64_t from = (uint64_t)(base + column);
+        i32x4 rsrc;
+        rsrc[0] = __builtin_amdgcn_readfirstlane((int)from);
+        rsrc[1] = __builtin_amdgcn_readfirstlane((int)((from >> 32) & 0xFFFFu));
+        rsrc[2] = __builtin_amdgcn_readfirstlane(records - column);
+        rsrc[3] = 0x00027000;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (threadIdx.x & ~63u) * 16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (ROWS * C % NT != 0 && (int)(threadIdx.x & ~63u) + i * NT >= ROWS * C) break;
+            load_to_lds(rsrc, offset[i], to + i * NT * 16);
+        }
+    }
+    // codes of the columns first .. first + 3 (a multiple of four)
+    __device__ static uint32_t read(const uint8_t *lds, int row, int first) {
+        return *(const uint32_t *)(lds + at(row, first >> 4) + (first & 15));
+    }
+};
+
 // everything this workgroup's loads and writes put into LDS is there, and nobody reads the buffer before it any more
-template <bool ASYNC>
+template <bool DIRECT>
 __device__ inline void tile_ready() {
-    if (ASYNC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
 
@@ -207,19 +253,19 @@ __device__ inline void tile_ready() {
 // inside it, and with them for the tiles in flight, again in every round.
 __device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }          // vmcnt(0)
 
-// Order of the LDS reads and products that the compiler has put into one block: AHEAD reads first, then PER reads
-// behind every product.  By itself it reads every operand right before its product and waits.
-template <typename T, int READS, int PRODUCTS, int AHEAD, int PER>
+// Order of as many LDS reads and products that the compiler has put into one block: a few reads first, then one behind
+// every product.  By itself it reads every operand of the forward pass's scores right before its product and waits.
+template <typename T, int N>
 __device__ inline void interleave() {
     if constexpr (sizeof(T) == 2) {
-        constexpr int N = (READS - AHEAD + PER - 1) / PER;
+        constexpr int AHEAD = N < 6 ? N : 6;
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < N - AHEAD; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - N, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
     }
 }
 
@@ -336,19 +382,56 @@ __device__ inline Place key_place(const RwkAttnArgs &p, long long b) {
     return s;
 }
 
-// the bias of one head in LDS, -infinity for codes that do not attend
-template <typename T, int NT>
-__device__ inline void load_table(const RwkAttnArgs &p, int head, float *table) {
-    for (int b = threadIdx.x; b <= p.a.n_buckets; b += NT)
-        table[b] = b < p.a.n_buckets ? (float)((const T *)p.a.table)[(long long)head * p.a.n_buckets + b] : -INFINITY;
+// code e of four, at most n_buckets
+__device__ inline int code_of(uint32_t codes, int e, int nb) { return min((int)((codes >> (8 * e)) & 255u), nb); }
+
+// Adds four values to a thread's own sums, NT floats apart, by their codes (a masked pair's 0 to any).  All four sums
+// are read before the first is written; an equal code before takes the place of what was read.  (The LDS float atomic
+// works through its lanes one by one: 180 cycles for a wavefront's 64 separate places, measured.)
+template <int NT>
+__device__ inline void add_by_code(float *sums, uint32_t codes, int last, const float *x) {
+    int c[4];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        c[e] = code_of(codes, e, last);
+        v[e] = sums[c[e] * NT];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int f = 0; f < e; ++f) v[e] = c[f] == c[e] ? v[f] : v[e];
+        v[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[c[e] * NT] = v[e];
 }
 
-// Bytes of LDS in front of the bias table: two buffers of two tiles, and the elements that the second product of
-// KS = 1 reads past the last row.
+// product of a probability and a value: 0 where the probability is 0 (a masked pair), whatever the value
+// (v_mul_legacy_f32)
+extern "C" __device__ float rwk_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ inline float weigh(float p, float x) { return rwk_mul_legacy(p, x); }
+
+// The bias of one head, bucket b in lane b of every wavefront, -infinity from n_buckets on: a look-up fetches another
+// lane's register.
+template <typename T>
+__device__ inline float load_table(const RwkAttnArgs &p, int head) {
+    const int b = (int)(threadIdx.x & 63);
+    return b < p.a.n_buckets ? (float)((const T *)p.a.table)[(long long)head * p.a.n_buckets + b] : -INFINITY;
+}
+__device__ inline float look_up(float table, int bucket) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * bucket, __builtin_bit_cast(int, table)));
+}
+
+// Bytes of LDS for the tiles: two buffers of two, and the elements that the second product of KS = 1 reads past the
+// last row.
 template <typename T, int KS, int ROWS> constexpr int tile_bytes() { return ROWS * 16 * KS * (int)sizeof(T); }
 template <typename T, int KS, int ROWS> constexpr int tiles_bytes() {
     return 4 * tile_bytes<T, KS, ROWS>() + (KS == 1 ? 32 * (int)sizeof(T) : 0);
 }
+// bytes of LDS behind the tiles for a bias: two buffers of codes of 32 NW rows and as many columns as the other
+// operand's tile has rows
+template <int NW, int COLS> constexpr int code_bytes() { return 2 * 32 * NW * COLS; }
 template <typename T, int NW> constexpr int tile_rows() { return sizeof(T) == 2 && NW > 1 ? 64 : 32; }
 
 // Scores below the reference by this much or less (in powers of two) leave it as it is: the sums and the output are
@@ -363,13 +446,14 @@ attention_forward_kernel(const RwkAttnArgs p) {
     constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;                                       // buffer b: keys at 2 b, values at 2 b + 1
-    float *table = (float *)(attn_lds + tiles_bytes<T, KS, BN>());
+    uint8_t *codes = (uint8_t *)attn_lds + tiles_bytes<T, KS, BN>();
+    typedef CodeLoader<32 * NW, BN, NT> Codes;
     const Place at = query_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int q0 = at.first + 32 * (int)(threadIdx.x >> 6), q = q0 + (lane & 31), qc = q < n ? q : n - 1;
     const bool causal = p.a.causal != 0;
     const int nb = (int)p.a.n_buckets;
-    if (BIAS) load_table<T, NT>(p, at.head, table);
+    const float table = BIAS ? load_table<T>(p, at.head) : 0.f;
 
     TileLoader<T, KS, BN, NT, ASYNC> keys((const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head, p.a.k_row, n, dim);
     TileLoader<T, KS, BN, NT, ASYNC> values((const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head, p.a.v_row, n, dim);
@@ -379,8 +463,8 @@ attention_forward_kernel(const RwkAttnArgs p) {
     const T *q_row = (const T *)p.a.q + (at.base + qc) * p.a.q_row + at.head * p.a.q_head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = load_global<T>(q_row, 16 * ks + 8 * h, dim);
-    const uint8_t *code_row = nullptr;
-    if (BIAS) code_row = p.a.codes + p.a.code_start[at.seg] + (long long)qc * ((n + 31) / 32 * 32);
+    const Codes code_tiles(BIAS ? p.a.codes + p.a.code_start[at.seg] : nullptr, at.first, n);
+    if (BIAS) code_tiles.issue(0, codes);
 
     // without a bias the maximum is taken over q . k and the scale meets it in the exponent; with one the scores are
     // the sum, and the difference is formed before the change of base, so that a bias of the type's lowest value
@@ -397,10 +481,11 @@ attention_forward_kernel(const RwkAttnArgs p) {
     for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
         const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
         T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
-        tile_ready<ASYNC>();
+        tile_ready<ASYNC || BIAS>();
         if (k0 + BN < end) {
             keys.issue(k0 + BN, next);
             values.issue(k0 + BN, next + BN * S::W);
+            if (BIAS) code_tiles.issue(k0 + BN, codes + (turn ^ 1) * 32 * NW * BN);
         }
         if (q0 < n && !(causal && k0 > q0 + 31)) {
             float s[TN][16];
@@ -412,19 +497,17 @@ attention_forward_kernel(const RwkAttnArgs p) {
                     x = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], x);
                 unpack(x, s[t]);
             }
-            interleave<T, TN * KS, TN * KS, TN * KS < 6 ? TN * KS : 6, 1>();
+            interleave<T, TN * KS>();
             if (BIAS) {
 #pragma unroll
                 for (int t = 0; t < TN; ++t)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        // columns from n on are padded with codes that do not attend
-                        const uint32_t codes = k0 + 32 * t < n
-                            ? *(const uint32_t *)(code_row + k0 + 32 * t + 8 * g + 4 * h) : 0xFFFFFFFFu;
+                        const uint32_t four = Codes::read(codes + turn * 32 * NW * BN, q - at.first, 32 * t + 8 * g + 4 * h);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int b = min((int)((codes >> (8 * e)) & 255u), nb);
-                            const float x = fmaf(s[t][4 * g + e], scale, table[b]);
+                            const int b = code_of(four, e, nb);
+                            const float x = fmaf(s[t][4 * g + e], scale, look_up(table, b));
                             s[t][4 * g + e] = b < nb ? x : -INFINITY;
                         }
                     }
@@ -492,22 +575,23 @@ attention_forward_kernel(const RwkAttnArgs p) {
 __device__ inline float reference(float ref, float inv, float c) { return __log2f(inv) / c - ref; }
 
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && !BIAS ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && (!BIAS || KS < 8) ? 2 : 1)
 attention_dq_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;
-    float *table = (float *)(attn_lds + tiles_bytes<T, KS, BN>()), *hist = table + 64;
+    uint8_t *codes = (uint8_t *)attn_lds + tiles_bytes<T, KS, BN>();
+    typedef CodeLoader<32 * NW, BN, NT> Codes;
+    float *hist = (float *)(codes + 2 * 32 * NW * BN);
     const Place at = query_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int q0 = at.first + 32 * (int)(threadIdx.x >> 6), q = q0 + (lane & 31), qc = q < n ? q : n - 1;
     const bool causal = p.a.causal != 0;
     const int nb = (int)p.a.n_buckets;
-    if (BIAS) {
-        load_table<T, NT>(p, at.head, table);
-        for (int b = 0; b <= nb; ++b) hist[b * NT + threadIdx.x] = 0.f;    // a thread's own sums
-    }
+    const float table = BIAS ? load_table<T>(p, at.head) : 0.f;
+    if (BIAS)
+        for (int b = 0; b < nb; ++b) hist[b * NT + threadIdx.x] = 0.f;     // a thread's own sums
 
     TileLoader<T, KS, BN, NT, ASYNC> keys((const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head, p.a.k_row, n, dim);
     TileLoader<T, KS, BN, NT, ASYNC> values((const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head, p.a.v_row, n, dim);
@@ -529,8 +613,8 @@ attention_dq_kernel(const RwkAttnArgs p) {
     delta += __shfl_xor(delta, 32, 64);
     const long long row_at = at.head * p.a.rows + at.base + qc;
     if (q < n && h == 0) p.a.delta[row_at] = delta;
-    const uint8_t *code_row = nullptr;
-    if (BIAS) code_row = p.a.codes + p.a.code_start[at.seg] + (long long)qc * ((n + 31) / 32 * 32);
+    const Codes code_tiles(BIAS ? p.a.codes + p.a.code_start[at.seg] : nullptr, at.first, n);
+    if (BIAS) code_tiles.issue(0, codes);
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
     const float ref = reference(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
 
@@ -544,10 +628,11 @@ attention_dq_kernel(const RwkAttnArgs p) {
     for (int k0 = 0, turn = 0; k0 < end; k0 += BN, turn ^= 1) {
         const T *k_tile = tiles + 2 * turn * BN * S::W, *v_tile = k_tile + BN * S::W;
         T *next = tiles + 2 * (turn ^ 1) * BN * S::W;
-        tile_ready<ASYNC>();
+        tile_ready<ASYNC || BIAS>();
         if (k0 + BN < end) {
             keys.issue(k0 + BN, next);
             values.issue(k0 + BN, next + BN * S::W);
+            if (BIAS) code_tiles.issue(k0 + BN, codes + (turn ^ 1) * 32 * NW * BN);
         }
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
@@ -565,39 +650,32 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 sx = mma(row_operand<T, KS>(k_tile, 32 * t + (lane & 31), ks, h), qf[ks], sx);
                 dx = mma(row_operand<T, KS>(v_tile, 32 * t + (lane & 31), ks, h), of[ks], dx);
             }
-            interleave<T, 2 * KS, 2 * KS, 2 * KS < 6 ? 2 * KS : 6, 1>();
             float s[16], d[16];
             unpack(sx, s);
             unpack(dx, d);
-            uint32_t codes[4];
+            uint32_t four[4];
             if (BIAS) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    codes[g] = *(const uint32_t *)(code_row + kt + 8 * g + 4 * h);
+                    four[g] = Codes::read(codes + turn * 32 * NW * BN, q - at.first, 32 * t + 8 * g + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int b = min((int)((codes[g] >> (8 * e)) & 255u), nb);
-                        const float x = fmaf(s[4 * g + e], scale, table[b]) + ref;
+                        const int b = code_of(four[g], e, nb);
+                        const float x = fmaf(s[4 * g + e], scale, look_up(table, b)) + ref;
                         s[4 * g + e] = b < nb ? x : -INFINITY;
                     }
                 }
             }
-            if (BIAS || kt + 32 > n || (causal && kt + 31 > q0)) {
+            if (kt + 32 > n || (causal && kt + 31 > q0)) {
                 const int last = causal ? min(q, n - 1) : n - 1;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
-                    d[i] = s[i] > -INFINITY ? d[i] : 0.f;        // a masked pair's value may be anything
-                }
+                for (int i = 0; i < 16; ++i) s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] * c) * d[i];
-            if (BIAS) {
+            for (int i = 0; i < 16; ++i) s[i] = weigh(exp2_fast(s[i] * c), d[i]);
+            if (BIAS && q < n) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int b = min((int)((codes[i >> 2] >> (8 * (i & 3))) & 255u), nb);
-                    hist[b * NT + threadIdx.x] += q < n ? s[i] : 0.f;
-                }
+                for (int g = 0; g < 4; ++g) add_by_code<NT>(hist + threadIdx.x, four[g], nb - 1, s + 4 * g);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -631,13 +709,14 @@ template <typename T, int KS> constexpr bool values_in_lds() { return sizeof(T) 
 template <typename T, int KS, int NW> constexpr int dkv_rows() {
     return values_in_lds<T, KS>() ? 32 : tile_rows<T, NW>();
 }
-template <typename T, int KS, int NW> constexpr int dkv_lds() {
-    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + (4 * dkv_rows<T, KS, NW>() + 64) * (int)sizeof(float) +
+template <typename T, int KS, int NW, bool BIAS> constexpr int dkv_lds() {
+    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + 4 * dkv_rows<T, KS, NW>() * (int)sizeof(float) +
+           (BIAS ? code_bytes<NW, dkv_rows<T, KS, NW>()>() : 0) +
            (values_in_lds<T, KS>() ? tile_bytes<T, KS, 32 * NW>() : 0);
 }
 
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, KS == 8 && (sizeof(T) == 4 || !ASYNC) ? 1 : 2)
+__global__ void __launch_bounds__(64 * NW, KS == 8 && (sizeof(T) == 4 || BIAS || !ASYNC) ? 1 : 2)
 attention_dkv_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BQ = dkv_rows<T, KS, NW>(), TQ = BQ / 32;
@@ -645,8 +724,10 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;                                       // buffer b: q at 2 b, d_out at 2 b + 1
     // per buffer and row: the reference, - delta
-    float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>()), *table = stats + 4 * BQ;
-    T *v_tile = (T *)(table + 64);
+    float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>());
+    uint8_t *codes = (uint8_t *)(stats + 4 * BQ);
+    typedef CodeLoader<32 * NW, BQ, NT> Codes;
+    T *v_tile = (T *)(codes + (BIAS ? 2 * 32 * NW * BQ : 0));
     const Place at = key_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int wave = (int)(threadIdx.x >> 6), k0 = at.first + 32 * wave, k = k0 + (lane & 31), kc = min(k, n - 1);
@@ -666,9 +747,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         values.issue(at.first, v_tile);
         values.commit(v_tile);                    // there with the first tile of queries
     }
-    const long long code_stride = (n + 31) / 32 * 32;
-    const uint8_t *code_at = nullptr;
-    if (BIAS) code_at = p.a.codes + p.a.code_start[at.seg];
+    const Codes code_tiles(BIAS ? p.a.codes_by_key + p.a.code_start[at.seg] : nullptr, at.first, n);
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
 
     f32x16 dk[DT], dv[DT];
@@ -680,12 +759,13 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         const long long row_at = head * p.a.rows + at.base;
         TileLoader<T, KS, BQ, NT, ASYNC> queries((const T *)p.a.q + at.base * p.a.q_row + head * p.a.q_head, p.a.q_row, n, dim);
         TileLoader<T, KS, BQ, NT, ASYNC> grads((const T *)p.a.d_out + at.base * p.a.do_row + head * p.a.do_head, p.a.do_row, n, dim);
-        __syncthreads();                          // the head before is done with the buffers and the table
-        if (BIAS) load_table<T, NT>(p, head, table);
+        const float table = BIAS ? load_table<T>(p, head) : 0.f;
+        __syncthreads();                          // the head before is done with the buffers
         float held[2];
         const auto start = [&](int q0, int turn) {
             queries.issue(q0, tiles + 2 * turn * BQ * S::W);
             grads.issue(q0, tiles + (2 * turn + 1) * BQ * S::W);
+            if (BIAS) code_tiles.issue(q0, codes + turn * 32 * NW * BQ);
             const int q = q0 + (int)threadIdx.x;
             if (threadIdx.x < BQ) {
                 const bool there = q < n;
@@ -705,7 +785,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         finish(0);
         loads_done();
         for (int q0 = begin, turn = 0; q0 < n; q0 += BQ, turn ^= 1) {
-            tile_ready<ASYNC>();
+            tile_ready<ASYNC || BIAS>();
             if (q0 + BQ < n) start(q0 + BQ, turn ^ 1);
             const T *q_tile = tiles + 2 * turn * BQ * S::W, *o_tile = q_tile + BQ * S::W;
             const float *st = stats + 2 * turn * BQ;
@@ -733,31 +813,31 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                     if constexpr (VL) dx = mma(o, row_operand<T, KS>(v_tile, 32 * wave + (lane & 31), ks, h), dx);
                     else dx = mma(o, vf[ks], dx);
                 }
-                interleave<T, 8 + (VL ? 3 : 2) * KS, 2 * KS, 8 + (KS < 2 ? 2 : 6), VL ? 2 : 1>();
                 float s[16], d[16];
                 unpack(sx, s);
                 unpack(dx, d);
                 if (BIAS) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = qt + reg_row(i, h);
-                        const int code = r < n ? min((int)code_at[r * code_stride + kc], nb) : nb;
-                        const float x = fmaf(s[i], scale, table[code]) + st[32 * t + reg_row(i, h)];
-                        s[i] = code < nb ? x : -INFINITY;
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int r = 32 * t + 8 * g4 + 4 * h;
+                        const uint32_t four = Codes::read(codes + turn * 32 * NW * BQ, k - at.first, r);
+                        const f32x4 ref = *(const f32x4 *)(st + r);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int code = code_of(four, e, nb);
+                            const float x = fmaf(s[4 * g4 + e], scale, look_up(table, code)) + ref[e];
+                            s[4 * g4 + e] = code < nb && q0 + r + e < n ? x : -INFINITY;
+                        }
                     }
                 }
-                if (BIAS || (causal && qt < k0 + 31)) {
-                    const int least = causal ? k : 0;
+                if (causal && qt < k0 + 31) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[i] = qt + reg_row(i, h) >= least ? s[i] : -INFINITY;
-                        d[i] = s[i] > -INFINITY ? d[i] : 0.f;
-                    }
+                    for (int i = 0; i < 16; ++i) s[i] = qt + reg_row(i, h) >= k ? s[i] : -INFINITY;
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     s[i] = exp2_fast(s[i] * c);
-                    d[i] *= s[i];
+                    d[i] = weigh(s[i], d[i]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -792,15 +872,14 @@ int launch_kernel(K kernel, long long grid, int threads, size_t lds, const RwkAt
 template <typename T, int KS, bool WIDE, bool BIAS, bool ASYNC>
 int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
     constexpr int NW = WIDE ? 4 : 1, NT = 64 * NW, ROWS = tile_rows<T, NW>();
+    constexpr int LDS = tiles_bytes<T, KS, ROWS>() + (BIAS ? code_bytes<NW, ROWS>() : 0);
     if (pass == kRwkAttnForward)
-        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
-                             tiles_bytes<T, KS, ROWS>() + 64 * sizeof(float), p, stream);
+        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT, LDS, p, stream);
     if (pass == kRwkAttnDq)
         return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
-                             tiles_bytes<T, KS, ROWS>() + (64 + (BIAS ? (p.a.n_buckets + 1) * NT : 0)) * sizeof(float), p,
-                             stream);
+                             LDS + (BIAS ? p.a.n_buckets * NT * sizeof(float) : 0), p, stream);
     return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT,
-                         dkv_lds<T, KS, NW>(), p, stream);
+                         dkv_lds<T, KS, NW, BIAS>(), p, stream);
 }
 
 // Rows whose elements are whole 16-byte chunks at 16-byte addresses, not too far apart for 32-bit offsets inside a

@@ -971,7 +971,8 @@ typedef struct {
     int32_t block_rows;             /* rows of a block: 32 or 128 */
     float *stats;                   /* (heads, rows, 2): row maximum and 1 / sum; NULL if no backward pass follows */
     float *delta;                   /* (heads, rows), written by the backward pass */
-    const uint8_t *codes;           /* rwk_pair_buckets_*; NULL without a bias */
+    const uint8_t *codes;           /* rwk_pair_buckets_*, query rows; NULL without a bias */
+    const uint8_t *codes_by_key;    /* the same, key rows; backward only */
     const int64_t *code_start;      /* first byte of every segment's codes */
     const void *table;              /* (heads, n_buckets) of `type` */
     int64_t n_buckets;              /* 0 without a bias, else 1 .. 32 */
@@ -988,20 +989,21 @@ int rwk_attention_backward(const rwk_attention *a, rwk_stream_t stream);
 
 /* Bucket codes of all ordered pairs (query row, key row) of every segment, as rwk_attention reads them: a segment of
  * n rows has n rows of codes, each padded to a multiple of 32 with 255 (a code that never attends), from byte
- * code_start[g].  From a dense list (segment after segment, n * n codes each, from byte pair_start[g]), ... */
+ * code_start[g] (a multiple of 16, as `codes` itself).  `codes` has a row per query, `codes_by_key` a row per key.
+ * items, n_items, block_rows: as in rwk_attention.  From a dense list (segment after segment, n * n codes each, from byte pair_start[g]), ... */
 int rwk_pair_buckets_dense(const uint8_t *dense, const int64_t *pair_start, const int32_t *seg_ptr,
-                           const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
-                           rwk_stream_t stream);
+                           const int64_t *code_start, const int32_t *items, int64_t n_items, int32_t block_rows,
+                           uint8_t *codes, uint8_t *codes_by_key, rwk_stream_t stream);
 /* ... from the difference j - i of the rows' places, clamped to [-reach, reach], through a table of 2 * reach + 1
  * codes, ... */
 int rwk_pair_buckets_relative(const uint8_t *by_offset, int64_t reach, const int32_t *seg_ptr,
-                              const int64_t *code_start, int64_t n_segments, int64_t rows, uint8_t *codes,
-                              rwk_stream_t stream);
+                              const int64_t *code_start, const int32_t *items, int64_t n_items, int32_t block_rows,
+                              uint8_t *codes, uint8_t *codes_by_key, rwk_stream_t stream);
 /* ... or from hop distances as rwk_khop_fill lists them: 0 for a row itself, the distance for the pairs listed,
- * far_code for the others. */
+ * far_code for the others.  Distances are symmetric: `codes` is codes_by_key, too. */
 int rwk_pair_buckets_hops(const int32_t *row_start, const int32_t *col, const int32_t *dist, int32_t far_code,
-                          const int32_t *seg_ptr, const int64_t *code_start, int64_t n_segments, int64_t rows,
-                          uint8_t *codes, rwk_stream_t stream);
+                          const int32_t *seg_ptr, const int64_t *code_start, const int32_t *items, int64_t n_items,
+                          int32_t block_rows, uint8_t *codes, rwk_stream_t stream);
 
 #ifdef __cplusplus
 }

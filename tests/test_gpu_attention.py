@@ -375,6 +375,8 @@ def test_dense_and_relative_codes(dev):
     codes = [torch.randint(0, 256, (n, n), device=dev).to(torch.uint8) for n in lengths]
     b = pair_buckets(seg, torch.cat([c.reshape(-1) for c in codes]))
     assert all(torch.equal(b.dense(i), c) for i, c in enumerate(codes))
+    b._codes = b._by_key                            # the copy with a row per key
+    assert all(torch.equal(b.dense(i), c.t()) for i, c in enumerate(codes))
     for n_buckets, reach, both in ((32, 128, True), (8, 20, False), (2, 5, True), (1, 9, False)):
         got = relative_buckets(seg, n_buckets, reach, both)
         per = n_buckets // 2 if both else n_buckets
@@ -389,6 +391,9 @@ def test_dense_and_relative_codes(dev):
                         math.log(d / exact) / math.log(reach / exact) * (per - exact))))
                     want[r, c] = bucket + (per if both and c > r else 0)
             assert np.array_equal(got.dense(i).cpu().numpy(), want), (n_buckets, i)
+        got._codes = got._by_key
+        assert np.array_equal(got.dense(3).cpu().numpy()[5, 7], relative_buckets(seg, n_buckets, reach, both).dense(
+            3).cpu().numpy()[7, 5])
 
 
 @pytest.mark.parametrize("far", ["bucket", "mask"])

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-NULL, SIZE, UNSUPPORTED = -1, -2, -3
+NULL, SIZE, UNSUPPORTED, ALIGN = -1, -2, -3, -4
 A = 4096          # stands for a device address: every call below returns before it would be used
 
 
@@ -64,13 +64,13 @@ def test_attention_entry_points(lib):
             setattr(a, name, value)
         return (lib.rwk_attention_backward if backward else lib.rwk_attention_forward)(ctypes.addressof(a), None)
     assert lib.rwk_attention_forward(None, None) == NULL and lib.rwk_attention_backward(None, None) == NULL
-    biased = dict(n_buckets=4, table=A, codes=A, code_start=A, d_table=A, d_table_partials=A)
+    biased = dict(n_buckets=4, table=A, codes=A, codes_by_key=A, code_start=A, d_table=A, d_table_partials=A)
     for backward in (False, True):
         names = ["q", "k", "v", "out", "seg_ptr", "q_items"]
         names += ["d_out", "dq", "dk", "dv", "stats", "delta", "k_items"] if backward else []
         for name in names:
             assert call(backward, **{name: None}) == NULL, name
-        for name in ["table", "codes", "code_start"] + (["d_table", "d_table_partials"] if backward else []):
+        for name in ["table", "codes", "code_start"] + (["codes_by_key", "d_table", "d_table_partials"] if backward else []):
             assert call(backward, **(biased | {name: None})) == NULL, name
         for bad in (dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(dim=0), dict(rows=-1), dict(rows=1 << 31),
                     dict(n_segments=-1), dict(n_items=-1), dict(n_items=1 << 30), dict(scale=0.0), dict(scale=-1.0),
@@ -78,24 +78,28 @@ def test_attention_entry_points(lib):
             assert call(backward, **bad) == SIZE, bad
         for bad in (dict(dim=129), dict(type=3), dict(type=-1), dict(block_rows=64), biased | dict(n_buckets=33)):
             assert call(backward, **bad) == UNSUPPORTED, bad
+        assert call(backward, **(biased | dict(codes=A + 8))) == ALIGN
     assert call(n_items=0, q=None, seg_ptr=None) == 0          # nothing to do
 
 
 def test_pair_bucket_entry_points(lib):
-    dense = lambda *a: lib.rwk_pair_buckets_dense(*a)
-    assert dense(A, A, A, A, 1, -1, A, None) == SIZE and dense(A, A, A, A, 0, 5, A, None) == SIZE
-    assert dense(A, A, A, A, 1, 1 << 31, A, None) == SIZE and dense(A, A, A, A, 1 << 31, 5, A, None) == SIZE
-    for i in (0, 1, 2, 3, 6):
-        args = [A, A, A, A, 1, 5, A, None]
-        args[i] = None
-        assert dense(*args) == NULL, i
-    assert dense(None, None, None, None, 0, 0, None, None) == 0
-    rel = lib.rwk_pair_buckets_relative
-    assert rel(A, -1, A, A, 1, 5, A, None) == SIZE and rel(A, 1 << 40, A, A, 1, 5, A, None) == SIZE
-    assert rel(None, 4, A, A, 1, 5, A, None) == NULL and rel(A, 4, None, A, 1, 5, A, None) == NULL
-    hops = lib.rwk_pair_buckets_hops
-    assert hops(A, A, A, -1, A, A, 1, 5, A, None) == SIZE and hops(A, A, A, 256, A, A, 1, 5, A, None) == SIZE
-    assert hops(None, A, A, 4, A, A, 1, 5, A, None) == NULL
+    def refused(entry, *front, outputs):
+        good = [*front, A, A, A, 3, 32, *[A] * outputs, None]
+        at = len(front)
+        call = lambda i, v: entry(*[v if j == i else x for j, x in enumerate(good)])
+        for i in (0, at, at + 1, at + 2, *range(at + 5, at + 5 + outputs)):
+            assert call(i, None) == NULL, i
+        assert call(at + 3, -1) == SIZE and call(at + 3, 1 << 31) == SIZE and call(at + 4, 64) == UNSUPPORTED
+        for i in range(at + 5, at + 5 + outputs):
+            assert call(i, A + 8) == ALIGN, i
+        return call
+    dense = refused(lib.rwk_pair_buckets_dense, A, A, outputs=2)
+    assert dense(1, None) == NULL
+    relative = refused(lib.rwk_pair_buckets_relative, A, 4, outputs=2)
+    assert relative(1, -1) == SIZE and relative(1, 1 << 40) == SIZE
+    hops = refused(lib.rwk_pair_buckets_hops, A, A, A, 4, outputs=1)
+    assert hops(3, -1) == SIZE and hops(3, 256) == SIZE
+    assert lib.rwk_pair_buckets_dense(None, None, None, None, None, 0, 32, None, None, None) == 0
 
 
 def test_no_cpu_fallback():
