@@ -10,6 +10,8 @@ import ctypes
 import os
 from ctypes import c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librwk.so")
 
@@ -187,10 +189,12 @@ def check(code: int, what: str):
         raise RwkError(f"{what} failed: {msg} (code {code})")
 
 
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
 def element_type(dtype):
     """``RWK_F32`` / ``RWK_F16`` / ``RWK_BF16`` of a torch dtype; ``TypeError`` for any other."""
-    import torch
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    code = _TYPES.get(dtype)
     if code is None:
         raise TypeError("expected float32, float16 or bfloat16, got %s" % dtype)
     return code
@@ -204,7 +208,6 @@ def ptr(t):
 def current_stream(device):
     """Raw ``hipStream_t`` of torch's current stream on ``device`` (no Stream object is built: this is called
     several times per training step)."""
-    import torch
     idx = device.index if device.index is not None else torch.cuda.current_device()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is not None:
@@ -226,7 +229,6 @@ _NO_GUARD = _NoGuard()
 def device_guard(device):
     """``torch.cuda.device(device)``, or a no-op context when ``device`` is already the current one (the usual
     case: one process per GPU; autograd's worker thread runs a backward on the device of its inputs)."""
-    import torch
     if device.index is None or torch.cuda.current_device() == device.index:
         return _NO_GUARD
     return torch.cuda.device(device)

@@ -14,8 +14,9 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / RWK_WAVE;
 
-// Sum over the TPR threads that share a row (a part of a wavefront, a wavefront or the workgroup), to all of them.
-// `red` holds kWaves floats and is used by workgroup-wide rows only; two alternating buffers save a barrier.
+// Sums over the TPR threads that share a row (a part of a wavefront, a wavefront or the workgroup), to all of them.
+// `red` holds kWaves entries and is used by workgroup-wide rows only; the callers alternate between two of them, which
+// saves the barrier after the reads.
 template <int TPR>
 __device__ inline float row_sum(float v, float *red) {
     if (TPR <= RWK_WAVE) return rwk_group_sum(v, TPR);
@@ -28,19 +29,42 @@ __device__ inline float row_sum(float v, float *red) {
     return s;
 }
 
+template <int TPR>
+__device__ inline void row_sums(float &a, float &c, float2 *red) {
+    if (TPR <= RWK_WAVE) {
+        a = rwk_group_sum(a, TPR);
+        c = rwk_group_sum(c, TPR);
+        return;
+    }
+    a = rwk_wave_sum(a);
+    c = rwk_wave_sum(c);
+    if ((threadIdx.x & (RWK_WAVE - 1)) == 0) red[threadIdx.x / RWK_WAVE] = make_float2(a, c);
+    __syncthreads();
+    a = c = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        a += red[w].x;
+        c += red[w].y;
+    }
+}
+
 // The V * IT elements of a row that thread t of TPR holds: vectors t, t + TPR, ...  Beyond the row: zeros.
-template <typename T, int TPR, int V, int IT>
-__device__ inline void load_row(const T *__restrict__ row, int width, int t, float (&out)[IT * V]) {
+template <typename T, int V, int IT>
+struct Row {
+    typename RwkPack<T, V>::type v[IT];
+    __device__ float at(int i) const { return (float)v[i / V][i % V]; }
+};
+
+template <int TPR, typename T, int V, int IT>
+__device__ inline void load_row(const T *__restrict__ row, int width, int t, Row<T, V, IT> &out) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int c = (t + i * TPR) * V;
         if (c + V <= width) {
-            const auto v = rwk_load<T, V>(row + c);
-#pragma unroll
-            for (int j = 0; j < V; ++j) out[i * V + j] = (float)v[j];
+            out.v[i] = rwk_load<T, V>(row + c);
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) out[i * V + j] = c + j < width ? (float)row[c + j] : 0.f;
+            for (int j = 0; j < V; ++j) out.v[i][j] = c + j < width ? row[c + j] : (T)0.f;
         }
     }
 }
@@ -71,30 +95,35 @@ norm_forward_kernel(const T *__restrict__ x, long long x_stride, const W *__rest
     __shared__ float red[2][kWaves];
     constexpr int kRows = kBlock / TPR;
     const int t = threadIdx.x % TPR;
-    for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows) {
-        const long long r = r0 + threadIdx.x / TPR;
-        const bool there = r < rows;                  // the whole workgroup takes part in the sums
-        float v[IT * V];
-        load_row<T, TPR, V, IT>(x + (there ? r : rows - 1) * x_stride, width, t, v);
-        float s = 0.f;
+    const long long step = (long long)gridDim.x * kRows;
+    Row<W, V, IT> w, b;
+    load_row<TPR>(weight, width, t, w);
+    if (bias != nullptr) load_row<TPR>(bias, width, t, b);
+    // the next row is on its way while this one is summed
+    long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    Row<T, V, IT> next;
+    load_row<TPR>(x + (r < rows ? r : rows - 1) * x_stride, width, t, next);
+    for (; r - threadIdx.x / TPR < rows; r += step) {       // the whole workgroup takes part in the sums
+        const bool there = r < rows;
+        float v[IT * V], s = 0.f;
 #pragma unroll
-        for (int i = 0; i < IT * V; ++i) s += v[i];
+        for (int i = 0; i < IT * V; ++i) {
+            v[i] = next.at(i);
+            s += v[i];
+        }
+        if (r + step - threadIdx.x / TPR < rows)
+            load_row<TPR>(x + (r + step < rows ? r + step : rows - 1) * x_stride, width, t, next);
         const float mean = row_sum<TPR>(s, red[0]) / (float)width;    // exact for constant rows
         float q = 0.f;
 #pragma unroll
-        for (int i = 0; i < IT; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = (t + i * TPR) * V + j < width ? v[i * V + j] - mean : 0.f;
-                v[i * V + j] = d;
-                q = fmaf(d, d, q);
-            }
+        for (int i = 0; i < IT * V; ++i) {
+            v[i] = (t + i / V * TPR) * V + i % V < width ? v[i] - mean : 0.f;
+            q = fmaf(v[i], v[i], q);
+        }
         const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / (float)width + eps);
-        float w[IT * V], b[IT * V];
-        load_row<W, TPR, V, IT>(weight, width, t, w);
-        if (bias != nullptr) load_row<W, TPR, V, IT>(bias, width, t, b);
 #pragma unroll
-        for (int i = 0; i < IT * V; ++i) v[i] = bias != nullptr ? fmaf(v[i] * rstd, w[i], b[i]) : v[i] * rstd * w[i];
+        for (int i = 0; i < IT * V; ++i)
+            v[i] = bias != nullptr ? fmaf(v[i] * rstd, w.at(i), b.at(i)) : v[i] * rstd * w.at(i);
         if (!there) continue;
         store_row<T, TPR, V, IT>(y + r * width, width, t, v);
         if (t == 0 && mean_out != nullptr) {
@@ -112,36 +141,48 @@ norm_backward_kernel(const T *__restrict__ x, long long x_stride, const T *__res
                      const float *__restrict__ rstd_in, long long rows, int width, T *__restrict__ dx,
                      float *__restrict__ partials) {
     constexpr int kRows = kBlock / TPR;
-    __shared__ float red[2][2][kWaves];
+    __shared__ float2 red[2][kWaves];
     const int t = threadIdx.x % TPR;
+    const long long step = (long long)gridDim.x * kRows;
     const float inv = 1.f / (float)width;
-    float w[IT * V], dw[IT * V], db[IT * V];
-    load_row<W, TPR, V, IT>(weight, width, t, w);
+    Row<W, V, IT> w;
+    load_row<TPR>(weight, width, t, w);
+    float dw[IT * V], db[IT * V];
 #pragma unroll
     for (int i = 0; i < IT * V; ++i) dw[i] = db[i] = 0.f;
-    int turn = 0;
-    for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows, turn ^= 1) {
-        const long long r = r0 + threadIdx.x / TPR;
+    // the next row is on its way while this one is summed
+    Row<T, V, IT> x_next, g_next;
+    float mean_next, rstd_next;
+    const auto fetch = [&](long long r) {
+        const long long rc = r < rows ? r : rows - 1;
+        load_row<TPR>(x + rc * x_stride, width, t, x_next);
+        load_row<TPR>(dy + rc * dy_stride, width, t, g_next);
+        mean_next = mean_in[rc];
+        rstd_next = rstd_in[rc];
+    };
+    long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    fetch(r);
+    for (int turn = 0; r - threadIdx.x / TPR < rows; r += step, turn ^= 1) {
+        const Row<T, V, IT> xr = x_next, gr = g_next;
+        const float mean = mean_next, rstd = rstd_next;
         const bool there = r < rows;
-        const long long rc = there ? r : rows - 1;
-        float h[IT * V], g[IT * V];
-        load_row<T, TPR, V, IT>(x + rc * x_stride, width, t, h);
-        load_row<T, TPR, V, IT>(dy + rc * dy_stride, width, t, g);
-        const float mean = mean_in[rc], rstd = rstd_in[rc];
-        float a = 0.f, c = 0.f;
+        if (r + step - threadIdx.x / TPR < rows) fetch(r + step);
+        float h[IT * V], g[IT * V], a = 0.f, c = 0.f;
 #pragma unroll
         for (int i = 0; i < IT * V; ++i) {
-            h[i] = (h[i] - mean) * rstd;              // beyond the row: dy = 0 and w = 0 take it out
+            h[i] = (xr.at(i) - mean) * rstd;              // beyond the row: dy = 0 and w = 0 take it out
+            g[i] = gr.at(i);
             if (there) {
                 dw[i] = fmaf(g[i], h[i], dw[i]);
                 db[i] += g[i];
             }
-            g[i] *= w[i];
+            g[i] *= w.at(i);
             a += g[i];
             c = fmaf(g[i], h[i], c);
         }
-        a = row_sum<TPR>(a, red[turn][0]) * inv;
-        c = row_sum<TPR>(c, red[turn][1]) * inv;
+        row_sums<TPR>(a, c, red[turn]);
+        a *= inv;
+        c *= inv;
 #pragma unroll
         for (int i = 0; i < IT * V; ++i) h[i] = rstd * (g[i] - a - h[i] * c);
         if (there) store_row<T, TPR, V, IT>(dx + r * width, width, t, h);
@@ -238,8 +279,8 @@ norm_weight_wide_kernel(const T *__restrict__ x, long long x_stride, const T *__
     out[width + c] = db;
 }
 
-// dw, db = column sums of the partial rows [dw | db], in row order within 16 fixed groups, then in group order
-constexpr int kSumCols = 64, kSumGroups = 16;
+// dw, db = column sums of the partial rows [dw | db], in row order within 32 fixed groups, then in group order
+constexpr int kSumCols = 32, kSumGroups = 32;
 template <typename W>
 __global__ void __launch_bounds__(kSumCols * kSumGroups)
 norm_weight_sum_kernel(const float *__restrict__ partials, int n_partials, int width, W *__restrict__ dw,
@@ -249,6 +290,7 @@ norm_weight_sum_kernel(const float *__restrict__ partials, int n_partials, int w
     const long long c = (long long)blockIdx.x * kSumCols + lane;
     float s = 0.f;
     if (c < 2ll * width)
+#pragma unroll 16
         for (int p = group; p < n_partials; p += kSumGroups) s += partials[(long long)p * 2 * width + c];
     part[group][lane] = s;
     __syncthreads();
@@ -264,27 +306,27 @@ norm_weight_sum_kernel(const float *__restrict__ partials, int n_partials, int w
 // ---------------------------------------------------------------------------------------------------------------
 // Launch shapes.  Threads per row: as few as hold the row in one vector each up to a wavefront, so that narrow rows
 // (node features of a few channels) still fill every lane; wider rows give each lane of a wavefront, then of a
-// workgroup, more vectors.  The backward pass keeps two column sums per element besides the row and turns to the
-// workgroup earlier.
+// workgroup, more vectors.  A wavefront alone needs no barrier: up to 256 vectors it is at least as fast as a workgroup
+// (65536 x 1024 bf16 forward 45 us = 6.0 TB/s; 40000 x 2048 fp16 53), at 512 its registers leave too few rows in flight
+// (32768 x 4096 bf16: 148 us, by workgroups 96 = 5.6 TB/s).  The backward pass keeps two column sums per element besides
+// the row and turns to the workgroup at 128.  A large copy runs at 5.1 TB/s on the same card.
+// Workgroups are few enough to stay resident and walk over the rows.  In the backward pass each also leaves a row of
+// partial sums: 512 of them are faster than 1024 for workgroup-wide rows (32768 x 4096 bf16: 150 + 5 us against
+// 169 + 8), but not for rows at odd addresses, whose loads take longer (16384 x 2001: 82 against 63) and narrow ones.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kMaxGrid = 4096;
-constexpr int kBackwardGrid = 1024;     // workgroups of the backward pass, each with one row of partial sums
 constexpr int kWideSplit = 64;
 
 constexpr int kRegisterWidth = 8192;    // wider rows do not fit a workgroup's registers
 
-int rows_per_block(int64_t width, int vec) {
-    const int64_t vectors = rwk_ceil_div(width, vec);
-    if (vectors <= 4) return kBlock / 4;
-    if (vectors <= 16) return kBlock / 16;
-    if (vectors <= 128) return kBlock / 64;
-    return 1;
+int row_threads(int64_t vectors) {         // of the backward pass
+    return vectors <= 4 ? 4 : vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : vectors <= 128 ? 64 : 256;
 }
 
 int64_t backward_blocks(int64_t rows, int64_t width, int vec) {
     if (width > kRegisterWidth) return rows < kWideSplit ? rows : kWideSplit;
-    const int64_t blocks = rwk_ceil_div(rows, rows_per_block(width, vec));
-    return blocks < kBackwardGrid ? blocks : kBackwardGrid;
+    const int threads = row_threads(rwk_ceil_div(width, vec));
+    const int64_t blocks = rwk_ceil_div(rows, kBlock / threads), most = threads == kBlock && width % vec == 0 ? 512 : 1024;
+    return blocks < most ? blocks : most;
 }
 
 struct NormArgs {
@@ -302,7 +344,8 @@ template <typename T, typename W, int TPR, int IT>
 int launch_forward(const NormArgs &a) {
     constexpr int V = RwkVecOf<T>::n;
     long long grid = rwk_ceil_div(a.rows, kBlock / TPR);
-    if (grid > kMaxGrid) grid = kMaxGrid;
+    constexpr long long kMost = TPR < RWK_WAVE ? 4096 : 2048;
+    if (grid > kMost) grid = kMost;
     hipLaunchKernelGGL((norm_forward_kernel<T, W, TPR, V, IT>), dim3((unsigned)grid), dim3(kBlock), 0, a.stream,
                        (const T *)a.x, a.x_stride, (const W *)a.weight, (const W *)a.bias, a.rows, a.width, a.eps,
                        (T *)a.out, a.mean, a.rstd);
@@ -315,10 +358,12 @@ int forward(const NormArgs &a) {
     constexpr int V = RwkVecOf<T>::n;
     const int64_t vectors = rwk_ceil_div(a.width, V);
     if (vectors <= 4) return launch_forward<T, W, 4, 1>(a);
+    if (vectors <= 8) return launch_forward<T, W, 8, 1>(a);
     if (vectors <= 16) return launch_forward<T, W, 16, 1>(a);
+    if (vectors <= 32) return launch_forward<T, W, 32, 1>(a);
     if (vectors <= 64) return launch_forward<T, W, 64, 1>(a);
     if (vectors <= 128) return launch_forward<T, W, 64, 2>(a);
-    if (vectors <= 256) return launch_forward<T, W, 256, 1>(a);
+    if (vectors <= 256) return launch_forward<T, W, 64, 4>(a);
     if (vectors <= 512) return launch_forward<T, W, 256, 2>(a);
     if (vectors <= 1024) return launch_forward<T, W, 256, 4>(a);
     if (vectors <= 2048 && V == 4) return launch_forward<T, W, 256, 8>(a);
@@ -358,8 +403,12 @@ int backward(const NormArgs &a) {
         RWK_LAUNCH_CHECK();
     } else if (vectors <= 4) {
         code = launch_backward<T, W, 4, 1>(a, blocks);
+    } else if (vectors <= 8) {
+        code = launch_backward<T, W, 8, 1>(a, blocks);
     } else if (vectors <= 16) {
         code = launch_backward<T, W, 16, 1>(a, blocks);
+    } else if (vectors <= 32) {
+        code = launch_backward<T, W, 32, 1>(a, blocks);
     } else if (vectors <= 64) {
         code = launch_backward<T, W, 64, 1>(a, blocks);
     } else if (vectors <= 128) {

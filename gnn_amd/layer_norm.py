@@ -16,16 +16,16 @@ from . import _lib
 __all__ = ["layer_norm", "LayerNorm"]
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as (rows, width) with adjacent elements in a row and rows at least a width apart; a view if it can be."""
-    t = t.reshape(-1, t.shape[-1])
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+def _rows(t: torch.Tensor):
+    """``t`` as (rows, width) with adjacent elements in a row and rows at least a width apart - a view if it can be -
+    and the rows' distance in elements."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, width
+    t = t.reshape(-1, width)
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
         t = t.contiguous()
-    return t
-
-
-def _stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t, t.stride(0) if t.shape[0] > 1 else width
 
 
 def _check(x, weight, bias):
@@ -47,58 +47,55 @@ def _check(x, weight, bias):
         raise TypeError("weight and bias must have the same type")
 
 
-def _forward(x, weight, bias, eps, stats):
-    """(y, mean, rstd, rows): ``rows`` is x as the kernel read it."""
-    rows = _rows(x)
-    n, width = rows.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
+def _forward(x, weight, bias, eps, keep):
+    """(y, stats, rows, stride): ``rows`` is x as the kernel read it, ``stats`` the rows' mean and 1 / deviation."""
+    rows, stride = _rows(x)
+    width, dev = x.shape[-1], x.device
+    n = x.numel() // width
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = mean = rstd = None
+    if keep:
+        stats = torch.empty((2, n), dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
     if n:
         w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        with _lib.device_guard(x.device):
+        with _lib.device_guard(dev):
             _lib.check(_lib.load().rwk_layer_norm_forward(
-                rows.data_ptr(), _stride(rows), w.data_ptr(), _lib.ptr(b), n, width, _lib.element_type(x.dtype),
-                _lib.element_type(w.dtype), eps, y.data_ptr(), _lib.ptr(mean), _lib.ptr(rstd),
-                _lib.current_stream(x.device)), "rwk_layer_norm_forward")
-    return y, mean, rstd, rows
+                rows.data_ptr(), stride, w.data_ptr(), _lib.ptr(b), n, width, _lib.element_type(x.dtype),
+                _lib.element_type(w.dtype), eps, y.data_ptr(), mean, rstd, _lib.current_stream(dev)),
+                "rwk_layer_norm_forward")
+    return y, stats, rows, stride
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd, rows = _forward(x.detach(), weight.detach(), None if bias is None else bias.detach(), eps, True)
-        ctx.save_for_backward(rows, weight, mean, rstd)
+        y, stats, rows, ctx.stride = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, stats)
         ctx.has_bias = bias is not None
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        rows, weight, mean, rstd = ctx.saved_tensors
-        n, width = rows.shape
-        shape = dy.shape
-        # one allocation for dw and db
-        dwb = torch.empty((2, width), dtype=weight.dtype, device=rows.device)
+        rows, weight, stats = ctx.saved_tensors
+        n, width, dev = stats.shape[1], dy.shape[-1], dy.device
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+        dw, db = torch.empty((2, width), dtype=weight.dtype, device=dev).unbind(0)
         if n == 0:
-            dwb.zero_()
-            return torch.empty(shape, dtype=rows.dtype, device=rows.device), dwb[0], \
-                dwb[1] if ctx.has_bias else None, None
-        dy = _rows(dy)
-        w = weight.contiguous()
-        lib = _lib.load()
-        code = _lib.element_type(rows.dtype)
-        dx = torch.empty(shape, dtype=rows.dtype, device=rows.device)
-        blocks = lib.rwk_layer_norm_backward_blocks(n, width, code)
-        partials = torch.empty((blocks, 2 * width), dtype=torch.float32, device=rows.device)
-        dw, db = dwb.unbind(0)
-        with _lib.device_guard(rows.device):
+            return dx, dw.zero_(), db.zero_() if ctx.has_bias else None, None
+        dy, dy_stride = _rows(dy)
+        lib, code = _lib.load(), _lib.element_type(dx.dtype)
+        partials = torch.empty((lib.rwk_layer_norm_backward_blocks(n, width, code), 2 * width), dtype=torch.float32,
+                               device=dev)
+        mean = stats.data_ptr()
+        with _lib.device_guard(dev):
             _lib.check(lib.rwk_layer_norm_backward(
-                rows.data_ptr(), _stride(rows), dy.data_ptr(), _stride(dy), w.data_ptr(), mean.data_ptr(),
-                rstd.data_ptr(), n, width, code, _lib.element_type(w.dtype), dx.data_ptr(), partials.data_ptr(),
-                dw.data_ptr(), db.data_ptr(), _lib.current_stream(rows.device)), "rwk_layer_norm_backward")
+                rows.data_ptr(), ctx.stride, dy.data_ptr(), dy_stride, weight.contiguous().data_ptr(), mean,
+                mean + 4 * n, n, width, code, _lib.element_type(weight.dtype), dx.data_ptr(), partials.data_ptr(),
+                dw.data_ptr(), db.data_ptr(), _lib.current_stream(dev)), "rwk_layer_norm_backward")
         return dx, dw, db if ctx.has_bias else None, None
 
 
