@@ -4,9 +4,9 @@
 //   p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 //
 // Bound by memory: per element p, m, v in and out and g in (28 bytes for fp32 with 32-bit states, 16 with 8-bit
-// states, 10 for 16-bit weights with 8-bit states).  The tensors are cut into chunks of kChunk elements, one
-// workgroup each; a table on the device says which tensor a chunk belongs to, the gradients' addresses - the only
-// ones that change from step to step - travel in the launch's arguments, so a step copies nothing to the device.
+// states, 10 for 16-bit weights with 8-bit states).  The tensors are cut into chunks, one workgroup
+// each; a table on the device describes them, the gradients' addresses - the only ones that change from step to step -
+// travel in the launch's arguments, so a step copies nothing to the device.
 // Every chunk counts its own steps (a tensor without a gradient is skipped and does not age), so a captured launch
 // replays correctly.
 //
@@ -26,8 +26,11 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kStateBlock = 256;                       // elements that share a scale: one wavefront, four per lane
-constexpr int kPerWave = 4;                            // blocks per wavefront, loaded together
-constexpr int kChunk = kBlock / RWK_WAVE * kPerWave * kStateBlock;
+// Blocks per wavefront, loaded together: four where there are chunks enough for every compute unit that way (50 M fp32
+// elements with 32-bit states 264 us, 5.3 TB/s), one for few elements, whose time is latency (1.3 M with 8-bit states:
+// 11.5 us by four, 8.9 by one).
+constexpr int chunk_elements(int per_wave) { return kBlock / RWK_WAVE * per_wave * kStateBlock; }
+constexpr int64_t kFewElements = 4 << 20;
 constexpr int kTensors = RWK_ADAMW_TENSORS;            // gradient addresses of one launch
 
 struct AdamwGrads {
@@ -101,27 +104,34 @@ __device__ inline void f8_decode(uint32_t codes, float scale, float (&out)[4]) {
     out[3] = hi[1] * scale;
 }
 
-template <typename T, bool STATE8>
-__global__ void __launch_bounds__(kBlock)
-adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk *__restrict__ chunks, int tensor_base,
-             AdamwGrads grads, const double *__restrict__ lr_ptr, AdamwHyper hyper,
-             long long *__restrict__ chunk_steps) {
-    const rwk_adamw_chunk chunk = chunks[blockIdx.x];
-    const T *grad = (const T *)grads.grad[chunk.tensor - tensor_base];
-    if (grad == nullptr) return;
-    const rwk_adamw_tensor t = tensors[chunk.tensor];
-    T *param = (T *)t.param;
-    const long long step = chunk_steps[blockIdx.x] + 1;
+// m / (sqrt(v) inv_root + eps) with the one-instruction root and reciprocal, good to an ulp each, on an update that is
+// a small part of the parameter; a root below 2^-63 that the instruction takes for zero counts for nothing beside eps.
+// Where eps says nothing, by the exact operations.
+constexpr float kPlainEps = 1e-12f;
+template <bool PLAIN>
+__device__ inline float ratio(float m, float v, float inv_root, float eps) {
+    if (!PLAIN && eps < kPlainEps) return m / fmaf(sqrtf(v), inv_root, eps);
+    return m * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), inv_root, eps));
+}
+
+// FULL: all of the chunk's elements exist (and eps is not tiny: ratio())
+template <typename T, bool STATE8, int kPerWave, bool FULL>
+__device__ inline void update(RwkGlobal<T> param, RwkGlobal<T> grad, const rwk_adamw_chunk &t, long long step, const double *__restrict__ lr_ptr, const AdamwHyper &hyper) {
+    const long long n = t.n, start = t.start;
+    // 32-bit states; 8-bit states by the bytes, and their scales
+    const RwkGlobal<float> avg = rwk_global<float>(t.exp_avg), avg_sq = rwk_global<float>(t.exp_avg_sq);
+    const RwkGlobal<uint8_t> avg8 = rwk_global<uint8_t>(t.exp_avg), avg_sq8 = rwk_global<uint8_t>(t.exp_avg_sq);
+    const RwkGlobal<float> scale = rwk_global<float>(t.exp_avg_scale), scale_sq = rwk_global<float>(t.exp_avg_sq_scale);
     const int lane = threadIdx.x & (RWK_WAVE - 1), wave = threadIdx.x / RWK_WAVE;
 
     float p[kPerWave][4], g[kPerWave][4], m[kPerWave][4], v[kPerWave][4];
-    const long long first = chunk.start + (long long)wave * kPerWave * kStateBlock + 4 * lane;
+    const long long first = start + (long long)wave * kPerWave * kStateBlock + 4 * lane;
 #pragma unroll
     for (int k = 0; k < kPerWave; ++k) {
         const long long i = first + (long long)k * kStateBlock;
 #pragma unroll
         for (int j = 0; j < 4; ++j) p[k][j] = g[k][j] = m[k][j] = v[k][j] = 0.f;
-        if (i + 4 <= t.n) {
+        if (FULL || i + 4 <= n) {
             const auto pv = rwk_load<T, 4>(param + i);
             const auto gv = rwk_load<T, 4>(grad + i);
 #pragma unroll
@@ -130,8 +140,8 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
                 g[k][j] = (float)gv[j];
             }
             if (!STATE8) {
-                const auto mv = rwk_load<float, 4>((const float *)t.exp_avg + i);
-                const auto vv = rwk_load<float, 4>((const float *)t.exp_avg_sq + i);
+                const auto mv = rwk_load<float, 4>(avg + i);
+                const auto vv = rwk_load<float, 4>(avg_sq + i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     m[k][j] = mv[j];
@@ -141,20 +151,20 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (i + j < t.n) {
+                if (i + j < n) {
                     p[k][j] = (float)param[i + j];
                     g[k][j] = (float)grad[i + j];
                     if (!STATE8) {
-                        m[k][j] = ((const float *)t.exp_avg)[i + j];
-                        v[k][j] = ((const float *)t.exp_avg_sq)[i + j];
+                        m[k][j] = avg[i + j];
+                        v[k][j] = avg_sq[i + j];
                     }
                 }
         }
         // the 8-bit states are padded to whole blocks: every lane of a block that begins inside the tensor reads them
-        if (STATE8 && i - 4 * lane < t.n) {
+        if (STATE8 && (FULL || i - 4 * lane < n)) {
             const long long b = (i - 4 * lane) / kStateBlock;
-            f8_decode(*(const uint32_t *)((const uint8_t *)t.exp_avg + i), t.exp_avg_scale[b], m[k]);
-            f8_decode(*(const uint32_t *)((const uint8_t *)t.exp_avg_sq + i), t.exp_avg_sq_scale[b], v[k]);
+            f8_decode(*(RwkGlobal<uint32_t>)(avg8 + i), scale[b], m[k]);
+            f8_decode(*(RwkGlobal<uint32_t>)(avg_sq8 + i), scale_sq[b], v[k]);
         }
     }
 
@@ -173,7 +183,7 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
         for (int j = 0; j < 4; ++j) {
             m[k][j] = m[k][j] * beta1 + g[k][j] * rest1;
             v[k][j] = v[k][j] * beta2 + g[k][j] * rest2 * g[k][j];
-            p[k][j] = fmaf(-size, m[k][j] / fmaf(sqrtf(v[k][j]), inv_root, hyper.eps), p[k][j] * decay);
+            p[k][j] = fmaf(-size, ratio<FULL>(m[k][j], v[k][j], inv_root, hyper.eps), p[k][j] * decay);
             if (STATE8) {
                 const float am = fabsf(m[k][j]), av = fabsf(v[k][j]);
                 // as integers: NaN is the largest
@@ -181,7 +191,7 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
                 top_v = __builtin_bit_cast(uint32_t, av) > __builtin_bit_cast(uint32_t, top_v) ? av : top_v;
             }
         }
-        if (i + 4 <= t.n) {
+        if (FULL || i + 4 <= n) {
             typename RwkPack<T, 4>::type pv;
 #pragma unroll
             for (int j = 0; j < 4; ++j) pv[j] = (T)p[k][j];
@@ -193,26 +203,26 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
                     mv[j] = m[k][j];
                     vv[j] = v[k][j];
                 }
-                rwk_store<float, 4>((float *)t.exp_avg + i, mv);
-                rwk_store<float, 4>((float *)t.exp_avg_sq + i, vv);
+                rwk_store<float, 4>(avg + i, mv);
+                rwk_store<float, 4>(avg_sq + i, vv);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (i + j < t.n) {
+                if (i + j < n) {
                     param[i + j] = (T)p[k][j];
                     if (!STATE8) {
-                        ((float *)t.exp_avg)[i + j] = m[k][j];
-                        ((float *)t.exp_avg_sq)[i + j] = v[k][j];
+                        avg[i + j] = m[k][j];
+                        avg_sq[i + j] = v[k][j];
                     }
                 }
         }
         if (STATE8) {
             const long long begin = i - 4 * lane;
-            if (begin >= t.n) continue;                       // the same for the whole wavefront
+            if (!FULL && begin >= n) continue;                       // the same for the whole wavefront
             float inv_m, inv_v;
             const float scale_m = block_scale(wave_max(top_m), &inv_m), scale_v = block_scale(wave_max(top_v), &inv_v);
-            const RwkPhilox4 r = rwk_philox4x32<7>((uint32_t)(i >> 2), (uint32_t)chunk.tensor + (uint32_t)t.id_offset,
+            const RwkPhilox4 r = rwk_philox4x32<7>((uint32_t)(i >> 2), t.stream,
                                                    (uint32_t)step, 0u, hyper.seed_lo, hyper.seed_hi);
             const uint32_t bits[4] = {r.x, r.y, r.z, r.w};
             uint32_t cm = 0, cv = 0;
@@ -225,60 +235,88 @@ adamw_kernel(const rwk_adamw_tensor *__restrict__ tensors, const rwk_adamw_chunk
                 cm |= a << (8 * j);
                 cv |= b << (8 * j);
             }
-            *(uint32_t *)((uint8_t *)t.exp_avg + i) = cm;
-            *(uint32_t *)((uint8_t *)t.exp_avg_sq + i) = cv;
+            *(RwkGlobal<uint32_t>)(avg8 + i) = cm;
+            *(RwkGlobal<uint32_t>)(avg_sq8 + i) = cv;
             if (lane == 0) {
-                t.exp_avg_scale[begin / kStateBlock] = scale_m;
-                t.exp_avg_sq_scale[begin / kStateBlock] = scale_v;
+                scale[begin / kStateBlock] = scale_m;
+                scale_sq[begin / kStateBlock] = scale_v;
             }
         }
     }
+}
+
+template <typename T, bool STATE8, int kPerWave>
+__global__ void __launch_bounds__(kBlock)
+adamw_kernel(const rwk_adamw_chunk *__restrict__ chunks, int tensor_base, AdamwGrads grads,
+             const double *__restrict__ lr_ptr, AdamwHyper hyper, long long *__restrict__ chunk_steps) {
+    const rwk_adamw_chunk chunk = chunks[blockIdx.x];
+    const long long step = chunk_steps[blockIdx.x] + 1;
+    const void *grad = grads.grad[chunk.tensor - tensor_base];
+    if (grad == nullptr) return;
+    const RwkGlobal<T> p = rwk_global<T>(chunk.param), g = rwk_global<T>((void *)grad);
+    if (chunk.start + chunk_elements(kPerWave) <= chunk.n && hyper.eps >= kPlainEps)
+        update<T, STATE8, kPerWave, true>(p, g, chunk, step, lr_ptr, hyper);
+    else
+        update<T, STATE8, kPerWave, false>(p, g, chunk, step, lr_ptr, hyper);
     if (threadIdx.x == 0) chunk_steps[blockIdx.x] = step;
 }
 
-template <typename T>
-int launch(int state_bits, const rwk_adamw_tensor *tensors, const rwk_adamw_chunk *chunks, int64_t n_chunks,
-           int tensor_base, const AdamwGrads &grads, const double *lr, const AdamwHyper &hyper, int64_t *steps,
-           hipStream_t stream) {
-    if (state_bits == 8) {
-        hipLaunchKernelGGL((adamw_kernel<T, true>), dim3((unsigned)n_chunks), dim3(kBlock), 0, stream, tensors, chunks,
-                           tensor_base, grads, lr, hyper, (long long *)steps);
-    } else {
-        hipLaunchKernelGGL((adamw_kernel<T, false>), dim3((unsigned)n_chunks), dim3(kBlock), 0, stream, tensors,
-                           chunks, tensor_base, grads, lr, hyper, (long long *)steps);
-    }
+struct AdamwLaunch {
+    const rwk_adamw_chunk *chunks;
+    unsigned n_chunks;
+    int tensor_base;
+    AdamwGrads grads;
+    const double *lr;
+    AdamwHyper hyper;
+    long long *steps;
+    hipStream_t stream;
+};
+
+template <typename T, bool STATE8, int PER>
+int launch(const AdamwLaunch &a) {
+    hipLaunchKernelGGL((adamw_kernel<T, STATE8, PER>), dim3(a.n_chunks), dim3(kBlock), 0, a.stream, a.chunks,
+                       a.tensor_base, a.grads, a.lr, a.hyper, a.steps);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
+}
+
+template <typename T>
+int launch_type(const AdamwLaunch &a, int state_bits, int64_t chunk_size) {
+    if (chunk_size == chunk_elements(1)) return state_bits == 8 ? launch<T, true, 1>(a) : launch<T, false, 1>(a);
+    return state_bits == 8 ? launch<T, true, 4>(a) : launch<T, false, 4>(a);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t rwk_adamw_chunk_size(void) { return kChunk; }
+int64_t rwk_adamw_chunk_size(int64_t n) { return n < kFewElements ? chunk_elements(1) : chunk_elements(4); }
 
-int rwk_adamw_step(const rwk_adamw_tensor *tensors, const rwk_adamw_chunk *chunks, int64_t n_chunks,
-                   int64_t tensor_base, const void *const *grads, int64_t n_grads, int32_t type, int32_t state_bits,
-                   const double *lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
-                   int64_t *chunk_steps, rwk_stream_t stream_) {
-    RWK_REQUIRE_PTR(tensors);
+int rwk_adamw_step(const rwk_adamw_chunk *chunks, int64_t n_chunks, int64_t chunk_size, int64_t tensor_base,
+                   const void *const *grads, int64_t n_grads, int32_t type, int32_t state_bits, const double *lr,
+                   double beta1, double beta2, double eps, double weight_decay, uint64_t seed, int64_t *chunk_steps,
+                   rwk_stream_t stream) {
     RWK_REQUIRE_PTR(chunks);
     RWK_REQUIRE_PTR(grads);
     RWK_REQUIRE_PTR(lr);
     RWK_REQUIRE_PTR(chunk_steps);
     if (n_chunks <= 0 || n_chunks > 0x7FFFFFFFll || tensor_base < 0 || tensor_base > 0x7FFFFFFFll || n_grads <= 0)
         return RWK_E_SIZE;
-    if (n_grads > kTensors || type < RWK_F32 || type > RWK_BF16 || (state_bits != 8 && state_bits != 32))
+    if (n_grads > kTensors || type < RWK_F32 || type > RWK_BF16 || (state_bits != 8 && state_bits != 32) ||
+        (chunk_size != chunk_elements(1) && chunk_size != chunk_elements(4)))
         return RWK_E_UNSUPPORTED;
-    AdamwGrads g;
-    for (int i = 0; i < kTensors; ++i) g.grad[i] = i < n_grads ? grads[i] : nullptr;
-    const AdamwHyper h{beta1, beta2, weight_decay, (float)eps, (uint32_t)seed, (uint32_t)(seed >> 32)};
-    hipStream_t stream = (hipStream_t)stream_;
-    if (type == RWK_F32)
-        return launch<float>(state_bits, tensors, chunks, n_chunks, (int)tensor_base, g, lr, h, chunk_steps, stream);
-    if (type == RWK_F16)
-        return launch<rwk_f16>(state_bits, tensors, chunks, n_chunks, (int)tensor_base, g, lr, h, chunk_steps, stream);
-    return launch<rwk_bf16>(state_bits, tensors, chunks, n_chunks, (int)tensor_base, g, lr, h, chunk_steps, stream);
+    AdamwLaunch a;
+    a.chunks = chunks;
+    a.n_chunks = (unsigned)n_chunks;
+    a.tensor_base = (int)tensor_base;
+    for (int i = 0; i < kTensors; ++i) a.grads.grad[i] = i < n_grads ? grads[i] : nullptr;
+    a.lr = lr;
+    a.hyper = AdamwHyper{beta1, beta2, weight_decay, (float)eps, (uint32_t)seed, (uint32_t)(seed >> 32)};
+    a.steps = (long long *)chunk_steps;
+    a.stream = (hipStream_t)stream;
+    if (type == RWK_F32) return launch_type<float>(a, state_bits, chunk_size);
+    if (type == RWK_F16) return launch_type<rwk_f16>(a, state_bits, chunk_size);
+    return launch_type<rwk_bf16>(a, state_bits, chunk_size);
 }
 
 }  // extern "C"

@@ -31,5 +31,21 @@ __device__ static inline void rwk_store(T *p, typename RwkPack<T, N>::type v) {
     *reinterpret_cast<typename RwkPack<T, N>::loose *>(p) = v;
 }
 
+// A pointer that came out of a table in memory, as one into global memory: the compiler cannot know, and accesses that
+// might be to LDS as well are slower.
+template <typename T> using RwkGlobal = __attribute__((address_space(1))) T *;
+template <typename T>
+__device__ static inline RwkGlobal<T> rwk_global(void *p) {
+    return (RwkGlobal<T>)(uintptr_t)p;
+}
+template <typename T, int N>
+__device__ static inline typename RwkPack<T, N>::type rwk_load(RwkGlobal<T> p) {
+    return *(RwkGlobal<typename RwkPack<T, N>::loose>)p;
+}
+template <typename T, int N>
+__device__ static inline void rwk_store(RwkGlobal<T> p, typename RwkPack<T, N>::type v) {
+    *(RwkGlobal<typename RwkPack<T, N>::loose>)p = v;
+}
+
 // sum over the 64 lanes, in a fixed order, to every lane
 __device__ static inline float rwk_wave_sum(float v) { return rwk_group_sum(v, 64); }

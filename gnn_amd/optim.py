@@ -322,24 +322,21 @@ class _AdamWTable:
         self.group, self.params = group, params
         self.dtype, self.device = params[0].dtype, params[0].device
         self.type = _lib.element_type(self.dtype)
-        size = int(_lib.load().rwk_adamw_chunk_size())
-        fields, steps = [], []
+        self.chunk_size = size = int(_lib.load().rwk_adamw_chunk_size(sum(p.numel() for p in params)))
+        rows, steps = [], []
         for i, (p, pid) in enumerate(zip(params, ids)):
             st = opt.state[p]
-            fields += [p.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
-                       st["exp_avg_scale"].data_ptr() if opt.state_bits == 8 else 0,
-                       st["exp_avg_sq_scale"].data_ptr() if opt.state_bits == 8 else 0, p.numel(), pid - i]
+            scales = (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()) if opt.state_bits == 8 else (0, 0)
+            rows.append((p.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), *scales, p.numel(), 0,
+                         i | pid << 32))                                               # rwk_adamw_chunk
             steps.append(int(st["step"]))
         n_chunks = -(-np.array([p.numel() for p in params], dtype=np.int64) // size)
         ends = np.cumsum(n_chunks)
         self.first_chunk = [0] + ends.tolist()
-        chunks = np.empty((int(ends[-1]), 2), dtype=np.int64)                          # rwk_adamw_chunk[]
-        chunks[:, 0] = np.repeat(np.arange(len(params)), n_chunks)
-        chunks[:, 1] = (np.arange(len(chunks)) - np.repeat(ends - n_chunks, n_chunks)) * size
-        fields = np.array(fields, dtype=np.int64)                                      # rwk_adamw_tensor[]
-        packed = torch.from_numpy(np.concatenate([fields, chunks.reshape(-1), np.repeat(steps, n_chunks)])).to(
-            self.device)                                                               # one copy to the device
-        self.table, self.chunks, self.steps = packed.split([fields.size, chunks.size, len(chunks)])
+        chunks = np.repeat(np.array(rows, dtype=np.int64), n_chunks, axis=0)
+        chunks[:, 6] = (np.arange(len(chunks)) - np.repeat(ends - n_chunks, n_chunks)) * size
+        packed = torch.from_numpy(np.concatenate([chunks.reshape(-1), np.repeat(steps, n_chunks)])).to(self.device)
+        self.chunks, self.steps = packed.split([chunks.size, len(chunks)])             # one copy to the device
         self.lr = torch.tensor([float(group["lr"])], dtype=torch.float64, device=self.device)
         self.lr_on_device = float(group["lr"])
         self.pointers = [p.data_ptr() for p in params]
@@ -380,7 +377,7 @@ class _AdamWTable:
                 if hi == lo or all(g is None for g in part):
                     continue
                 _lib.check(lib.rwk_adamw_step(
-                    self.table.data_ptr(), self.chunks.data_ptr() + 16 * lo, hi - lo, base,
+                    self.chunks.data_ptr() + 64 * lo, hi - lo, self.chunk_size, base,
                     (ctypes.c_void_p * len(part))(*part), len(part), self.type, opt.state_bits, self.lr.data_ptr(),
                     float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                     float(group["weight_decay"]), opt.seed, self.steps.data_ptr() + 8 * lo, stream),

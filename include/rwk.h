@@ -914,10 +914,11 @@ int rwk_layer_norm_backward(const void *x, int64_t x_stride, const void *dy, int
  * ------------------------------------------------------------------------------------- */
 #define RWK_ADAMW_TENSORS 256   /* gradients of one launch */
 
-/* One parameter tensor; the table of them lies on the device.  32-bit states: exp_avg and exp_avg_sq are float32 of
- * n elements, the scales are unused.  8-bit states: float8 (e4m3) values, padded to a multiple of 256 and 4-byte
- * aligned, with one float32 scale per 256 consecutive elements; a moment is value * scale.  id_offset is added to
- * the tensor's place in the table to name its random stream. */
+/* Elements [start, start + chunk size) of a parameter tensor of n elements, as far as it reaches; the table of all
+ * chunks lies on the device.  32-bit states: exp_avg and exp_avg_sq are float32 of n elements, the scales are unused.
+ * 8-bit states: float8 (e4m3) values, padded to a multiple of 256 and 4-byte aligned, with one float32 scale per 256
+ * consecutive elements; a moment is value * scale.  The addresses are those of the tensor's first element.  `tensor`
+ * is the tensor's place among the gradients of all launches, `stream` names its random numbers. */
 typedef struct {
     void *param;
     void *exp_avg;
@@ -925,25 +926,22 @@ typedef struct {
     float *exp_avg_scale;
     float *exp_avg_sq_scale;
     int64_t n;
-    int64_t id_offset;
-} rwk_adamw_tensor;
-
-/* Elements [start, start + rwk_adamw_chunk_size()) of a tensor, as far as it reaches. */
-typedef struct {
-    int64_t tensor;
     int64_t start;
+    int32_t tensor;
+    uint32_t stream;
 } rwk_adamw_chunk;
 
-int64_t rwk_adamw_chunk_size(void);
+/* Elements per chunk for tensors of n elements in all. */
+int64_t rwk_adamw_chunk_size(int64_t n);
 
-/* One step of the tensors [tensor_base, tensor_base + n_grads) of `tensors`, whose n_chunks chunks `chunks` lists.
- * grads (host): one device address per tensor, NULL = the tensor is left as it is.  Parameters and gradients are of
- * `type`, states of state_bits (8 or 32).  lr: float64[1] on the device.  chunk_steps (int64, n_chunks, device): the
- * steps taken so far per chunk, advanced here.  seed: key of the 8-bit states' rounding bits. */
-int rwk_adamw_step(const rwk_adamw_tensor *tensors, const rwk_adamw_chunk *chunks, int64_t n_chunks,
-                   int64_t tensor_base, const void *const *grads, int64_t n_grads, int32_t type, int32_t state_bits,
-                   const double *lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
-                   int64_t *chunk_steps, rwk_stream_t stream);
+/* One step of the tensors [tensor_base, tensor_base + n_grads), whose n_chunks chunks of chunk_size elements `chunks`
+ * lists.  grads (host): one device address per tensor, NULL = the tensor is left as it is.  Parameters and gradients
+ * are of `type`, states of state_bits (8 or 32).  lr: float64[1] on the device.  chunk_steps (int64, n_chunks,
+ * device): the steps taken so far per chunk, advanced here.  seed: key of the 8-bit states' rounding bits. */
+int rwk_adamw_step(const rwk_adamw_chunk *chunks, int64_t n_chunks, int64_t chunk_size, int64_t tensor_base,
+                   const void *const *grads, int64_t n_grads, int32_t type, int32_t state_bits, const double *lr,
+                   double beta1, double beta2, double eps, double weight_decay, uint64_t seed, int64_t *chunk_steps,
+                   rwk_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Attention inside packed segments (the graphs of a block-diagonal batch, walks or prompts laid end to end), causal or

@@ -40,16 +40,16 @@ def test_layer_norm_entry_points(lib):
 
 def test_adamw_entry_point(lib):
     def step(n=1, **k):
-        args = dict(tensors=A, chunks=A, n_chunks=1, base=0, grads=(ctypes.c_void_p * n)(*[A] * n), n_grads=n, type=0, bits=32, lr=A, b1=0.9, b2=0.999, eps=1e-8, wd=0.0, seed=0, steps=A,
+        args = dict(chunks=A, n_chunks=1, size=1024, base=0, grads=(ctypes.c_void_p * n)(*[A] * n), n_grads=n, type=0, bits=32, lr=A, b1=0.9, b2=0.999, eps=1e-8, wd=0.0, seed=0, steps=A,
                     stream=None) | k
         return lib.rwk_adamw_step(*args.values())
-    for name in ("tensors", "chunks", "grads", "lr", "steps"):
+    for name in ("chunks", "grads", "lr", "steps"):
         assert step(**{name: None}) == NULL, name
     for bad in (dict(n_chunks=0), dict(n_chunks=-3), dict(base=-1), dict(n_grads=0), dict(n_chunks=1 << 40)):
         assert step(**bad) == SIZE, bad
-    for bad in (dict(type=3), dict(type=-1), dict(bits=16), dict(bits=0), dict(n=257)):
+    for bad in (dict(type=3), dict(type=-1), dict(bits=16), dict(bits=0), dict(n=257), dict(size=0), dict(size=2048)):
         assert step(**bad) == UNSUPPORTED, bad
-    assert lib.rwk_adamw_chunk_size() % 256 == 0
+    assert {lib.rwk_adamw_chunk_size(n) for n in (0, 1, 10 ** 6, 10 ** 9)} == {1024, 4096}
 
 
 def test_attention_entry_points(lib):
