@@ -144,10 +144,9 @@ SIGNATURES = {
     "rwk_model_train_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rwk_model_train_pass_plan": (c_int, [_P, _P, _I64, _P, _I64, _P, _P]),
     "rwk_model_train_pass": (c_int, [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int]),
-    "rwk_layer_norm_forward": (c_int, [_P, _I64, _P, _P, _I64, _I64, c_int32, c_int32, c_float, _P, _P, _P, _P]),
+    "rwk_layer_norm_forward": (c_int, [_P, _P]),
     "rwk_layer_norm_backward_blocks": (_I64, [_I64, _I64, c_int32]),
-    "rwk_layer_norm_backward": (c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, c_int32, c_int32, _P, _P, _P, _P,
-                                        _P]),
+    "rwk_layer_norm_backward": (c_int, [_P, _P]),
     "rwk_adamw_chunk_size": (_I64, [_I64]),
     "rwk_adamw_step": (c_int, [_P, _I64, _I64, _I64, _P, _I64, c_int32, c_int32, _P, c_double, c_double, c_double,
                                c_double, c_uint64, _P, _P]),

@@ -747,6 +747,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         values.issue(at.first, v_tile);
         values.commit(v_tile);                    // there with the first tile of queries
     }
+    const T *v_own = v_tile + 32 * wave * S::W;   // the swizzle repeats: offsets as in the other tiles
     const Codes code_tiles(BIAS ? p.a.codes_by_key + p.a.code_start[at.seg] : nullptr, at.first, n);
     const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
 
@@ -810,7 +811,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                 for (int ks = 0; ks < KS; ++ks) {
                     sx = mma(row_operand<T, KS>(q_tile, 32 * t + (lane & 31), ks, h), kf[ks], sx);
                     const Frag<T> o = row_operand<T, KS>(o_tile, 32 * t + (lane & 31), ks, h);
-                    if constexpr (VL) dx = mma(o, row_operand<T, KS>(v_tile, 32 * wave + (lane & 31), ks, h), dx);
+                    if constexpr (VL) dx = mma(o, row_operand<T, KS>(v_own, lane & 31, ks, h), dx);
                     else dx = mma(o, vf[ks], dx);
                 }
                 float s[16], d[16];

@@ -329,14 +329,7 @@ int64_t backward_blocks(int64_t rows, int64_t width, int vec) {
     return blocks < most ? blocks : most;
 }
 
-struct NormArgs {
-    const void *x, *dy, *weight, *bias;
-    long long x_stride, dy_stride, rows;
-    int width;
-    float eps;
-    void *out;                    // y or dx
-    float *mean, *rstd, *partials;
-    void *dw, *db;
+struct NormArgs : rwk_layer_norm {
     hipStream_t stream;
 };
 
@@ -347,8 +340,8 @@ int launch_forward(const NormArgs &a) {
     constexpr long long kMost = TPR < RWK_WAVE ? 4096 : 2048;
     if (grid > kMost) grid = kMost;
     hipLaunchKernelGGL((norm_forward_kernel<T, W, TPR, V, IT>), dim3((unsigned)grid), dim3(kBlock), 0, a.stream,
-                       (const T *)a.x, a.x_stride, (const W *)a.weight, (const W *)a.bias, a.rows, a.width, a.eps,
-                       (T *)a.out, a.mean, a.rstd);
+                       (const T *)a.x, (long long)a.x_stride, (const W *)a.weight, (const W *)a.bias, (long long)a.rows, (int)a.width, a.eps,
+                       (T *)a.y, a.mean, a.rstd);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }
@@ -369,7 +362,7 @@ int forward(const NormArgs &a) {
     if (vectors <= 2048 && V == 4) return launch_forward<T, W, 256, 8>(a);
     if (a.rows > 0x7FFFFFFFll) return RWK_E_SIZE;
     hipLaunchKernelGGL((norm_forward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(kBlock), 0, a.stream,
-                       (const T *)a.x, a.x_stride, (const W *)a.weight, (const W *)a.bias, a.width, a.eps, (T *)a.out,
+                       (const T *)a.x, (long long)a.x_stride, (const W *)a.weight, (const W *)a.bias, (int)a.width, a.eps, (T *)a.y,
                        a.mean, a.rstd);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
@@ -379,8 +372,8 @@ template <typename T, typename W, int TPR, int IT>
 int launch_backward(const NormArgs &a, int64_t blocks) {
     constexpr int V = RwkVecOf<T>::n;
     hipLaunchKernelGGL((norm_backward_kernel<T, W, TPR, V, IT>), dim3((unsigned)blocks), dim3(kBlock), 0, a.stream,
-                       (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, (const W *)a.weight, a.mean, a.rstd,
-                       a.rows, a.width, (T *)a.out, a.partials);
+                       (const T *)a.x, (long long)a.x_stride, (const T *)a.dy, (long long)a.dy_stride, (const W *)a.weight, a.mean, a.rstd,
+                       (long long)a.rows, (int)a.width, (T *)a.dx, a.partials);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }
@@ -394,12 +387,12 @@ int backward(const NormArgs &a) {
     if (a.width > kRegisterWidth) {
         if (a.rows > 0x7FFFFFFFll) return RWK_E_SIZE;
         hipLaunchKernelGGL((norm_backward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(kBlock), 0, a.stream,
-                           (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, (const W *)a.weight, a.mean,
-                           a.rstd, a.width, (T *)a.out);
+                           (const T *)a.x, (long long)a.x_stride, (const T *)a.dy, (long long)a.dy_stride, (const W *)a.weight, a.mean,
+                           a.rstd, (int)a.width, (T *)a.dx);
         RWK_LAUNCH_CHECK();
         hipLaunchKernelGGL((norm_weight_wide_kernel<T>), dim3((unsigned)rwk_ceil_div(a.width, kBlock), (unsigned)blocks),
-                           dim3(kBlock), 0, a.stream, (const T *)a.x, a.x_stride, (const T *)a.dy, a.dy_stride, a.mean,
-                           a.rstd, a.rows, a.width, a.partials);
+                           dim3(kBlock), 0, a.stream, (const T *)a.x, (long long)a.x_stride, (const T *)a.dy, (long long)a.dy_stride, a.mean,
+                           a.rstd, (long long)a.rows, (int)a.width, a.partials);
         RWK_LAUNCH_CHECK();
     } else if (vectors <= 4) {
         code = launch_backward<T, W, 4, 1>(a, blocks);
@@ -424,19 +417,29 @@ int backward(const NormArgs &a) {
     }
     if (code != RWK_OK) return code;
     hipLaunchKernelGGL((norm_weight_sum_kernel<W>), dim3((unsigned)rwk_ceil_div(2ll * a.width, kSumCols)),
-                       dim3(kSumCols * kSumGroups), 0, a.stream, a.partials, (int)blocks, a.width, (W *)a.dw,
+                       dim3(kSumCols * kSumGroups), 0, a.stream, a.partials, (int)blocks, (int)a.width, (W *)a.dw,
                        (W *)a.db);
     RWK_LAUNCH_CHECK();
     return RWK_OK;
 }
 
-int check(const NormArgs &a, int32_t type, int32_t weight_type) {
+int check(const rwk_layer_norm &a, bool backward) {
     RWK_REQUIRE_PTR(a.x);
     RWK_REQUIRE_PTR(a.weight);
-    RWK_REQUIRE_PTR(a.out);
-    if (type < RWK_F32 || type > RWK_BF16 || (weight_type != type && weight_type != RWK_F32)) return RWK_E_UNSUPPORTED;
-    if (a.rows <= 0 || a.width <= 0 || a.x_stride < a.width) return RWK_E_SIZE;
-    return RWK_OK;
+    if (a.type < RWK_F32 || a.type > RWK_BF16 || (a.weight_type != a.type && a.weight_type != RWK_F32))
+        return RWK_E_UNSUPPORTED;
+    if (a.rows <= 0 || a.width <= 0 || a.width > 0x3FFFFFFF || a.x_stride < a.width) return RWK_E_SIZE;
+    if (!backward) {
+        RWK_REQUIRE_PTR(a.y);
+        return (a.mean == nullptr) != (a.rstd == nullptr) ? RWK_E_NULL : RWK_OK;
+    }
+    RWK_REQUIRE_PTR(a.dy);
+    RWK_REQUIRE_PTR(a.dx);
+    RWK_REQUIRE_PTR(a.mean);
+    RWK_REQUIRE_PTR(a.rstd);
+    RWK_REQUIRE_PTR(a.partials);
+    RWK_REQUIRE_PTR(a.dw);
+    return a.dy_stride < a.width ? RWK_E_SIZE : RWK_OK;
 }
 
 }  // namespace
@@ -448,40 +451,26 @@ int64_t rwk_layer_norm_backward_blocks(int64_t rows, int64_t width, int32_t type
     return backward_blocks(rows, width, type == RWK_F32 ? 4 : 8);
 }
 
-int rwk_layer_norm_forward(const void *x, int64_t x_stride, const void *weight, const void *bias, int64_t rows,
-                           int64_t width, int32_t type, int32_t weight_type, float eps, void *y, float *mean,
-                           float *rstd, rwk_stream_t stream) {
-    if (width > 0x3FFFFFFF) return RWK_E_SIZE;
-    NormArgs a{};
-    a.x = x; a.weight = weight; a.bias = bias; a.x_stride = x_stride; a.rows = rows; a.width = (int)width; a.eps = eps;
-    a.out = y; a.mean = mean; a.rstd = rstd; a.stream = (hipStream_t)stream;
-    const int code = check(a, type, weight_type);
+int rwk_layer_norm_forward(const rwk_layer_norm *args, rwk_stream_t stream) {
+    RWK_REQUIRE_PTR(args);
+    const int code = check(*args, false);
     if (code != RWK_OK) return code;
-    if ((mean == nullptr) != (rstd == nullptr)) return RWK_E_NULL;
-    if (type == RWK_F32) return forward<float, float>(a);
-    if (type == RWK_F16) return weight_type == RWK_F32 ? forward<rwk_f16, float>(a) : forward<rwk_f16, rwk_f16>(a);
-    return weight_type == RWK_F32 ? forward<rwk_bf16, float>(a) : forward<rwk_bf16, rwk_bf16>(a);
+    const NormArgs a{*args, (hipStream_t)stream};
+    const bool wide = a.weight_type == RWK_F32;
+    if (a.type == RWK_F32) return forward<float, float>(a);
+    if (a.type == RWK_F16) return wide ? forward<rwk_f16, float>(a) : forward<rwk_f16, rwk_f16>(a);
+    return wide ? forward<rwk_bf16, float>(a) : forward<rwk_bf16, rwk_bf16>(a);
 }
 
-int rwk_layer_norm_backward(const void *x, int64_t x_stride, const void *dy, int64_t dy_stride, const void *weight,
-                            const float *mean, const float *rstd, int64_t rows, int64_t width, int32_t type,
-                            int32_t weight_type, void *dx, float *partials, void *dw, void *db, rwk_stream_t stream) {
-    if (width > 0x3FFFFFFF) return RWK_E_SIZE;
-    NormArgs a{};
-    a.x = x; a.dy = dy; a.weight = weight; a.x_stride = x_stride; a.dy_stride = dy_stride; a.rows = rows;
-    a.width = (int)width; a.out = dx; a.mean = (float *)mean; a.rstd = (float *)rstd; a.partials = partials;
-    a.dw = dw; a.db = db; a.stream = (hipStream_t)stream;
-    const int code = check(a, type, weight_type);
+int rwk_layer_norm_backward(const rwk_layer_norm *args, rwk_stream_t stream) {
+    RWK_REQUIRE_PTR(args);
+    const int code = check(*args, true);
     if (code != RWK_OK) return code;
-    RWK_REQUIRE_PTR(dy);
-    RWK_REQUIRE_PTR(mean);
-    RWK_REQUIRE_PTR(rstd);
-    RWK_REQUIRE_PTR(partials);
-    RWK_REQUIRE_PTR(dw);
-    if (dy_stride < width) return RWK_E_SIZE;
-    if (type == RWK_F32) return backward<float, float>(a);
-    if (type == RWK_F16) return weight_type == RWK_F32 ? backward<rwk_f16, float>(a) : backward<rwk_f16, rwk_f16>(a);
-    return weight_type == RWK_F32 ? backward<rwk_bf16, float>(a) : backward<rwk_bf16, rwk_bf16>(a);
+    const NormArgs a{*args, (hipStream_t)stream};
+    const bool wide = a.weight_type == RWK_F32;
+    if (a.type == RWK_F32) return backward<float, float>(a);
+    if (a.type == RWK_F16) return wide ? backward<rwk_f16, float>(a) : backward<rwk_f16, rwk_f16>(a);
+    return wide ? backward<rwk_bf16, float>(a) : backward<rwk_bf16, rwk_bf16>(a);
 }
 
 }  // extern "C"

@@ -8,12 +8,22 @@ only.
 """
 from __future__ import annotations
 
+import ctypes
+from ctypes import c_float, c_int32, c_int64, c_void_p
+
 import torch
 import torch.nn as nn
 
 from . import _lib
 
 __all__ = ["layer_norm", "LayerNorm"]
+
+
+class _Args(ctypes.Structure):
+    """``rwk_layer_norm`` of ``rwk.h``."""
+    _fields_ = [(n, c_void_p) for n in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dx", "partials", "dw", "db")] \
+        + [(n, c_int64) for n in ("x_stride", "dy_stride", "rows", "width")] \
+        + [("type", c_int32), ("weight_type", c_int32), ("eps", c_float)]
 
 
 def _rows(t: torch.Tensor):
@@ -48,54 +58,61 @@ def _check(x, weight, bias):
 
 
 def _forward(x, weight, bias, eps, keep):
-    """(y, stats, rows, stride): ``rows`` is x as the kernel read it, ``stats`` the rows' mean and 1 / deviation."""
+    """(y, what the backward pass needs): x as the kernel read it, the weight, the rows' mean and 1 / deviation, the
+    call's arguments."""
     rows, stride = _rows(x)
-    width, dev = x.shape[-1], x.device
-    n = x.numel() // width
+    dev, a = x.device, _Args()
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = mean = rstd = None
+    a.x_stride, a.width, a.eps = stride, x.shape[-1], eps
+    a.rows = n = x.numel() // x.shape[-1]
+    a.type, a.weight_type = _lib.element_type(x.dtype), _lib.element_type(weight.dtype)
+    stats = None
     if keep:
         stats = torch.empty((2, n), dtype=torch.float32, device=dev)
-        mean = stats.data_ptr()
-        rstd = mean + 4 * n
+        a.mean = at = stats.data_ptr()
+        a.rstd = at + 4 * n
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
     if n:
-        w = weight.contiguous()
-        b = None if bias is None else bias.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+            a.bias = bias.data_ptr()
+        a.x, a.weight, a.y = rows.data_ptr(), weight.data_ptr(), y.data_ptr()
         with _lib.device_guard(dev):
-            _lib.check(_lib.load().rwk_layer_norm_forward(
-                rows.data_ptr(), stride, w.data_ptr(), _lib.ptr(b), n, width, _lib.element_type(x.dtype),
-                _lib.element_type(w.dtype), eps, y.data_ptr(), mean, rstd, _lib.current_stream(dev)),
-                "rwk_layer_norm_forward")
-    return y, stats, rows, stride
+            _lib.check(_lib.load().rwk_layer_norm_forward(ctypes.addressof(a), _lib.current_stream(dev)),
+                       "rwk_layer_norm_forward")
+    return y, rows, weight, stats, a
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats, rows, ctx.stride = _forward(x, weight, bias, eps, True)
+        y, rows, weight, stats, ctx.args = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(rows, weight, stats)
         ctx.has_bias = bias is not None
+        ctx.blocks = _lib.load().rwk_layer_norm_backward_blocks(stats.shape[1], x.shape[-1], ctx.args.type)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        # little is done here: the engine's thread has just woken up, and everything in it takes twice its time
         rows, weight, stats = ctx.saved_tensors
-        n, width, dev = stats.shape[1], dy.shape[-1], dy.device
+        a, dev = ctx.args, dy.device
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-        dw, db = torch.empty((2, width), dtype=weight.dtype, device=dev).unbind(0)
-        if n == 0:
-            return dx, dw.zero_(), db.zero_() if ctx.has_bias else None, None
-        dy, dy_stride = _rows(dy)
-        lib, code = _lib.load(), _lib.element_type(dx.dtype)
-        partials = torch.empty((lib.rwk_layer_norm_backward_blocks(n, width, code), 2 * width), dtype=torch.float32,
-                               device=dev)
-        mean = stats.data_ptr()
-        with _lib.device_guard(dev):
-            _lib.check(lib.rwk_layer_norm_backward(
-                rows.data_ptr(), ctx.stride, dy.data_ptr(), dy_stride, weight.contiguous().data_ptr(), mean,
-                mean + 4 * n, n, width, code, _lib.element_type(weight.dtype), dx.data_ptr(), partials.data_ptr(),
-                dw.data_ptr(), db.data_ptr(), _lib.current_stream(dev)), "rwk_layer_norm_backward")
+        dw, db = torch.empty((2, a.width), dtype=weight.dtype, device=dev).unbind(0)
+        if a.rows == 0:
+            dw.zero_()
+            db.zero_()
+        else:
+            dy, a.dy_stride = _rows(dy)
+            partials = torch.empty((ctx.blocks, 2 * a.width), dtype=torch.float32, device=dev)
+            a.x, a.weight, a.mean, a.dy = rows.data_ptr(), weight.data_ptr(), stats.data_ptr(), dy.data_ptr()
+            a.rstd = a.mean + 4 * a.rows
+            a.dx, a.partials, a.dw, a.db = dx.data_ptr(), partials.data_ptr(), dw.data_ptr(), db.data_ptr()
+            with _lib.device_guard(dev):
+                _lib.check(_lib.load().rwk_layer_norm_backward(ctypes.addressof(a), _lib.current_stream(dev)),
+                           "rwk_layer_norm_backward")
         return dx, dw, db if ctx.has_bias else None, None
 
 

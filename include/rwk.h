@@ -894,20 +894,27 @@ int rwk_row_scale(const float *x, const float *scale, int64_t n, int64_t d, floa
  * type: RWK_F32, RWK_F16 or RWK_BF16; weight_type: the same, or RWK_F32 for weights kept in fp32.
  * ------------------------------------------------------------------------------------- */
 
-/* y (rows, width) contiguous = (x - mean) * rstd * weight + bias; x has rows x_stride >= width elements apart, bias
- * may be NULL.  mean and rstd (rows, float32) are written when both are given (the backward pass needs them). */
-int rwk_layer_norm_forward(const void *x, int64_t x_stride, const void *weight, const void *bias, int64_t rows,
-                           int64_t width, int32_t type, int32_t weight_type, float eps, void *y, float *mean,
-                           float *rstd, rwk_stream_t stream);
+typedef struct {
+    const void *x;              /* rows x_stride >= width elements apart */
+    const void *weight, *bias;  /* bias may be NULL */
+    void *y;                    /* contiguous */
+    float *mean, *rstd;         /* (rows): written by the forward pass if both are given, read by the backward pass */
+    /* backward only */
+    const void *dy;             /* rows dy_stride apart */
+    void *dx;                   /* contiguous */
+    float *partials;            /* rwk_layer_norm_backward_blocks() rows of 2 * width */
+    void *dw, *db;              /* of weight_type; db may be NULL */
+    int64_t x_stride, dy_stride, rows, width;
+    int32_t type, weight_type;
+    float eps;
+} rwk_layer_norm;
 
+/* y = (x - mean) * rstd * weight + bias */
+int rwk_layer_norm_forward(const rwk_layer_norm *a, rwk_stream_t stream);
 /* Rows of `partials` (float32, 2 * width each) that rwk_layer_norm_backward needs. */
 int64_t rwk_layer_norm_backward_blocks(int64_t rows, int64_t width, int32_t type);
-
-/* dx (rows, width) contiguous, dw and db (width, of weight_type; db may be NULL) from dy (rows dy_stride apart) and
- * what the forward pass left.  Sums run in a fixed order. */
-int rwk_layer_norm_backward(const void *x, int64_t x_stride, const void *dy, int64_t dy_stride, const void *weight,
-                            const float *mean, const float *rstd, int64_t rows, int64_t width, int32_t type,
-                            int32_t weight_type, void *dx, float *partials, void *dw, void *db, rwk_stream_t stream);
+/* dx, dw and db from dy and what the forward pass left.  Sums run in a fixed order. */
+int rwk_layer_norm_backward(const rwk_layer_norm *a, rwk_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * AdamW over many tensors in one launch (the optimiser step of main.py:79,87 with decoupled weight decay).

@@ -17,21 +17,25 @@ def lib():
 
 
 def test_layer_norm_entry_points(lib):
-    fwd = lambda **k: lib.rwk_layer_norm_forward(*(dict(
-        x=A, x_stride=64, weight=A, bias=None, rows=4, width=64, type=0, weight_type=0, eps=1e-5, y=A, mean=None,
-        rstd=None, stream=None) | k).values())
-    bwd = lambda **k: lib.rwk_layer_norm_backward(*(dict(
-        x=A, x_stride=64, dy=A, dy_stride=64, weight=A, mean=A, rstd=A, rows=4, width=64, type=0, weight_type=0, dx=A,
-        partials=A, dw=A, db=None, stream=None) | k).values())
-    for call, names in ((fwd, ("x", "weight", "y")), (bwd, ("x", "dy", "weight", "mean", "rstd", "dx", "partials", "dw"))):
+    from gnn_amd.layer_norm import _Args
+
+    def call(entry, **k):
+        a = _Args()
+        good = {n: A for n in ("x", "weight", "y", "mean", "rstd", "dy", "dx", "partials", "dw")}
+        for name, value in (good | dict(x_stride=64, dy_stride=64, rows=4, width=64) | k).items():
+            setattr(a, name, value)
+        return entry(ctypes.addressof(a), None)
+    fwd, bwd = lib.rwk_layer_norm_forward, lib.rwk_layer_norm_backward
+    assert fwd(None, None) == NULL and bwd(None, None) == NULL
+    for entry, names in ((fwd, ("x", "weight", "y", "mean", "rstd")),
+                         (bwd, ("x", "dy", "weight", "mean", "rstd", "dx", "partials", "dw"))):
         for name in names:
-            assert call(**{name: None}) == NULL, name
+            assert call(entry, **{name: None}) == NULL, name
         for bad in (dict(rows=0), dict(rows=-1), dict(width=0), dict(width=1 << 40), dict(x_stride=63)):
-            assert call(**bad) == SIZE, bad
+            assert call(entry, **bad) == SIZE, bad
         for bad in (dict(type=3), dict(type=-1), dict(weight_type=1), dict(type=1, weight_type=2)):
-            assert call(**bad) == UNSUPPORTED, bad
-    assert fwd(mean=A) == NULL and fwd(rstd=A) == NULL
-    assert bwd(dy_stride=1) == SIZE
+            assert call(entry, **bad) == UNSUPPORTED, bad
+    assert call(bwd, dy_stride=1) == SIZE
     blocks = lib.rwk_layer_norm_backward_blocks
     assert blocks(0, 8, 0) == 0 and blocks(8, 0, 0) == 0 and blocks(1, 8, 0) == 1
     for rows, width in ((10 ** 6, 64), (10 ** 6, 4096), (10 ** 6, 100000)):
