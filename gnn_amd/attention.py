@@ -30,7 +30,7 @@ _P, _I64 = c_void_p, c_int64
 
 class _Args(ctypes.Structure):
     """``rwk_attention`` of ``rwk.h``."""
-    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("d_out", _P), ("dq", _P), ("dk", _P), ("dv", _P),
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("out_low", _P), ("d_out", _P), ("dq", _P), ("dk", _P), ("dv", _P),
                 ("q_row", _I64), ("q_head", _I64), ("k_row", _I64), ("k_head", _I64), ("v_row", _I64),
                 ("v_head", _I64), ("do_row", _I64), ("do_head", _I64), ("seg_ptr", _P), ("n_segments", _I64),
                 ("rows", _I64), ("heads", _I64), ("kv_heads", _I64), ("dim", _I64), ("scale", c_float),
@@ -223,12 +223,18 @@ def _forward(q, k, v, segments, causal, scale, table, buckets, stats):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if segments.total < q.shape[0]:
         out[segments.total:].zero_()
-    st = torch.empty((q.shape[1], q.shape[0], 2), dtype=torch.float32, device=q.device) if stats else None
-    a.out, a.stats = out.data_ptr(), _lib.ptr(st)
+    st = low = None
+    a.out = out.data_ptr()
+    if stats:
+        st = torch.empty((q.shape[1], q.shape[0], 2), dtype=torch.float32, device=q.device)
+        a.stats = st.data_ptr()
+        if a.type:                                     # 16 bits: what the rounding of out leaves over
+            low = torch.empty_like(out)
+            a.out_low = low.data_ptr()
     with _lib.device_guard(q.device):
         _lib.check(_lib.load().rwk_attention_forward(ctypes.addressof(a), _lib.current_stream(q.device)),
                    "rwk_attention_forward")
-    return out, st
+    return out, st, low
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -236,15 +242,15 @@ class _PackedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, segments, causal, scale, buckets):
         q, k, v = _heads(q.detach()), _heads(k.detach()), _heads(v.detach())
         table = None if table is None else table.detach().contiguous()
-        out, stats = _forward(q, k, v, segments, causal, scale, table, buckets, True)
-        ctx.save_for_backward(q, k, v, table, out, stats)
+        out, stats, low = _forward(q, k, v, segments, causal, scale, table, buckets, True)
+        ctx.save_for_backward(q, k, v, table, out, stats, low)
         ctx.rest = (segments, causal, scale, buckets)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, table, out, stats = ctx.saved_tensors
+        q, k, v, table, out, stats, low = ctx.saved_tensors
         segments, causal, scale, buckets = ctx.rest
         dev = q.device
         d_out = _heads(d_out)
@@ -256,7 +262,8 @@ class _PackedAttention(torch.autograd.Function):
             for t in (dq, dk, dv):
                 t[segments.total:].zero_()
         delta = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
-        a.out, a.stats, a.delta = out.data_ptr(), stats.data_ptr(), delta.data_ptr()
+        a.out, a.out_low = out.data_ptr(), _lib.ptr(low)
+        a.stats, a.delta = stats.data_ptr(), delta.data_ptr()
         a.d_out, a.dq, a.dk, a.dv = d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         a.do_row, a.do_head, _ = d_out.stride()
         d_table = None
@@ -282,8 +289,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
 
     Returns (N, H, D), contiguous.  A row that attends to nothing gives zeros.  Differentiable once with respect to
     q, k, v and bias.  Sums, softmax statistics and the bias gradient are fp32; for the 16-bit types probabilities are
-    rounded to the type before they meet ``v``.  Rows that do not attend to a row are unaffected by values that are
-    not finite in its ``k``; in ``v`` such values reach the rows of the same block of a causal segment."""
+    rounded to the type before they meet ``v``.  What a pair's rows hold counts for nothing where the pair does not
+    attend, values that are not finite included (blocks of rows whose result is not finite take much longer)."""
     if not q.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
     _lib.element_type(q.dtype)

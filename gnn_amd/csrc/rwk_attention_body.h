@@ -323,23 +323,27 @@ __device__ inline Frag<T> column_operand(const T *tile, int first, int dt, int l
     return f;
 }
 
-// a transposed result, DT tiles of 32 elements: lane l % 32 is the row, its registers four elements each
-template <typename T, int DT>
+// a transposed result, DT tiles of 32 elements: lane l % 32 is the row, its registers four elements each.  LOW: what
+// the rounding to T left over, as T.
+template <bool LOW, typename T, int DT>
 __device__ inline void store_rows(T *row, int dim, int h, const f32x16 (&acc)[DT], float scale) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = 32 * dt + 8 * g + 4 * h;
-            if (d + 4 <= dim) {
-                typename RwkPack<T, 4>::type v;
+            typename RwkPack<T, 4>::type v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[dt][4 * g + e] * scale);
+            for (int e = 0; e < 4; ++e) {
+                const float x = acc[dt][4 * g + e] * scale;
+                v[e] = LOW ? (T)(x - (float)(T)x) : (T)x;
+            }
+            if (d + 4 <= dim) {
                 rwk_store<T, 4>(row + d, v);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (d + e < dim) row[d + e] = (T)(acc[dt][4 * g + e] * scale);
+                    if (d + e < dim) row[d + e] = v[e];
             }
         }
 }
@@ -421,6 +425,153 @@ __device__ inline float load_table(const RwkAttnArgs &p, int head) {
 }
 __device__ inline float look_up(float table, int bucket) {
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * bucket, __builtin_bit_cast(int, table)));
+}
+
+// What the backward pass adds to a row's scores so that their exponential is the probability: minus the forward
+// pass's reference, and the logarithm of 1 / sum.  -infinity for a row without pairs and for rows that do not exist.
+__device__ inline float reference(float ref, float inv, float c) { return __log2f(inv) / c - ref; }
+
+// ---------------------------------------------------------------------------------------------------------------
+// A pair that does not attend counts for nothing whatever its rows hold, but a matrix instruction adds 0 times what it
+// finds: not a number where that is not finite.  So rows whose result is not finite are computed again, pair by pair and
+// without matrix instructions, leaving out the pairs whose weight is zero.  Slow, and only ever run for such rows.
+// Lanes l and l + 32 share a row, eight elements each of every sixteen.  Elements are taken sixteen at a time, each time
+// with all the row's products over again: few registers, so that the code costs the kernels' loops none.
+// ---------------------------------------------------------------------------------------------------------------
+// whether the lane's row is not finite
+template <int KS, int DT>
+__device__ inline bool not_finite(const f32x16 (&acc)[DT]) {
+    constexpr int N = KS == 1 ? 8 : 16;           // KS = 1: the upper half is no element's
+    float t = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < N; ++i) t = fmaf(acc[dt][i], 0.f, t);
+    t += __shfl_xor(t, 32, 64);
+    return t != t;                                // 0 times infinity, or NaN
+}
+__device__ inline bool any_lane(bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; }
+
+template <typename T>
+__device__ inline float row_product(const T *a, const T *b, int h, int dim) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int d = 8 * h; d < dim + 8 * h; d += 16) {            // both halves in the same rounds
+        const Frag<T> x = load_global<T>(a, d, dim), y = load_global<T>(b, d, dim);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf((float)x.v[e], (float)y.v[e], sum);
+    }
+    return sum + __shfl_xor(sum, 32, 64);
+}
+
+template <typename T>
+__device__ inline void add_row(float (&acc)[8], float weight, const T *row, int d, int dim) {
+    if (weight == 0.f) return;
+    const Frag<T> x = load_global<T>(row, d, dim);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(weight, (float)x.v[e], acc[e]);
+}
+
+template <bool LOW, typename T>
+__device__ inline void store_eight(T *row, const float (&acc)[8], float scale, int d, int dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = acc[e] * scale;
+        if (d + e < dim) row[d + e] = LOW ? (T)(x - (float)(T)x) : (T)x;
+    }
+}
+
+// exponent (less the reference's part) of pair (q, k) from its product, -infinity if it does not attend
+template <bool BIAS>
+__device__ inline float pair_score(const RwkAttnArgs &p, const Place &at, float table, int q, int k, float product) {
+    bool on = q < at.n && k < at.n && !(p.a.causal != 0 && k > q);
+    float x = product;
+    if (BIAS) {
+        const int nb = (int)p.a.n_buckets;
+        int b = nb;
+        if (on) b = min((int)p.a.codes[p.a.code_start[at.seg] + (long long)q * ((at.n + 31) / 32 * 32) + k], nb);
+        x = fmaf(product, p.a.scale, look_up(table, b));
+        on = on && b < nb;
+    }
+    return on ? x : -INFINITY;
+}
+
+// The lane's row of the operands, at `row` (clamped to the segment) of head or kv_head.
+template <typename T>
+__device__ inline const T *row_of(const void *base, long long row, long long stride, long long head, long long head_stride) {
+    return (const T *)base + row * stride + head * head_stride;
+}
+
+template <typename T, bool BIAS>
+__device__ inline void exact_forward(const RwkAttnArgs &p, const Place &at, float table, int q, int end, float base,
+                                     float inv, float c, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
+    const long long row = at.base + min(q, at.n - 1);
+    const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
+#pragma unroll 1
+    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
+        float o[8] = {};
+#pragma unroll 1
+        for (int k = 0; k < end; ++k) {
+            const T *k_row = row_of<T>(p.a.k, at.base + k, p.a.k_row, at.kv_head, p.a.k_head);
+            const float x = pair_score<BIAS>(p, at, table, q, k, row_product(q_row, k_row, h, dim));
+            add_row(o, exp2_fast((x - base) * c), row_of<T>(p.a.v, at.base + k, p.a.v_row, at.kv_head, p.a.v_head), d, dim);
+        }
+        const long long to = (row * p.a.heads + at.head) * dim;
+        if (mine) store_eight<false>((T *)p.a.out + to, o, inv, d, dim);
+        if (mine && p.a.out_low != nullptr) store_eight<true>((T *)p.a.out_low + to, o, inv, d, dim);
+    }
+}
+
+template <typename T, bool BIAS>
+__device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end, float ref, float delta,
+                                float c, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
+    const long long row = at.base + min(q, at.n - 1);
+    const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
+    const T *o_row = row_of<T>(p.a.d_out, row, p.a.do_row, at.head, p.a.do_head);
+#pragma unroll 1
+    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
+        float g[8] = {};
+#pragma unroll 1
+        for (int k = 0; k < end; ++k) {
+            const T *k_row = row_of<T>(p.a.k, at.base + k, p.a.k_row, at.kv_head, p.a.k_head);
+            const T *v_row = row_of<T>(p.a.v, at.base + k, p.a.v_row, at.kv_head, p.a.v_head);
+            const float x = pair_score<BIAS>(p, at, table, q, k, row_product(q_row, k_row, h, dim));
+            const float w = weigh(exp2_fast((x + ref) * c), row_product(o_row, v_row, h, dim) - delta);
+            add_row(g, w, k_row, d, dim);
+        }
+        if (mine) store_eight<false>((T *)p.a.dq + (row * p.a.heads + at.head) * dim, g, p.a.scale, d, dim);
+    }
+}
+
+template <typename T, bool BIAS>
+__device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int k, int begin, float c, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
+    const long long row = at.base + min(k, at.n - 1);
+    const T *k_row = row_of<T>(p.a.k, row, p.a.k_row, at.kv_head, p.a.k_head);
+    const T *v_row = row_of<T>(p.a.v, row, p.a.v_row, at.kv_head, p.a.v_head);
+#pragma unroll 1
+    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
+        float gk[8] = {}, gv[8] = {};
+#pragma unroll 1
+        for (int head = at.head; head < at.head + p.group; ++head) {
+            const float table = BIAS ? load_table<T>(p, head) : 0.f;
+#pragma unroll 1
+            for (int q = begin; q < at.n; ++q) {
+                const T *q_row = row_of<T>(p.a.q, at.base + q, p.a.q_row, head, p.a.q_head);
+                const T *o_row = row_of<T>(p.a.d_out, at.base + q, p.a.do_row, head, p.a.do_head);
+                const long long st = head * p.a.rows + at.base + q;
+                const float x = pair_score<BIAS>(p, at, table, q, k, row_product(k_row, q_row, h, dim));
+                const float w = exp2_fast((x + reference(p.a.stats[2 * st], p.a.stats[2 * st + 1], c)) * c);
+                add_row(gv, w, o_row, d, dim);
+                add_row(gk, weigh(w, row_product(v_row, o_row, h, dim) - p.a.delta[st]), q_row, d, dim);
+            }
+        }
+        const long long to = (row * p.a.kv_heads + at.kv_head) * dim;
+        if (mine) store_eight<false>((T *)p.a.dk + to, gk, p.a.scale, d, dim);
+        if (mine) store_eight<false>((T *)p.a.dv + to, gv, 1.f, d, dim);
+    }
 }
 
 // Bytes of LDS for the tiles: two buffers of two, and the elements that the second product of KS = 1 reads past the
@@ -559,20 +710,21 @@ attention_forward_kernel(const RwkAttnArgs p) {
         keys.commit(next);
         values.commit(next + BN * S::W);
     }
-    if (q >= n) return;
     sum += __shfl_xor(sum, 32, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;      // a row without pairs: zeros
-    store_rows<T, DT>((T *)p.a.out + ((at.base + q) * p.a.heads + at.head) * dim, dim, h, acc, inv);
-    if (p.a.stats != nullptr && h == 0) {
+    const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
+    const bool again = q < n && not_finite<KS>(acc);
+    if (q < n && !again) {
+        store_rows<false, T, DT>((T *)p.a.out + o_at, dim, h, acc, inv);
+        if (p.a.out_low != nullptr) store_rows<true, T, DT>((T *)p.a.out_low + o_at, dim, h, acc, inv);
+    }
+    if (q < n && p.a.stats != nullptr && h == 0) {
         float *st = p.a.stats + 2 * (at.head * p.a.rows + at.base + q);
         st[0] = ref == -INFINITY ? 0.f : ref;
         st[1] = inv;
     }
+    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, ref == -INFINITY ? 0.f : ref, inv, c, again);
 }
-
-// What the backward pass adds to a row's scores so that their exponential is the probability: minus the forward
-// pass's reference, and the logarithm of 1 / sum.  -infinity for a row without pairs and for rows that do not exist.
-__device__ inline float reference(float ref, float inv, float c) { return __log2f(inv) / c - ref; }
 
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && (!BIAS || KS < 8) ? 2 : 1)
@@ -609,6 +761,11 @@ attention_dq_kernel(const RwkAttnArgs p) {
         const Frag<T> o = load_global<T>((const T *)p.a.out + o_at, 16 * ks + 8 * h, dim);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf((float)of[ks].v[e], (float)o.v[e], delta);
+        if (sizeof(T) == 2 && p.a.out_low != nullptr) {
+            const Frag<T> low = load_global<T>((const T *)p.a.out_low + o_at, 16 * ks + 8 * h, dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)of[ks].v[e], (float)low.v[e], delta);
+        }
     }
     delta += __shfl_xor(delta, 32, 64);
     const long long row_at = at.head * p.a.rows + at.base + qc;
@@ -688,7 +845,9 @@ attention_dq_kernel(const RwkAttnArgs p) {
         keys.commit(next);
         values.commit(next + BN * S::W);
     }
-    if (q < n) store_rows<T, DT>((T *)p.a.dq + o_at, dim, h, acc, scale);
+    const bool again = q < n && not_finite<KS>(acc);
+    if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc, scale);
+    if (any_lane(again)) exact_dq<T, BIAS>(p, at, table, q, end, ref, delta, c, again);
     if (BIAS) {
         __syncthreads();
         // a wavefront per bucket sums the threads' slots in a fixed order
@@ -853,10 +1012,13 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             if (q0 + BQ < n) finish(turn ^ 1);
         }
     }
-    if (k >= n) return;
-    const long long to = ((at.base + k) * p.a.kv_heads + at.kv_head) * dim;
-    store_rows<T, DT>((T *)p.a.dk + to, dim, h, dk, scale);
-    store_rows<T, DT>((T *)p.a.dv + to, dim, h, dv, 1.f);
+    const long long to = ((at.base + kc) * p.a.kv_heads + at.kv_head) * dim;
+    const bool bad_k = not_finite<KS>(dk), bad_v = not_finite<KS>(dv), again = k < n && (bad_k || bad_v);
+    if (k < n && !again) {
+        store_rows<false, T, DT>((T *)p.a.dk + to, dim, h, dk, scale);
+        store_rows<false, T, DT>((T *)p.a.dv + to, dim, h, dv, 1.f);
+    }
+    if (any_lane(again)) exact_dkv<T, BIAS>(p, at, k, begin, c, again);
 }
 
 template <typename K>

@@ -964,6 +964,8 @@ int rwk_adamw_step(const rwk_adamw_chunk *chunks, int64_t n_chunks, int64_t chun
 typedef struct {
     const void *q, *k, *v;          /* (rows, heads, dim), (rows, kv_heads, dim) */
     void *out;
+    void *out_low;                  /* what the rounding of `out` left over, of the same type, or NULL: with it the
+                                     * backward pass of the 16-bit types takes out . d_out from the unrounded out */
     const void *d_out;              /* backward only, as are dq, dk, dv, delta, d_table, d_table_partials */
     void *dq, *dk, *dv;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;

@@ -5,7 +5,7 @@ Tolerances (``u`` = half a step of the element type, e = 2^-24, one fp32 roundin
   p           twice the score's error (its own and the sum's), n e for the sum, and u for the 16-bit types, which
               round it before the second product (nothing for fp32)
   out         p's error against |v|, n e for the sum, u for the result
-  delta       |do| against out's error and D e
+  delta       |do| against the error of out before its rounding (kept with its remainder), and D e
   ds          p's error against |dp - delta|, the errors of dp (D e) and delta against p, u as for p
   dq, dk, dv  the error of ds or p against the magnitudes of the other factor, n e, u; dk, dv summed over the group
   d_bias      the error of the unrounded ds summed, e per addition, u
@@ -72,10 +72,9 @@ def truth(q, k, v, do, lengths, causal, scale=None, bias=None, codes=None):
         rel = s_err + (s_err * p).sum(2, keepdim=True) + (n + 16) * E
         o = p @ c
         o_err = ((rel + up) * p) @ c.abs() + (n + 4) * E * (p @ c.abs())
-        o_all = o_err + u * (o.abs() + o_err)
         dp = d @ c.transpose(1, 2)
         delta = (d * o).sum(2, keepdim=True)
-        de = (d.abs() * o_all).sum(2, keepdim=True) + dim * E * (d.abs() * o.abs()).sum(2, keepdim=True)
+        de = (d.abs() * (o_err + u * u * o.abs() + torch.finfo(dtype).tiny)).sum(2, keepdim=True) + dim * E * (d.abs() * o.abs()).sum(2, keepdim=True)
         dpe = dim * E * (d.abs() @ c.abs().transpose(1, 2))
         ds = p * (dp - delta)
         ds_err = p * (rel * (dp - delta).abs() + dpe + de) * (1 + rel) + 4 * E * ds.abs()
@@ -244,6 +243,40 @@ def test_keys_that_are_masked_may_hold_anything(dev):
     bad[77] = float("inf")
     got = run(q, bad, v, do, lengths, False, bias=bias, codes=codes)
     assert torch.equal(got[0], clean[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [16, 40, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_masked_pairs_may_hold_anything(dev, dtype, dim, bad):
+    """Padded nodes whose codes do not attend hold values that are not finite in q, k and v: all other rows and all
+    gradients are those of a batch with zeros there.  Causal: rows behind a row that is not finite in k and v."""
+    lengths = [70, 200]
+    q, k, v, do, bias, codes = make(dev, dtype, lengths, 4, 2, dim, buckets=4)
+    holes = [3, 40, 64, 69, 71, 150, 269]
+    for c, lo in zip(codes, (0, 70)):
+        for x in holes:
+            if lo <= x < lo + c.shape[0]:
+                c[x - lo] = 255
+                c[:, x - lo] = 255
+    clean = []
+    for t in (q, k, v):
+        t[holes] = 0
+        clean.append(t.clone())
+        t[holes] = bad
+    want, err = truth(*clean, do, lengths, False, bias=bias, codes=codes)
+    check(run(q, k, v, do, lengths, False, bias=bias, codes=codes), want, err)
+    q, k, v, do, _, _ = make(dev, dtype, lengths, 4, 2, dim)
+    want, err = truth(q, k, v, do, lengths, True)
+    k, v = k.clone(), v.clone()
+    k[50:70] = bad
+    v[50:70] = bad
+    k[200:270:3] = bad
+    v[200:270:3] = bad
+    got = run(q, k, v, do, lengths, True)[0]
+    keep = list(range(50)) + list(range(70, 200))
+    check([got[keep]], [want[0][keep]], [err[0][keep]])
+    assert not got[200:].isfinite().all(1).all(1).any()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
