@@ -348,6 +348,80 @@ __device__ inline void store_rows(T *row, int dim, int h, const f32x16 (&acc)[DT
         }
 }
 
+// Result of the second product: DT tiles of 32 elements by the wavefront's 32 rows.
+template <typename T, int KS>
+struct Result {
+    f32x16 a[Shape<T, KS>::DT];
+    __device__ void clear() {
+#pragma unroll
+        for (auto &x : a) x = f32x16{};
+    }
+    __device__ void scale(float by) {             // of the lane's row
+#pragma unroll
+        for (auto &x : a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= by;
+    }
+    // `f`: eight weights of the lane's row, for the tile's rows first .. first + 15 as column_operand has them
+    template <typename F>
+    __device__ void add(const T *tile, int first, const F &f, int lane) {
+#pragma unroll
+        for (int dt = 0; dt < Shape<T, KS>::DT; ++dt) a[dt] = mma(column_operand<T, KS>(tile, first, dt, lane), f, a[dt]);
+    }
+    __device__ void finish() {}
+};
+
+// fp32, up to 16 elements: a tile of 32 would be half empty, and the products are what bounds such kernels.  Two tiles
+// of 16 elements by 16 rows instead, the summed index four at a time: a lane gives away the weights of the row that its
+// neighbouring sixteen lanes hold and takes theirs for another key (2 of 3 products' time; 1024 protein-sized graphs,
+// 4 heads of 16: 2.62 to 2.20 ms).
+struct SwappedRows { float low, high; };
+__device__ inline SwappedRows swap_rows(float x, float y) {          // lanes 16-31, 48-63 of x with 0-15, 32-47 of y
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+    return {__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])};
+}
+template <>
+struct Result<float, 1> {
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    using S = Shape<float, 1>;
+    f32x4 low, high;                              // rows 0 - 15 and 16 - 31: lane l row l % 16, elements 4 (l / 16) ..
+    f32x16 a[1];
+    __device__ void clear() { low = high = f32x4{}; }
+    __device__ void scale(float by) {
+        const SwappedRows r = swap_rows(by, by);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            low[e] *= r.low;
+            high[e] *= r.high;
+        }
+    }
+    __device__ void add(const float *tile, int first, const Frag<float> &f, int lane) {
+        const int odd = (lane >> 4) & 1, col = lane & 15;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const int row = first + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) + odd;
+            const float x = tile[S::at(row, col >> 2) + (col & 3)];
+            const SwappedRows r = swap_rows(f.v[e], f.v[e + 1]);
+            low = __builtin_amdgcn_mfma_f32_16x16x4f32(x, r.low, low, 0, 0, 0);
+            high = __builtin_amdgcn_mfma_f32_16x16x4f32(x, r.high, high, 0, 0, 0);
+        }
+    }
+    __device__ void finish() {                    // as a 32 x 32 result, elements 16 .. 31 zeros
+        a[0] = f32x16{};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const SwappedRows r = swap_rows(low[e], high[e]);
+            const auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, r.low),
+                                                            __builtin_bit_cast(uint32_t, r.high), false, false);
+            x[e] = __builtin_bit_cast(float, (uint32_t)t[0]);
+            x[4 + e] = __builtin_bit_cast(float, (uint32_t)t[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[0][i] = x[i];
+    }
+};
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // One workgroup's place in the launch: consecutive workgroups go to different dies, so the key / value head varies
@@ -389,47 +463,85 @@ __device__ inline Place key_place(const RwkAttnArgs &p, long long b) {
 // code e of four, at most n_buckets
 __device__ inline int code_of(uint32_t codes, int e, int nb) { return min((int)((codes >> (8 * e)) & 255u), nb); }
 
-// Adds four values to a thread's own sums, NT floats apart, by their codes (a masked pair's 0 to any).  All four sums
-// are read before the first is written; an equal code before takes the place of what was read.  (The LDS float atomic
-// works through its lanes one by one: 180 cycles for a wavefront's 64 separate places, measured.)
-template <int NT>
-__device__ inline void add_by_code(float *sums, uint32_t codes, int last, const float *x) {
-    int c[4];
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        c[e] = code_of(codes, e, last);
-        v[e] = sums[c[e] * NT];
+// The bias gradient's sums of a dQ workgroup: every thread its own per bucket, NT floats apart, without atomics.  (The
+// LDS float atomic works through its lanes one by one: 180 cycles for a wavefront's 64 separate places, measured.)
+// SPLIT: four sets of them, one per place among four neighbouring pairs, each with a slot for the pairs that have no
+// bucket, so that four values are read, added and written without a look at each other's codes (fp32, 8 buckets, 1024
+// protein-sized graphs: 715 us for 809).  Otherwise all four
+// sums are read before the first is written, and an equal code before takes the place of what was read.
+template <int NT, bool SPLIT>
+struct BucketSums {
+    float *at;
+    int nb;
+    __device__ static int slots(int nb) { return SPLIT ? 4 * (nb + 1) : nb; }
+    __device__ BucketSums(float *sums, int nb_) : at(sums + threadIdx.x), nb(nb_) {
+        for (int b = 0; b < slots(nb); ++b) at[b * NT] = 0.f;
     }
+    __device__ void add(uint32_t codes, const float *x) {       // a masked pair's 0 to any
+        int c[4];
+        float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e) {
+            c[e] = SPLIT ? e * (nb + 1) + code_of(codes, e, nb) : code_of(codes, e, nb - 1);
+            v[e] = at[c[e] * NT];
+        }
 #pragma unroll
-        for (int f = 0; f < e; ++f) v[e] = c[f] == c[e] ? v[f] : v[e];
-        v[e] += x[e];
+        for (int e = 0; e < 4; ++e) {
+            if (!SPLIT) {
+#pragma unroll
+                for (int f = 0; f < e; ++f) v[e] = c[f] == c[e] ? v[f] : v[e];
+            }
+            v[e] += x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[c[e] * NT] = v[e];
     }
+    // the lane's part of a bucket's sum over the workgroup, in a fixed order
+    __device__ float part(int b) const {
+        const float *from = at - threadIdx.x + (threadIdx.x & 63);
+        float v = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sums[c[e] * NT] = v[e];
-}
+        for (int e = 0; e < (SPLIT ? 4 : 1); ++e)
+#pragma unroll
+            for (int w = 0; w < NT; w += 64) v += from[(e * (nb + 1) + b) * NT + w];
+        return v;
+    }
+};
 
 // product of a probability and a value: 0 where the probability is 0 (a masked pair), whatever the value
 // (v_mul_legacy_f32)
 extern "C" __device__ float rwk_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ inline float weigh(float p, float x) { return rwk_mul_legacy(p, x); }
 
-// The bias of one head, bucket b in lane b of every wavefront, -infinity from n_buckets on: a look-up fetches another
-// lane's register.
+// The bias of one head times log2(e), bucket b in lane b of every wavefront, -infinity from n_buckets on (a pair that
+// does not attend): a look-up fetches another lane's register.  Finite entries stay finite, the type's lowest value too:
+// a row that has nothing else weighs its pairs alike.
 template <typename T>
 __device__ inline float load_table(const RwkAttnArgs &p, int head) {
     const int b = (int)(threadIdx.x & 63);
-    return b < p.a.n_buckets ? (float)((const T *)p.a.table)[(long long)head * p.a.n_buckets + b] : -INFINITY;
+    const float x = b < p.a.n_buckets ? (float)((const T *)p.a.table)[(long long)head * p.a.n_buckets + b] : -INFINITY;
+    const float most = 3.402823466e38f;
+    return fabsf(x) <= most ? fminf(fmaxf(x * kLog2e, -most), most) : x;
 }
 __device__ inline float look_up(float table, int bucket) {
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * bucket, __builtin_bit_cast(int, table)));
 }
 
-// What the backward pass adds to a row's scores so that their exponential is the probability: minus the forward
-// pass's reference, and the logarithm of 1 / sum.  -infinity for a row without pairs and for rows that do not exist.
-__device__ inline float reference(float ref, float inv, float c) { return __log2f(inv) / c - ref; }
+// How the backward pass has a row's probabilities again: exp2((score + start) c + shift).  Without a bias one number
+// does, the products begin at it.  With one the reference can be so large - a row all of whose pairs carry a mask's
+// -1e9 - that the sum's logarithm would be lost beside it.  -infinity for a row without pairs and for rows that do
+// not exist.
+template <bool BIAS>
+struct RowWeight {
+    float start, shift;
+    __device__ RowWeight(float ref, float inv, float c) {
+        shift = __log2f(inv);
+        start = BIAS ? -ref : shift / c - ref;
+    }
+    __device__ float of(float score, float c) const {          // BIAS: c = 1
+        return exp2_fast(BIAS ? (score + start) + shift : (score + start) * c);
+    }
+};
 
 // ---------------------------------------------------------------------------------------------------------------
 // A pair that does not attend counts for nothing whatever its rows hold, but a matrix instruction adds 0 times what it
@@ -490,7 +602,7 @@ __device__ inline float pair_score(const RwkAttnArgs &p, const Place &at, float 
         const int nb = (int)p.a.n_buckets;
         int b = nb;
         if (on) b = min((int)p.a.codes[p.a.code_start[at.seg] + (long long)q * ((at.n + 31) / 32 * 32) + k], nb);
-        x = fmaf(product, p.a.scale, look_up(table, b));
+        x = fmaf(product, p.a.scale * kLog2e, look_up(table, b));
         on = on && b < nb;
     }
     return on ? x : -INFINITY;
@@ -524,8 +636,8 @@ __device__ inline void exact_forward(const RwkAttnArgs &p, const Place &at, floa
 }
 
 template <typename T, bool BIAS>
-__device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end, float ref, float delta,
-                                float c, bool mine) {
+__device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end,
+                                const RowWeight<BIAS> &weight, float delta, float c, bool mine) {
     const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
     const long long row = at.base + min(q, at.n - 1);
     const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
@@ -538,7 +650,7 @@ __device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float tab
             const T *k_row = row_of<T>(p.a.k, at.base + k, p.a.k_row, at.kv_head, p.a.k_head);
             const T *v_row = row_of<T>(p.a.v, at.base + k, p.a.v_row, at.kv_head, p.a.v_head);
             const float x = pair_score<BIAS>(p, at, table, q, k, row_product(q_row, k_row, h, dim));
-            const float w = weigh(exp2_fast((x + ref) * c), row_product(o_row, v_row, h, dim) - delta);
+            const float w = weigh(weight.of(x, c), row_product(o_row, v_row, h, dim) - delta);
             add_row(g, w, k_row, d, dim);
         }
         if (mine) store_eight<false>((T *)p.a.dq + (row * p.a.heads + at.head) * dim, g, p.a.scale, d, dim);
@@ -563,7 +675,7 @@ __device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int k, i
                 const T *o_row = row_of<T>(p.a.d_out, at.base + q, p.a.do_row, head, p.a.do_head);
                 const long long st = head * p.a.rows + at.base + q;
                 const float x = pair_score<BIAS>(p, at, table, q, k, row_product(k_row, q_row, h, dim));
-                const float w = exp2_fast((x + reference(p.a.stats[2 * st], p.a.stats[2 * st + 1], c)) * c);
+                const float w = RowWeight<BIAS>(p.a.stats[2 * st], p.a.stats[2 * st + 1], c).of(x, c);
                 add_row(gv, w, o_row, d, dim);
                 add_row(gk, weigh(w, row_product(v_row, o_row, h, dim) - p.a.delta[st]), q_row, d, dim);
             }
@@ -591,7 +703,7 @@ template <typename T, int NW> constexpr int tile_rows() { return sizeof(T) == 2 
 constexpr float kSlack = 8.f;
 
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC ? 2 : 1)
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && ASYNC) || KS == 1 ? 2 : 1)
 attention_forward_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
@@ -618,12 +730,10 @@ attention_forward_kernel(const RwkAttnArgs p) {
     if (BIAS) code_tiles.issue(0, codes);
 
     // without a bias the maximum is taken over q . k and the scale meets it in the exponent; with one the scores are
-    // the sum, and the difference is formed before the change of base, so that a bias of the type's lowest value
-    // stays finite
-    const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e, slack = kSlack / c;
-    f32x16 acc[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+    // the sum, in units of log2(e) (load_table)
+    const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale, slack = kSlack / c;
+    Result<T, KS> acc;
+    acc.clear();
     float ref = -INFINITY, sum = 0.f;           // ref: what the exponentials are taken relative to
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
     keys.commit(tiles);
@@ -682,10 +792,7 @@ attention_forward_kernel(const RwkAttnArgs p) {
                 const float shrink = ref == now ? 1.f : exp2_fast((ref - now) * c);
                 ref = now;
                 sum *= shrink;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
+                acc.scale(shrink);
             }
             const float base = ref == -INFINITY ? 0.f : ref, base_c = base * c;
             float part = 0.f;
@@ -693,41 +800,37 @@ attention_forward_kernel(const RwkAttnArgs p) {
             for (int t = 0; t < TN; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[t][i] = exp2_fast(BIAS ? (s[t][i] - base) * c : fmaf(s[t][i], c, -base_c));
+                    s[t][i] = exp2_fast(BIAS ? s[t][i] - base : fmaf(s[t][i], c, -base_c));
                     part += s[t][i];
                 }
             sum += part;
 #pragma unroll
             for (int t = 0; t < TN; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const Frag<T> pf = pack<T>(s[t], u);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        acc[dt] = mma(column_operand<T, KS>(v_tile, 32 * t + 16 * u, dt, lane), pf, acc[dt]);
-                }
+                for (int u = 0; u < 2; ++u) acc.add(v_tile, 32 * t + 16 * u, pack<T>(s[t], u), lane);
         }
         keys.commit(next);
         values.commit(next + BN * S::W);
     }
+    acc.finish();
     sum += __shfl_xor(sum, 32, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;      // a row without pairs: zeros
     const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
-    const bool again = q < n && not_finite<KS>(acc);
+    const bool again = q < n && not_finite<KS>(acc.a);
     if (q < n && !again) {
-        store_rows<false, T, DT>((T *)p.a.out + o_at, dim, h, acc, inv);
-        if (p.a.out_low != nullptr) store_rows<true, T, DT>((T *)p.a.out_low + o_at, dim, h, acc, inv);
+        store_rows<false, T, DT>((T *)p.a.out + o_at, dim, h, acc.a, inv);
+        if (p.a.out_low != nullptr) store_rows<true, T, DT>((T *)p.a.out_low + o_at, dim, h, acc.a, inv);
     }
+    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, ref == -INFINITY ? 0.f : ref, inv, c, again);
     if (q < n && p.a.stats != nullptr && h == 0) {
         float *st = p.a.stats + 2 * (at.head * p.a.rows + at.base + q);
         st[0] = ref == -INFINITY ? 0.f : ref;
         st[1] = inv;
     }
-    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, ref == -INFINITY ? 0.f : ref, inv, c, again);
 }
 
-template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && ASYNC && (!BIAS || KS < 8) ? 2 : 1)
+template <typename T, int KS, int NW, bool BIAS, bool SPLIT, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && ASYNC && (!BIAS || KS < 8)) || KS == 1 ? 2 : 1)
 attention_dq_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
@@ -735,15 +838,13 @@ attention_dq_kernel(const RwkAttnArgs p) {
     T *tiles = (T *)attn_lds;
     uint8_t *codes = (uint8_t *)attn_lds + tiles_bytes<T, KS, BN>();
     typedef CodeLoader<32 * NW, BN, NT> Codes;
-    float *hist = (float *)(codes + 2 * 32 * NW * BN);
     const Place at = query_place(p, blockIdx.x);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int q0 = at.first + 32 * (int)(threadIdx.x >> 6), q = q0 + (lane & 31), qc = q < n ? q : n - 1;
     const bool causal = p.a.causal != 0;
     const int nb = (int)p.a.n_buckets;
     const float table = BIAS ? load_table<T>(p, at.head) : 0.f;
-    if (BIAS)
-        for (int b = 0; b < nb; ++b) hist[b * NT + threadIdx.x] = 0.f;     // a thread's own sums
+    BucketSums<NT, SPLIT> buckets((float *)(codes + 2 * 32 * NW * BN), BIAS ? nb : 0);
 
     TileLoader<T, KS, BN, NT, ASYNC> keys((const T *)p.a.k + at.base * p.a.k_row + at.kv_head * p.a.k_head, p.a.k_row, n, dim);
     TileLoader<T, KS, BN, NT, ASYNC> values((const T *)p.a.v + at.base * p.a.v_row + at.kv_head * p.a.v_head, p.a.v_row, n, dim);
@@ -772,12 +873,11 @@ attention_dq_kernel(const RwkAttnArgs p) {
     if (q < n && h == 0) p.a.delta[row_at] = delta;
     const Codes code_tiles(BIAS ? p.a.codes + p.a.code_start[at.seg] : nullptr, at.first, n);
     if (BIAS) code_tiles.issue(0, codes);
-    const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
-    const float ref = reference(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
+    const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale;
+    const RowWeight<BIAS> weight(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
 
-    f32x16 acc[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+    Result<T, KS> acc;
+    acc.clear();
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
     keys.commit(tiles);
     values.commit(tiles + BN * S::W);
@@ -799,7 +899,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
             f32x16 sx, dx;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                sx[i] = BIAS ? 0.f : ref;
+                sx[i] = BIAS ? 0.f : weight.start;
                 dx[i] = -delta;
             }
 #pragma unroll
@@ -818,7 +918,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int b = code_of(four[g], e, nb);
-                        const float x = fmaf(s[4 * g + e], scale, look_up(table, b)) + ref;
+                        const float x = (fmaf(s[4 * g + e], scale, look_up(table, b)) + weight.start) + weight.shift;
                         s[4 * g + e] = b < nb ? x : -INFINITY;
                     }
                 }
@@ -829,33 +929,25 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 for (int i = 0; i < 16; ++i) s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = weigh(exp2_fast(s[i] * c), d[i]);
+            for (int i = 0; i < 16; ++i) s[i] = weigh(exp2_fast(BIAS ? s[i] : s[i] * c), d[i]);
             if (BIAS && q < n) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) add_by_code<NT>(hist + threadIdx.x, four[g], nb - 1, s + 4 * g);
+                for (int g = 0; g < 4; ++g) buckets.add(four[g], s + 4 * g);
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Frag<T> sf = pack<T>(s, u);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = mma(column_operand<T, KS>(k_tile, 32 * t + 16 * u, dt, lane), sf, acc[dt]);
-            }
+            for (int u = 0; u < 2; ++u) acc.add(k_tile, 32 * t + 16 * u, pack<T>(s, u), lane);
         }
         keys.commit(next);
         values.commit(next + BN * S::W);
     }
-    const bool again = q < n && not_finite<KS>(acc);
-    if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc, scale);
-    if (any_lane(again)) exact_dq<T, BIAS>(p, at, table, q, end, ref, delta, c, again);
+    acc.finish();
+    const bool again = q < n && not_finite<KS>(acc.a);
+    if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc.a, p.a.scale);
+    if (any_lane(again)) exact_dq<T, BIAS>(p, at, table, q, end, weight, delta, c, again);
     if (BIAS) {
         __syncthreads();
-        // a wavefront per bucket sums the threads' slots in a fixed order
-        for (int b = threadIdx.x >> 6; b < nb; b += NW) {
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) v += hist[b * NT + 64 * w + lane];
-            v = rwk_wave_sum(v);
+        for (int b = threadIdx.x >> 6; b < nb; b += NW) {                  // a wavefront per bucket
+            const float v = rwk_wave_sum(buckets.part(b));
             if (lane == 0) p.a.d_table_partials[((long long)at.head * nb + b) * p.a.n_items + at.item] = v;
         }
     }
@@ -863,28 +955,30 @@ attention_dq_kernel(const RwkAttnArgs p) {
 
 // dK and dV of 32 keys per wavefront.  Two wavefronts per SIMD hide each other's exponentials and LDS reads, which
 // leaves 256 registers each: at 128 elements of 16 bits the sums take 128 and the keys 32 of them, and the values stay
-// in LDS.
+// in LDS.  fp32 of up to 16 elements needs half of that, and four hide more (1024 protein-sized graphs: 791 us, 829 by
+// three).
 template <typename T, int KS> constexpr bool values_in_lds() { return sizeof(T) == 2 && KS == 8; }
 template <typename T, int KS, int NW> constexpr int dkv_rows() {
     return values_in_lds<T, KS>() ? 32 : tile_rows<T, NW>();
 }
 template <typename T, int KS, int NW, bool BIAS> constexpr int dkv_lds() {
-    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + 4 * dkv_rows<T, KS, NW>() * (int)sizeof(float) +
+    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + (BIAS ? 6 : 4) * dkv_rows<T, KS, NW>() * (int)sizeof(float) +
            (BIAS ? code_bytes<NW, dkv_rows<T, KS, NW>()>() : 0) +
            (values_in_lds<T, KS>() ? tile_bytes<T, KS, 32 * NW>() : 0);
 }
 
 template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, KS == 8 && (sizeof(T) == 4 || BIAS || !ASYNC) ? 1 : 2)
+__global__ void __launch_bounds__(64 * NW, KS == 8 && (sizeof(T) == 4 || BIAS || !ASYNC) ? 1 : sizeof(T) == 4 && KS == 1 ? 4 : 2)
 attention_dkv_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BQ = dkv_rows<T, KS, NW>(), TQ = BQ / 32;
     constexpr bool VL = values_in_lds<T, KS>();
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;                                       // buffer b: q at 2 b, d_out at 2 b + 1
-    // per buffer and row: the reference, - delta
+    // per buffer and row: the start of its scores, - delta, with a bias the shift of its weights
+    constexpr int NS = BIAS ? 3 : 2;
     float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>());
-    uint8_t *codes = (uint8_t *)(stats + 4 * BQ);
+    uint8_t *codes = (uint8_t *)(stats + 2 * NS * BQ);
     typedef CodeLoader<32 * NW, BQ, NT> Codes;
     T *v_tile = (T *)(codes + (BIAS ? 2 * 32 * NW * BQ : 0));
     const Place at = key_place(p, blockIdx.x);
@@ -908,11 +1002,11 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     }
     const T *v_own = v_tile + 32 * wave * S::W;   // the swizzle repeats: offsets as in the other tiles
     const Codes code_tiles(BIAS ? p.a.codes_by_key + p.a.code_start[at.seg] : nullptr, at.first, n);
-    const float scale = p.a.scale, c = BIAS ? kLog2e : scale * kLog2e;
+    const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale;
 
-    f32x16 dk[DT], dv[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
+    Result<T, KS> dk, dv;
+    dk.clear();
+    dv.clear();
     const int begin = causal ? at.first : 0;
     for (int g = 0; g < p.group; ++g) {
         const int head = at.head + g;
@@ -921,7 +1015,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         TileLoader<T, KS, BQ, NT, ASYNC> grads((const T *)p.a.d_out + at.base * p.a.do_row + head * p.a.do_head, p.a.do_row, n, dim);
         const float table = BIAS ? load_table<T>(p, head) : 0.f;
         __syncthreads();                          // the head before is done with the buffers
-        float held[2];
+        float held[NS];
         const auto start = [&](int q0, int turn) {
             queries.issue(q0, tiles + 2 * turn * BQ * S::W);
             grads.issue(q0, tiles + (2 * turn + 1) * BQ * S::W);
@@ -929,8 +1023,11 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             const int q = q0 + (int)threadIdx.x;
             if (threadIdx.x < BQ) {
                 const bool there = q < n;
-                held[0] = there ? reference(p.a.stats[2 * (row_at + q)], p.a.stats[2 * (row_at + q) + 1], c) : -INFINITY;
+                const RowWeight<BIAS> w(there ? p.a.stats[2 * (row_at + q)] : 0.f,
+                                        there ? p.a.stats[2 * (row_at + q) + 1] : 0.f, c);
+                held[0] = w.start;
                 held[1] = there ? -p.a.delta[row_at + q] : 0.f;
+                if (BIAS) held[NS - 1] = w.shift;
             }
         };
         const auto finish = [&](int turn) {
@@ -938,7 +1035,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             grads.commit(tiles + (2 * turn + 1) * BQ * S::W);
             if (threadIdx.x < BQ) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) stats[(2 * turn + j) * BQ + threadIdx.x] = held[j];
+                for (int j = 0; j < NS; ++j) stats[(NS * turn + j) * BQ + threadIdx.x] = held[j];
             }
         };
         start(begin, 0);
@@ -948,7 +1045,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             tile_ready<ASYNC || BIAS>();
             if (q0 + BQ < n) start(q0 + BQ, turn ^ 1);
             const T *q_tile = tiles + 2 * turn * BQ * S::W, *o_tile = q_tile + BQ * S::W;
-            const float *st = stats + 2 * turn * BQ;
+            const float *st = stats + NS * turn * BQ;
 #pragma unroll
             for (int t = 0; t < TQ; ++t) {
                 const int qt = q0 + 32 * t;
@@ -981,12 +1078,12 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                     for (int g4 = 0; g4 < 4; ++g4) {
                         const int r = 32 * t + 8 * g4 + 4 * h;
                         const uint32_t four = Codes::read(codes + turn * 32 * NW * BQ, k - at.first, r);
-                        const f32x4 ref = *(const f32x4 *)(st + r);
+                        const f32x4 begins = *(const f32x4 *)(st + r), shift = *(const f32x4 *)(st + 2 * BQ + r);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int code = code_of(four, e, nb);
-                            const float x = fmaf(s[4 * g4 + e], scale, look_up(table, code)) + ref[e];
-                            s[4 * g4 + e] = code < nb && q0 + r + e < n ? x : -INFINITY;
+                            const int b = code_of(four, e, nb);
+                            const float x = (fmaf(s[4 * g4 + e], scale, look_up(table, b)) + begins[e]) + shift[e];
+                            s[4 * g4 + e] = b < nb ? x : -INFINITY;
                         }
                     }
                 }
@@ -996,27 +1093,25 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = exp2_fast(s[i] * c);
+                    s[i] = exp2_fast(BIAS ? s[i] : s[i] * c);
                     d[i] = weigh(s[i], d[i]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const Frag<T> pf = pack<T>(s, u), sf = pack<T>(d, u);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        dv[dt] = mma(column_operand<T, KS>(o_tile, 32 * t + 16 * u, dt, lane), pf, dv[dt]);
-                        dk[dt] = mma(column_operand<T, KS>(q_tile, 32 * t + 16 * u, dt, lane), sf, dk[dt]);
-                    }
+                    dv.add(o_tile, 32 * t + 16 * u, pack<T>(s, u), lane);
+                    dk.add(q_tile, 32 * t + 16 * u, pack<T>(d, u), lane);
                 }
             }
             if (q0 + BQ < n) finish(turn ^ 1);
         }
     }
     const long long to = ((at.base + kc) * p.a.kv_heads + at.kv_head) * dim;
-    const bool bad_k = not_finite<KS>(dk), bad_v = not_finite<KS>(dv), again = k < n && (bad_k || bad_v);
+    dk.finish();
+    dv.finish();
+    const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a), again = k < n && (bad_k || bad_v);
     if (k < n && !again) {
-        store_rows<false, T, DT>((T *)p.a.dk + to, dim, h, dk, scale);
-        store_rows<false, T, DT>((T *)p.a.dv + to, dim, h, dv, 1.f);
+        store_rows<false, T, DT>((T *)p.a.dk + to, dim, h, dk.a, p.a.scale);
+        store_rows<false, T, DT>((T *)p.a.dv + to, dim, h, dv.a, 1.f);
     }
     if (any_lane(again)) exact_dkv<T, BIAS>(p, at, k, begin, c, again);
 }
@@ -1038,9 +1133,14 @@ int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
     constexpr int LDS = tiles_bytes<T, KS, ROWS>() + (BIAS ? code_bytes<NW, ROWS>() : 0);
     if (pass == kRwkAttnForward)
         return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT, LDS, p, stream);
-    if (pass == kRwkAttnDq)
-        return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT,
-                             LDS + (BIAS ? p.a.n_buckets * NT * sizeof(float) : 0), p, stream);
+    if (pass == kRwkAttnDq) {
+        const int nb = (int)p.a.n_buckets, split = LDS + 4 * (nb + 1) * NT * (int)sizeof(float);
+        // four sets of bucket sums where three workgroups still share a compute unit's 160 KB
+        if (BIAS && split <= 160 * 1024 / 3)
+            return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT, split, p, stream);
+        return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, false, ASYNC>, p.a.n_items * p.a.heads, NT,
+                             LDS + nb * NT * (int)sizeof(float), p, stream);
+    }
     return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT,
                          dkv_lds<T, KS, NW, BIAS>(), p, stream);
 }

@@ -400,6 +400,20 @@ def test_repeatable_on_any_stream_and_in_a_captured_graph(dev):
 
 
 # --- bucket codes -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", ["lowest", -1e9, -3e4, 3e4, 1e30])
+@pytest.mark.parametrize("dim", [16, 64])
+def test_rows_whose_pairs_all_carry_one_large_bias(dev, dtype, value, dim):
+    """Queries of zeros: every pair's score is the bias alone, and softmax knows differences only, so the results and
+    gradients are those of a bias of zeros, however large it is."""
+    q, k, v, do, bias, codes = make(dev, dtype, [70, 3, 131], 4, 2, dim, seed=5, buckets=3, holes=True)
+    q.zero_()
+    want, err = truth(q, k, v, do, [70, 3, 131], False, bias=torch.zeros_like(bias), codes=codes)
+    lowest = torch.finfo(dtype).min
+    bias.fill_(lowest if value == "lowest" else max(lowest, min(-lowest, value)))
+    check(run(q, k, v, do, [70, 3, 131], False, bias=bias, codes=codes), want, err)
+
+
 def test_dense_and_relative_codes(dev):
     from gnn_amd import packed_segments, pair_buckets, relative_buckets
     lengths = [3, 0, 64, 131, 1]
