@@ -36,7 +36,8 @@ class _Args(ctypes.Structure):
                 ("rows", _I64), ("heads", _I64), ("kv_heads", _I64), ("dim", _I64), ("scale", c_float),
                 ("causal", c_int32), ("type", c_int32), ("block_rows", c_int32), ("stats", _P), ("delta", _P),
                 ("codes", _P), ("codes_by_key", _P), ("code_start", _P), ("table", _P), ("n_buckets", _I64), ("d_table", _P),
-                ("d_table_partials", _P), ("q_items", _P), ("k_items", _P), ("n_items", _I64)]
+                ("d_table_partials", _P), ("q_items", _P), ("k_items", _P), ("n_items", _I64), ("key_parts", c_int32),
+                ("dkv_partials", _P)]
 
 
 class PackedSegments:
@@ -47,8 +48,6 @@ class PackedSegments:
         self.lengths, self.device = lengths, device
         starts = np.concatenate([[0], np.cumsum(lengths)])
         self.n_segments, self.total = int(lengths.size), int(starts[-1])
-        if self.total >= 2 ** 31:
-            raise NotImplementedError("at most 2^31 - 1 rows")
         self.starts = starts
         # Four wavefronts that share the tiles they read pay while most of their 32-row slots are filled; where
         # blocks of 128 rows would hold over half as much padding again as blocks of 32, a wavefront works alone.
@@ -62,12 +61,28 @@ class PackedSegments:
         lists = [np.stack([seg, first], 1)[np.argsort(-work, kind="stable")]
                  for work in (n, np.minimum(n, first + b), n - first)]       # the longest blocks start first
         self.n_items = int(seg.size)
+        # rows that a block of keys meets: at most, and on average per place of 512 (two workgroups a compute unit)
+        self._key_work = [(int(w.max(initial=0)), int(w.sum()) / 512) for w in (n, n - first)]
         packed = torch.from_numpy(np.ascontiguousarray(np.concatenate(
             [starts] + [x.reshape(-1) for x in lists]), dtype=np.int32)).to(device)
         self._arrays = packed
         at = packed.data_ptr()
         self._seg_ptr = at
         self._items, self._q_causal, self._k_causal = (at + 4 * (starts.size + 2 * i * self.n_items) for i in range(3))
+
+    def key_parts(self, heads: int, kv_heads: int, causal: bool) -> int:
+        """Workgroups that share a block of keys in the backward pass, each with its part of the query heads.  Whole,
+        the longest block may be what all others wait for; every part has sums of its own that go through memory
+        once more (a row's as long as 0.006 rows of products, measured) and the parts need a launch to add them.
+        4 prompts of up to 8192 tokens, 4 query heads to a key head, 128 elements: dK and dV 2.32 ms whole, 1.96 ms in
+        two parts and 0.06 ms for their sum; 48 of up to 1500, 64 elements: 256 us whole, 244 and 27 us."""
+        group = heads // kv_heads
+        most, share = self._key_work[causal]
+        share *= heads
+
+        def time(p):
+            return max(most * (group // p), share) + (200 + 0.006 * p * self.total * kv_heads if p > 1 else 0)
+        return min((p for p in range(1, group + 1) if group % p == 0), key=time)
 
     @property
     def seg_ptr(self) -> torch.Tensor:
@@ -97,6 +112,8 @@ def packed_segments(lengths, device=None) -> PackedSegments:
         raise TypeError("lengths must be a list of integers")
     if array.size and int(array.min()) < 0:
         raise ValueError("lengths must not be negative")
+    if sum(array.tolist()) >= 2 ** 31:
+        raise NotImplementedError("at most 2^31 - 1 rows")
     device = torch.device("cuda" if device is None else device)
     if device.type != "cuda":
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
@@ -262,6 +279,10 @@ class _PackedAttention(torch.autograd.Function):
             for t in (dq, dk, dv):
                 t[segments.total:].zero_()
         delta = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
+        a.key_parts = segments.key_parts(q.shape[1], k.shape[1], causal)
+        if a.key_parts > 1:
+            parts = torch.empty((a.key_parts, 2, k.numel()), dtype=torch.float32, device=dev)
+            a.dkv_partials = parts.data_ptr()
         a.out, a.out_low = out.data_ptr(), _lib.ptr(low)
         a.stats, a.delta = stats.data_ptr(), delta.data_ptr()
         a.d_out, a.dq, a.dk, a.dv = d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
@@ -284,7 +305,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
     head ``h // (H / H_kv)``) and D at most 128, all float32, float16 or bfloat16; slices of one projection's output
     are read in place.  ``segments``: which rows belong together (:func:`packed_segments`); rows behind the last
     segment give zeros and take no gradient.  ``causal``: a row attends to itself and the rows before it.  ``scale``:
-    factor of the products, ``D ** -0.5`` by default.  ``bias`` (H, n_buckets <= 32) of the same type, with
+    factor of the products, positive, ``D ** -0.5`` by default.  ``bias`` (H, n_buckets <= 32) of the same type, with
     ``buckets``: added to the scaled products by the pair's bucket; an entry may be ``-inf``.
 
     Returns (N, H, D), contiguous.  A row that attends to nothing gives zeros.  Differentiable once with respect to
@@ -310,8 +331,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
     if segments.n_items * q.shape[1] >= 2 ** 31 or q.shape[0] >= 2 ** 31:
         raise NotImplementedError("more blocks of rows than a launch holds")
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError("scale must be positive and finite")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError("scale must be in 1e-30 .. 1e30")
     if (bias is None) != (buckets is None):
         raise ValueError("bias and buckets go together")
     if bias is not None:

@@ -8,6 +8,7 @@ struct RwkAttnArgs {
     rwk_attention a;          // as the caller described it
     const int *items;         // a.q_items or a.k_items: segment, first row of the block inside the segment
     int group;                // query heads per key / value head
+    int parts, part_heads;    // dK, dV: workgroups that share a block of keys, query heads of each
 };
 
 // Which launch of the operator: the forward pass, dQ (which also leaves delta and the partial sums of d_table) or

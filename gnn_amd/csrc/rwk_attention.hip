@@ -21,6 +21,41 @@ bias_sum_kernel(const float *__restrict__ partials, long long n_items, T *__rest
     if (threadIdx.x == 0) d_table[blockIdx.x] = (T)(part[0] + part[1] + part[2] + part[3]);
 }
 
+// dK and dV from their parts, which lie 2 n elements apart, dV n behind dK: elements of the rows inside segments
+template <typename T>
+__global__ void __launch_bounds__(kBlock)
+dkv_sum_kernel(const float *__restrict__ partials, int parts, long long n, const int *__restrict__ rows, long long width,
+               T *__restrict__ dk, T *__restrict__ dv) {
+    const long long end = *rows * width, i = ((long long)blockIdx.x * kBlock + threadIdx.x) * 4;
+    if (i >= end) return;
+    const float *from = partials + blockIdx.y * n + i;
+    T *to = (blockIdx.y == 0 ? dk : dv) + i;
+    if (i + 4 <= end) {
+        auto sum = rwk_load<float, 4>(from);
+        for (int part = 1; part < parts; ++part) sum += rwk_load<float, 4>(from + 2 * part * n);
+        typename RwkPack<T, 4>::type v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)sum[e];
+        rwk_store<T, 4>(to, v);
+    } else {
+        for (int e = 0; i + e < end; ++e) {
+            float sum = from[e];
+            for (int part = 1; part < parts; ++part) sum += from[2 * part * n + e];
+            to[e] = (T)sum;
+        }
+    }
+}
+
+template <typename T>
+int dkv_sum(const rwk_attention &a, hipStream_t stream) {
+    const long long width = a.kv_heads * a.dim, n = a.rows * width;
+    const dim3 grid((unsigned)rwk_ceil_div(n, 4 * kBlock), 2);
+    hipLaunchKernelGGL(dkv_sum_kernel<T>, grid, dim3(kBlock), 0, stream, a.dkv_partials, (int)a.key_parts, n,
+                       a.seg_ptr + a.n_segments, width, (T *)a.dk, (T *)a.dv);
+    RWK_LAUNCH_CHECK();
+    return RWK_OK;
+}
+
 int bias_sum(const rwk_attention &a, hipStream_t stream) {
     const dim3 grid((unsigned)(a.heads * a.n_buckets));
     if (a.type == RWK_F32)
@@ -43,7 +78,11 @@ int check(const rwk_attention *a, bool backward) {
         a->rows >= 0x7FFFFFFFll || a->n_segments < 0 || a->n_items < 0 || a->n_buckets < 0)
         return RWK_E_SIZE;
     if (a->dim > 128 || a->n_buckets > 32 || (a->block_rows != 32 && a->block_rows != 128)) return RWK_E_UNSUPPORTED;
-    if (!(a->scale > 0.f) || a->n_items > 0x7FFFFFFFll / a->heads) return RWK_E_SIZE;
+    // scales whose reciprocal times log2(e) is a normal number, too
+    if (!(a->scale >= 1e-30f && a->scale <= 1e30f) || a->n_items > 0x7FFFFFFFll / a->heads) return RWK_E_SIZE;
+    if (a->key_parts < 0 || (a->key_parts > 1 && (a->heads / a->kv_heads % a->key_parts != 0 ||
+                                                  a->rows > (1ll << 33) / a->kv_heads)))
+        return RWK_E_SIZE;
     if (a->n_buckets > 0) {
         RWK_REQUIRE_PTR(a->table);
         if (backward) {
@@ -72,6 +111,7 @@ int check(const rwk_attention *a, bool backward) {
         RWK_REQUIRE_PTR(a->stats);
         RWK_REQUIRE_PTR(a->delta);
         RWK_REQUIRE_PTR(a->k_items);
+        if (a->key_parts > 1) RWK_REQUIRE_PTR(a->dkv_partials);
     }
     return RWK_OK;
 }
@@ -81,6 +121,8 @@ int launch(RwkAttnPass pass, const rwk_attention &a, const int32_t *items, hipSt
     p.a = a;
     p.items = items;
     p.group = (int)(a.heads / a.kv_heads);
+    p.parts = a.key_parts > 1 ? a.key_parts : 1;
+    p.part_heads = p.group / p.parts;
     if (a.type == RWK_F32) return rwk_attention_launch_f32(pass, p, stream);
     if (a.type == RWK_F16) return rwk_attention_launch_f16(pass, p, stream);
     return rwk_attention_launch_bf16(pass, p, stream);
@@ -209,6 +251,10 @@ int rwk_attention_backward(const rwk_attention *a, rwk_stream_t stream) {
     if (a->n_items > 0) {
         code = launch(kRwkAttnDq, *a, a->q_items, (hipStream_t)stream);       // leaves delta for the second launch
         if (code == RWK_OK) code = launch(kRwkAttnDkv, *a, a->k_items, (hipStream_t)stream);
+        if (code == RWK_OK && a->key_parts > 1)
+            code = a->type == RWK_F32   ? dkv_sum<float>(*a, (hipStream_t)stream)
+                   : a->type == RWK_F16 ? dkv_sum<rwk_f16>(*a, (hipStream_t)stream)
+                                        : dkv_sum<rwk_bf16>(*a, (hipStream_t)stream);
         if (code != RWK_OK) return code;
     }
     return a->n_buckets > 0 ? bias_sum(*a, (hipStream_t)stream) : RWK_OK;

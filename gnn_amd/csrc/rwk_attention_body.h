@@ -453,9 +453,12 @@ __device__ inline Place query_place(const RwkAttnArgs &p, long long b) {
     find_rows(p, s);
     return s;
 }
-// of a launch over key / value heads
-__device__ inline Place key_place(const RwkAttnArgs &p, long long b) {
+// of a launch over key / value heads and the parts of their query heads
+__device__ inline Place key_place(const RwkAttnArgs &p, long long b, int *part) {
     Place s = place_of(p, b);
+    *part = s.item % p.parts;
+    s.item /= p.parts;
+    s.head += *part * p.part_heads;
     find_rows(p, s);
     return s;
 }
@@ -657,8 +660,23 @@ __device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float tab
     }
 }
 
+// Where dK and dV of a part of the query heads go: straight out, or as fp32 sums for dkv_sum_kernel.
+struct KeyGradients {
+    long long at;                                 // of the workgroup's first key
+    float *dk, *dv;                               // a part's sums, or null
+    __device__ KeyGradients(const RwkAttnArgs &p, const Place &s, int part) {
+        const long long n = p.a.rows * p.a.kv_heads * p.a.dim;
+        at = (s.base * p.a.kv_heads + s.kv_head) * p.a.dim;
+        dk = dv = nullptr;
+        if (p.parts > 1) {
+            dk = p.a.dkv_partials + 2 * part * n + at;
+            dv = dk + n;
+        }
+    }
+};
+
 template <typename T, bool BIAS>
-__device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int k, int begin, float c, bool mine) {
+__device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int part, int k, int begin, float c, bool mine) {
     const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
     const long long row = at.base + min(k, at.n - 1);
     const T *k_row = row_of<T>(p.a.k, row, p.a.k_row, at.kv_head, p.a.k_head);
@@ -667,7 +685,7 @@ __device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int k, i
     for (int d = 8 * h; d < dim + 8 * h; d += 16) {
         float gk[8] = {}, gv[8] = {};
 #pragma unroll 1
-        for (int head = at.head; head < at.head + p.group; ++head) {
+        for (int head = at.head; head < at.head + p.part_heads; ++head) {
             const float table = BIAS ? load_table<T>(p, head) : 0.f;
 #pragma unroll 1
             for (int q = begin; q < at.n; ++q) {
@@ -680,9 +698,15 @@ __device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int k, i
                 add_row(gk, weigh(w, row_product(v_row, o_row, h, dim) - p.a.delta[st]), q_row, d, dim);
             }
         }
-        const long long to = (row * p.a.kv_heads + at.kv_head) * dim;
-        if (mine) store_eight<false>((T *)p.a.dk + to, gk, p.a.scale, d, dim);
-        if (mine) store_eight<false>((T *)p.a.dv + to, gv, 1.f, d, dim);
+        const KeyGradients out(p, at, part);
+        const long long to = (row - at.base) * p.a.kv_heads * dim;
+        if (mine && p.parts > 1) {
+            store_eight<false>(out.dk + to, gk, p.a.scale, d, dim);
+            store_eight<false>(out.dv + to, gv, 1.f, d, dim);
+        } else if (mine) {
+            store_eight<false>((T *)p.a.dk + out.at + to, gk, p.a.scale, d, dim);
+            store_eight<false>((T *)p.a.dv + out.at + to, gv, 1.f, d, dim);
+        }
     }
 }
 
@@ -981,7 +1005,8 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     uint8_t *codes = (uint8_t *)(stats + 2 * NS * BQ);
     typedef CodeLoader<32 * NW, BQ, NT> Codes;
     T *v_tile = (T *)(codes + (BIAS ? 2 * 32 * NW * BQ : 0));
-    const Place at = key_place(p, blockIdx.x);
+    int part;
+    const Place at = key_place(p, blockIdx.x, &part);
     const int lane = threadIdx.x & 63, h = lane >> 5, dim = (int)p.a.dim, n = at.n;
     const int wave = (int)(threadIdx.x >> 6), k0 = at.first + 32 * wave, k = k0 + (lane & 31), kc = min(k, n - 1);
     const bool causal = p.a.causal != 0;
@@ -1008,7 +1033,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     dk.clear();
     dv.clear();
     const int begin = causal ? at.first : 0;
-    for (int g = 0; g < p.group; ++g) {
+    for (int g = 0; g < p.part_heads; ++g) {
         const int head = at.head + g;
         const long long row_at = head * p.a.rows + at.base;
         TileLoader<T, KS, BQ, NT, ASYNC> queries((const T *)p.a.q + at.base * p.a.q_row + head * p.a.q_head, p.a.q_row, n, dim);
@@ -1105,15 +1130,19 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             if (q0 + BQ < n) finish(turn ^ 1);
         }
     }
-    const long long to = ((at.base + kc) * p.a.kv_heads + at.kv_head) * dim;
+    const KeyGradients out(p, at, part);
+    const long long to = kc * p.a.kv_heads * dim;
     dk.finish();
     dv.finish();
     const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a), again = k < n && (bad_k || bad_v);
-    if (k < n && !again) {
-        store_rows<false, T, DT>((T *)p.a.dk + to, dim, h, dk.a, p.a.scale);
-        store_rows<false, T, DT>((T *)p.a.dv + to, dim, h, dv.a, 1.f);
+    if (k < n && !again && p.parts > 1) {
+        store_rows<false, float, DT>(out.dk + to, dim, h, dk.a, p.a.scale);
+        store_rows<false, float, DT>(out.dv + to, dim, h, dv.a, 1.f);
+    } else if (k < n && !again) {
+        store_rows<false, T, DT>((T *)p.a.dk + out.at + to, dim, h, dk.a, p.a.scale);
+        store_rows<false, T, DT>((T *)p.a.dv + out.at + to, dim, h, dv.a, 1.f);
     }
-    if (any_lane(again)) exact_dkv<T, BIAS>(p, at, k, begin, c, again);
+    if (any_lane(again)) exact_dkv<T, BIAS>(p, at, part, k, begin, c, again);
 }
 
 template <typename K>
@@ -1141,7 +1170,7 @@ int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
         return launch_kernel(attention_dq_kernel<T, KS, NW, BIAS, false, ASYNC>, p.a.n_items * p.a.heads, NT,
                              LDS + nb * NT * (int)sizeof(float), p, stream);
     }
-    return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads, NT,
+    return launch_kernel(attention_dkv_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.kv_heads * p.parts, NT,
                          dkv_lds<T, KS, NW, BIAS>(), p, stream);
 }
 
@@ -1149,7 +1178,7 @@ int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
 // tile, are loaded straight into LDS.
 template <typename T>
 bool chunked(const RwkAttnArgs &p, bool backward) {
-    const long long e = 16 / (long long)sizeof(T), far = 0x7FFFFFFFll / (64 * (long long)sizeof(T)) - 1;
+    const long long e = 16 / (long long)sizeof(T), far = 0x7FFFFFFFll / (128 * (long long)sizeof(T)) - 1;
     const auto fits = [&](const void *at, long long row, long long head) {
         return (uintptr_t)at % 16 == 0 && row % e == 0 && head % e == 0 && row >= 0 && row < far;
     };

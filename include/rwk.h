@@ -972,11 +972,12 @@ typedef struct {
     const int32_t *seg_ptr;         /* n_segments + 1 first rows */
     int64_t n_segments, rows;
     int64_t heads, kv_heads, dim;   /* heads a multiple of kv_heads, dim 1 .. 128 */
-    float scale;                    /* positive */
+    float scale;                    /* 1e-30 .. 1e30 */
     int32_t causal;
     int32_t type;                   /* RWK_F32, RWK_F16, RWK_BF16 */
     int32_t block_rows;             /* rows of a block: 32 or 128 */
-    float *stats;                   /* (heads, rows, 2): row maximum and 1 / sum; NULL if no backward pass follows */
+    float *stats;                   /* (heads, rows, 2): what a row's exponentials were taken relative to (with a bias in
+                                     * units of log2(e)) and 1 / their sum; NULL if no backward pass follows */
     float *delta;                   /* (heads, rows), written by the backward pass */
     const uint8_t *codes;           /* rwk_pair_buckets_*, query rows; NULL without a bias */
     const uint8_t *codes_by_key;    /* the same, key rows; backward only */
@@ -989,6 +990,10 @@ typedef struct {
      * segment once; the order decides only which block starts first */
     const int32_t *q_items, *k_items;
     int64_t n_items;
+    /* backward: workgroups that share a block of keys, each with as many of its query heads (1 .. heads / kv_heads, a
+     * divisor; 0: one), and for more than one their sums, (key_parts, 2, rows, kv_heads, dim) */
+    int32_t key_parts;
+    float *dkv_partials;
 } rwk_attention;
 
 int rwk_attention_forward(const rwk_attention *a, rwk_stream_t stream);

@@ -414,6 +414,54 @@ def test_rows_whose_pairs_all_carry_one_large_bias(dev, dtype, value, dim):
     check(run(q, k, v, do, [70, 3, 131], False, bias=bias, codes=codes), want, err)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("parts", [1, 2, 3, 6])
+@pytest.mark.parametrize("dim,buckets", [(37, 0), (128, 0), (16, 5), (64, 5)])
+def test_query_heads_in_parts(dev, dtype, parts, dim, buckets, monkeypatch):
+    """dK and dV summed by several workgroups per block of keys; once with a masked key that is not finite."""
+    from gnn_amd.attention import PackedSegments
+    assert PackedSegments.key_parts(_segments([4096, 100], dev), 6, 1, True) > 1
+    assert PackedSegments.key_parts(_segments([20] * 8, dev), 6, 1, True) == 1
+    monkeypatch.setattr(PackedSegments, "key_parts", lambda *a: parts)
+    lengths = [70, 0, 3, 131]
+    q, k, v, do, bias, codes = make(dev, dtype, lengths, 12, 2, dim, tail=5, seed=parts, buckets=buckets, holes=True)
+    want, err = truth(q, k, v, do, lengths, True, bias=bias, codes=codes)
+    got = run(q, k, v, do, lengths, True, bias=bias, codes=codes)
+    check(got, want, err)
+    for t in got[:4]:
+        assert not t[sum(lengths):].any()
+    do[100], want, err = math.inf, [t[:100] for t in want], [t[:100] for t in err]      # a row of the last segment
+    later = run(q, k, v, do, lengths, True, bias=bias, codes=codes)
+    assert torch.equal(later[0], got[0])
+    assert buckets or not torch.isfinite(later[3][73:101]).all()            # with holes row 100 may attend to nothing
+    for a, b in zip(later[1:4], got[1:4]):
+        assert torch.equal(a[:73], b[:73]) and torch.allclose(a[101:204].double(), b[101:204].double(), rtol=0.1, atol=0.1)
+
+
+def _segments(lengths, dev):
+    from gnn_amd import packed_segments
+    return packed_segments(lengths, dev)
+
+
+@pytest.mark.parametrize("dim,heads", [(128, 1), (64, 2)])
+def test_rows_gigabytes_apart(dev, dim, heads):
+    """Rows of one tile lie further apart than 32-bit offsets reach."""
+    q, k, v, do, _, _ = make(dev, torch.bfloat16, [128], heads, heads, dim, seed=3)
+    apart = (1 << 24) - 8
+    if torch.cuda.mem_get_info(dev)[0] < 16 << 30:
+        pytest.skip("needs 16 GiB of free memory")
+    want = run(q, k, v, do, [128], False)
+    far = torch.empty(128 * apart, dtype=torch.bfloat16, device=dev)
+    wide = [torch.as_strided(far, (128, heads, dim), (apart, dim, 1), at) for at in (0, 1024, 2048)]
+    for x, t in zip(wide, (q, k, v)):
+        x.copy_(t)
+    from gnn_amd import packed_attention
+    leaves = [x.detach().requires_grad_() for x in wide]
+    out = packed_attention(*leaves, _segments([128], dev))
+    for a, b in zip([out, *torch.autograd.grad(out, leaves, do)], want):
+        assert torch.equal(a, b)
+
+
 def test_dense_and_relative_codes(dev):
     from gnn_amd import packed_segments, pair_buckets, relative_buckets
     lengths = [3, 0, 64, 131, 1]
