@@ -181,10 +181,10 @@ def relative_buckets(segments: PackedSegments, n_buckets: int = 32, max_distance
     exact = max(1, per // 2)
     if int(max_distance) <= exact:
         raise ValueError("max_distance must exceed the distances with a bucket of their own (%d)" % exact)
-    reach = int(max_distance)
+    reach = min(int(max_distance), int(segments.lengths.max(initial=1)))       # no rows lie further apart
     d = np.arange(-reach, reach + 1)                            # key row - query row
     dist = np.abs(d) if bidirectional else np.maximum(-d, 0)
-    wide = exact + np.floor(np.log(np.maximum(dist, exact) / exact) / math.log(reach / exact) * (per - exact))
+    wide = exact + np.floor(np.log(np.maximum(dist, exact) / exact) / math.log(int(max_distance) / exact) * (per - exact))
     code = np.where(dist < exact, dist, np.minimum(wide, per - 1)).astype(np.int64)
     if bidirectional:
         code = code + np.where(d > 0, per, 0)

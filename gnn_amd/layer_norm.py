@@ -98,7 +98,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         # little is done here: the engine's thread has just woken up, and everything in it takes twice its time
         rows, weight, stats = ctx.saved_tensors
-        a, dev = ctx.args, dy.device
+        a, dev = _Args.from_buffer_copy(ctx.args), dy.device          # a copy: a graph may be walked by two threads
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
         dw, db = torch.empty((2, a.width), dtype=weight.dtype, device=dev).unbind(0)
         if a.rows == 0:

@@ -351,8 +351,8 @@ class _AdamWTable:
                 self.lr.fill_(lr)
             self.lr_on_device = lr
 
-    def step(self, lib, opt: "AdamW"):
-        import ctypes
+    def gather(self):
+        """Addresses of the gradients, checked; keeps what they belong to, for the launches read it asynchronously."""
         keep, grads = [], []
         for p in self.params:
             g = p.grad
@@ -367,6 +367,11 @@ class _AdamWTable:
                 keep.append(g)
                 g = g.data_ptr()
             grads.append(g)
+        self._keep = keep
+        return grads
+
+    def step(self, lib, opt: "AdamW", grads):
+        import ctypes
         self.push_lr()
         group, stream = self.group, _lib.current_stream(self.device)
         limit = 256                                       # RWK_ADAMW_TENSORS: gradient addresses of one launch
@@ -382,7 +387,6 @@ class _AdamWTable:
                     float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                     float(group["weight_decay"]), opt.seed, self.steps.data_ptr() + 8 * lo, stream),
                     "rwk_adamw_step")
-        self._keep = keep                                 # the launches read them asynchronously
 
     def read_steps(self, opt: "AdamW"):
         steps = self.steps.tolist()
@@ -499,9 +503,19 @@ class AdamW(torch.optim.Optimizer):
         if self._tables is None or any([p.data_ptr() for p in t.params] != t.pointers for t in self._tables):
             self._build_tables()
         lib = _lib.load()
-        for t in self._tables:
-            t.step(lib, self)
+        grads = [t.gather() for t in self._tables]        # all are checked before anything changes
+        for t, g in zip(self._tables, grads):
+            t.step(lib, self, g)
         return loss
+
+    def __getstate__(self):                               # copy.deepcopy, pickle: tables are built anew
+        for t in self._tables or ():
+            t.read_steps(self)
+        return super().__getstate__() | {"state_bits": self.state_bits, "seed": self.seed}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._tables = None
 
     def state_dict(self):
         for t in self._tables or ():                      # the step counts live on the device

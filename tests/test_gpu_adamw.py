@@ -298,3 +298,39 @@ def test_parameters_that_move_and_strided_gradients(dev):
         if t == 0:
             p.data = p.data.clone()                              # another address: the tables follow
     assert torch.equal(p, q) and float(a.state_dict()["state"][0]["step"]) == 3
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_copies_go_on_by_themselves(dev, bits):
+    """A deep copy has tensors of its own, the step counts of the original and the same numbers from then on."""
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.float32, SIZES)
+    opt = AdamW(params, **HYPER, state_bits=bits, seed=7)
+    for gs in grads[:2]:
+        for p, g in zip(params, gs):
+            p.grad = g.clone()
+        opt.step()
+    twin = copy.deepcopy(opt)
+    copies = twin.param_groups[0]["params"]
+    for o, ps in ((opt, params), (twin, copies)):
+        for gs in grads[2:]:
+            for p, g in zip(ps, gs):
+                p.grad = g.clone()
+            o.step()
+    assert all(a.data_ptr() != b.data_ptr() and torch.equal(a, b) for a, b in zip(params, copies))
+    a, b = (o.state_dict()["state"] for o in (opt, twin))
+    assert all(int(a[i]["step"]) == 4 == int(b[i]["step"]) for i in a)
+
+
+def test_a_refused_step_changes_nothing(dev):
+    """Gradients are checked before the first launch, those of later groups and types too."""
+    from gnn_amd import AdamW
+    a, b = torch.nn.Parameter(torch.ones(300, device=dev)), torch.nn.Parameter(torch.ones(5, device=dev).half())
+    opt = AdamW([{"params": [a]}, {"params": [b], "lr": 1.0}])
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    before = a.detach().clone()
+    b.grad = torch.sparse_coo_tensor(torch.tensor([[0]], device=dev), torch.ones(1, device=dev).half(), (5,))
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert torch.equal(a, before) and int(opt.state_dict()["state"][0]["step"]) == 1

@@ -491,6 +491,14 @@ def test_dense_and_relative_codes(dev):
             3).cpu().numpy()[7, 5])
 
 
+def test_relative_codes_of_a_reach_beyond_any_segment(dev):
+    from gnn_amd import packed_segments, relative_buckets
+    seg = packed_segments([9, 33], dev)
+    got = relative_buckets(seg, 8, 2 ** 40, False)
+    assert got.dense(1)[32, :].tolist() == [4] * 29 + [3, 2, 1, 0] and got.dense(1)[0, 1:].eq(0).all()
+    assert torch.equal(got.dense(0), got.dense(1)[:9, :9])
+
+
 @pytest.mark.parametrize("far", ["bucket", "mask"])
 def test_hop_codes(dev, far):
     import os

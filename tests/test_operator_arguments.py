@@ -106,6 +106,30 @@ def test_pair_bucket_entry_points(lib):
     assert lib.rwk_pair_buckets_dense(None, None, None, None, None, 0, 32, None, None, None) == 0
 
 
+def test_attention_scales_and_parts(lib):
+    from gnn_amd.attention import _Args
+
+    def call(**k):
+        a = _Args()
+        for name in ("q", "k", "v", "out", "d_out", "dq", "dk", "dv", "seg_ptr", "stats", "delta", "q_items", "k_items"):
+            setattr(a, name, A)
+        for name, value in (dict(heads=12, kv_heads=2, dim=64, rows=10, n_segments=1, n_items=1, scale=1.0, type=0,
+                                 block_rows=32) | k).items():
+            setattr(a, name, value)
+        return lib.rwk_attention_backward(ctypes.addressof(a), None)
+    for bad in (dict(scale=1e-31), dict(scale=1e31), dict(scale=float("inf")), dict(key_parts=-1), dict(key_parts=4),
+                dict(key_parts=12), dict(key_parts=5)):
+        assert call(**bad) == SIZE, bad
+    assert call(key_parts=3) == NULL                           # no place for the parts' sums
+
+
+def test_lengths_that_wrap_around():
+    from gnn_amd import packed_segments
+    for lengths in ([2 ** 62, 2 ** 62, 2 ** 62, 2 ** 62], [2 ** 31], torch.tensor([2 ** 30, 2 ** 30])):
+        with pytest.raises(NotImplementedError, match="rows"):
+            packed_segments(lengths)
+
+
 def test_no_cpu_fallback():
     from gnn_amd import AdamW, layer_norm, packed_attention, packed_segments
     with pytest.raises(RuntimeError, match="HIP devices only"):
