@@ -221,8 +221,8 @@ def _describe(q, k, v, segments, causal, scale, table, buckets):
     a.q_row, a.q_head, _ = q.stride()
     a.k_row, a.k_head, _ = k.stride()
     a.v_row, a.v_head, _ = v.stride()
-    a.seg_ptr, a.n_segments, a.rows = segments._seg_ptr, segments.n_segments, q.shape[0]
-    a.heads, a.dim = q.shape[1:]
+    a.seg_ptr, a.n_segments = segments._seg_ptr, segments.n_segments
+    a.rows, a.heads, a.dim = q.shape
     a.kv_heads = k.shape[1]
     a.scale, a.causal, a.type = scale, causal, _lib.element_type(q.dtype)
     a.block_rows, a.n_items = segments.block_rows, segments.n_items
@@ -237,19 +237,20 @@ def _describe(q, k, v, segments, causal, scale, table, buckets):
 
 def _forward(q, k, v, segments, causal, scale, table, buckets, stats):
     a = _describe(q, k, v, segments, causal, scale, table, buckets)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if segments.total < q.shape[0]:
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if segments.total < a.rows:
         out[segments.total:].zero_()
     st = low = None
     a.out = out.data_ptr()
     if stats:
-        st = torch.empty((q.shape[1], q.shape[0], 2), dtype=torch.float32, device=q.device)
+        st = torch.empty((a.heads, a.rows, 2), dtype=torch.float32, device=q.device)
         a.stats = st.data_ptr()
         if a.type:                                     # 16 bits: what the rounding of out leaves over
             low = torch.empty_like(out)
             a.out_low = low.data_ptr()
-    with _lib.device_guard(q.device):
-        _lib.check(_lib.load().rwk_attention_forward(ctypes.addressof(a), _lib.current_stream(q.device)),
+    dev = segments.device
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().rwk_attention_forward(ctypes.addressof(a), _lib.current_stream(dev)),
                    "rwk_attention_forward")
     return out, st, low
 
@@ -314,33 +315,36 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
     attend, values that are not finite included (blocks of rows whose result is not finite take much longer)."""
     if not q.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
-    _lib.element_type(q.dtype)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"expected q (N, H, D), k and v (N, H_kv, D), got {tuple(q.shape)}, {tuple(k.shape)}, "
+    shape, k_shape, dtype, device = q.shape, k.shape, q.dtype, q.device          # every look costs a small call time
+    _lib.element_type(dtype)
+    if len(shape) != 3 or len(k_shape) != 3 or k_shape != v.shape or shape[0] != k_shape[0] or shape[2] != k_shape[2]:
+        raise ValueError(f"expected q (N, H, D), k and v (N, H_kv, D), got {tuple(shape)}, {tuple(k_shape)}, "
                          f"{tuple(v.shape)}")
-    if q.shape[1] < 1 or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{q.shape[1]} query heads cannot share {k.shape[1]} key / value heads")
-    if not 1 <= q.shape[2] <= 128:
+    rows, heads, dim = shape
+    kv_heads = k_shape[1]
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} key / value heads")
+    if not 1 <= dim <= 128:
         raise NotImplementedError("heads of 1 to 128 elements")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("q, k and v must have the same type")
-    if k.device != q.device or v.device != q.device or segments.device != q.device:
+    if k.device != device or v.device != device or segments.device != device:
         raise RuntimeError("q, k, v and segments must be on the same device")
-    if segments.total > q.shape[0]:
-        raise ValueError(f"the segments cover {segments.total} rows of {q.shape[0]}")
-    if segments.n_items * q.shape[1] >= 2 ** 31 or q.shape[0] >= 2 ** 31:
+    if segments.total > rows:
+        raise ValueError(f"the segments cover {segments.total} rows of {rows}")
+    if segments.n_items * heads >= 2 ** 31 or rows >= 2 ** 31:
         raise NotImplementedError("more blocks of rows than a launch holds")
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    scale = dim ** -0.5 if scale is None else float(scale)
     if not 1e-30 <= scale <= 1e30:
         raise ValueError("scale must be in 1e-30 .. 1e30")
     if (bias is None) != (buckets is None):
         raise ValueError("bias and buckets go together")
     if bias is not None:
-        if bias.dim() != 2 or bias.shape[0] != q.shape[1] or not 1 <= bias.shape[1] <= 32:
-            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({q.shape[1]}, 1..32)")
-        if bias.dtype != q.dtype:
+        if bias.dim() != 2 or bias.shape[0] != heads or not 1 <= bias.shape[1] <= 32:
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({heads}, 1..32)")
+        if bias.dtype is not dtype:
             raise TypeError("bias must have the type of q")
-        if bias.device != q.device:
+        if bias.device != device:
             raise RuntimeError("q and bias must be on the same device")
         if buckets.segments is not segments:
             raise ValueError("the buckets were made for other segments")

@@ -41,19 +41,20 @@ def _rows(t: torch.Tensor):
 def _check(x, weight, bias):
     if not x.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
-    _lib.element_type(x.dtype)
-    if x.dim() < 1 or x.shape[-1] == 0:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    _lib.element_type(dtype)
+    if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("x needs a last dimension of at least one")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
-            raise ValueError(f"{name} has shape {tuple(t.shape)} for rows of {x.shape[-1]}")
-        if t.dtype != x.dtype and t.dtype != torch.float32:
+        if tuple(t.shape) != shape[-1:]:
+            raise ValueError(f"{name} has shape {tuple(t.shape)} for rows of {shape[-1]}")
+        if t.dtype is not dtype and t.dtype is not torch.float32:
             raise TypeError(f"{name} must have the type of x or float32")
-        if t.device != x.device:
+        if t.device != device:
             raise RuntimeError(f"x and {name} must be on the same device")
-    if bias is not None and bias.dtype != weight.dtype:
+    if bias is not None and bias.dtype is not weight.dtype:
         raise TypeError("weight and bias must have the same type")
 
 
@@ -62,9 +63,10 @@ def _forward(x, weight, bias, eps, keep):
     call's arguments."""
     rows, stride = _rows(x)
     dev, a = x.device, _Args()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    a.x_stride, a.width, a.eps = stride, x.shape[-1], eps
-    a.rows = n = x.numel() // x.shape[-1]
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    width = x.shape[-1]
+    a.x_stride, a.width, a.eps = stride, width, eps
+    a.rows = n = x.numel() // width
     a.type, a.weight_type = _lib.element_type(x.dtype), _lib.element_type(weight.dtype)
     stats = None
     if keep:

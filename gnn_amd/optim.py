@@ -354,14 +354,14 @@ class _AdamWTable:
     def gather(self):
         """Addresses of the gradients, checked; keeps what they belong to, for the launches read it asynchronously."""
         keep, grads = [], []
+        dtype, device, strided = self.dtype, self.device, torch.strided
         for p in self.params:
             g = p.grad
             if g is not None:
-                if g.layout != torch.strided:
+                if g.layout is not strided:
                     raise RuntimeError("gnn_amd.AdamW does not take sparse gradients")
-                if g.dtype is not self.dtype or g.device != self.device:
+                if g.dtype is not dtype or g.device != device:
                     raise TypeError("a gradient must have its parameter's type and device")
-                g = g.detach()
                 if not g.is_contiguous():
                     g = g.contiguous()
                 keep.append(g)
