@@ -101,7 +101,7 @@ class _LayerNorm(torch.autograd.Function):
         # little is done here: the engine's thread has just woken up, and everything in it takes twice its time
         rows, weight, stats = ctx.saved_tensors
         a, dev = _Args.from_buffer_copy(ctx.args), dy.device          # a copy: a graph may be walked by two threads
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
         dw, db = torch.empty((2, a.width), dtype=weight.dtype, device=dev).unbind(0)
         if a.rows == 0:
             dw.zero_()
@@ -116,7 +116,6 @@ class _LayerNorm(torch.autograd.Function):
                 _lib.check(_lib.load().rwk_layer_norm_backward(ctypes.addressof(a), _lib.current_stream(dev)),
                            "rwk_layer_norm_backward")
         return dx, dw, db if ctx.has_bias else None, None
-
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, eps: float = 1e-5) -> torch.Tensor:
     """``x`` (..., D) float32, float16 or bfloat16; ``weight`` and ``bias`` (D,) of the same type or both float32.

@@ -228,3 +228,17 @@ def test_gradient_against_differences(dev):
                 vals.append(loss(*args))
             diff = (vals[0] - vals[1]) / (2 * step)
             assert abs(diff - float(grad.view(-1)[i])) <= 1e-4 * (1 + abs(diff))
+
+
+def test_one_derivative(dev):
+    """Gradients may be asked for with a graph; their own derivative raises."""
+    from gnn_amd import layer_norm
+    x, w, b, dy = make(dev, 20, 33, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    plain = torch.autograd.grad(layer_norm(*leaves), leaves, dy)
+    y = layer_norm(*leaves)
+    again = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    graph = torch.autograd.grad(y, leaves, dy.requires_grad_(), create_graph=True)
+    assert all(torch.equal(p, a) and torch.equal(p, g) for p, a, g in zip(plain, again, graph))
+    with pytest.raises(RuntimeError, match="once"):
+        graph[0].sum().backward()
