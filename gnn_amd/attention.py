@@ -36,7 +36,7 @@ class _Args(ctypes.Structure):
                 ("rows", _I64), ("heads", _I64), ("kv_heads", _I64), ("dim", _I64), ("scale", c_float),
                 ("causal", c_int32), ("type", c_int32), ("block_rows", c_int32), ("stats", _P), ("delta", _P),
                 ("codes", _P), ("codes_by_key", _P), ("code_start", _P), ("table", _P), ("n_buckets", _I64), ("d_table", _P),
-                ("d_table_partials", _P), ("q_items", _P), ("k_items", _P), ("n_items", _I64), ("key_parts", c_int32),
+                ("d_table_partials", _P), ("q_items", _P), ("k_items", _P), ("n_items", _I64), ("key_parts", c_int32), ("few_keys", c_int32),
                 ("dkv_partials", _P)]
 
 
@@ -61,6 +61,7 @@ class PackedSegments:
         lists = [np.stack([seg, first], 1)[np.argsort(-work, kind="stable")]
                  for work in (n, np.minimum(n, first + b), n - first)]       # the longest blocks start first
         self.n_items = int(seg.size)
+        self.few_keys = int(lengths.max(initial=0)) <= 256
         # rows that a block of keys meets: at most, and on average per place of 512 (two workgroups a compute unit)
         self._key_work = [(int(w.max(initial=0)), int(w.sum()) / 512) for w in (n, n - first)]
         packed = torch.from_numpy(np.ascontiguousarray(np.concatenate(
@@ -225,7 +226,7 @@ def _describe(q, k, v, segments, causal, scale, table, buckets):
     a.rows, a.heads, a.dim = q.shape
     a.kv_heads = k.shape[1]
     a.scale, a.causal, a.type = scale, causal, _lib.element_type(q.dtype)
-    a.block_rows, a.n_items = segments.block_rows, segments.n_items
+    a.block_rows, a.n_items, a.few_keys = segments.block_rows, segments.n_items, segments.few_keys
     a.q_items = segments._q_causal if causal else segments._items
     a.k_items = segments._k_causal if causal else segments._items
     if table is not None:

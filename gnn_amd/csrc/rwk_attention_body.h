@@ -368,6 +368,14 @@ struct Result {
 #pragma unroll
         for (int dt = 0; dt < Shape<T, KS>::DT; ++dt) a[dt] = mma(column_operand<T, KS>(tile, first, dt, lane), f, a[dt]);
     }
+    // the same with what the rounding of the weights left over
+    __device__ void add(const T *tile, int first, const Frag<T> &f, const Frag<T> &rest, int lane) {
+#pragma unroll
+        for (int dt = 0; dt < Shape<T, KS>::DT; ++dt) {
+            const Frag<T> x = column_operand<T, KS>(tile, first, dt, lane);
+            a[dt] = mma(x, f, mma(x, rest, a[dt]));
+        }
+    }
     __device__ void finish() {}
 };
 
@@ -530,20 +538,26 @@ __device__ inline float look_up(float table, int bucket) {
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * bucket, __builtin_bit_cast(int, table)));
 }
 
-// How the backward pass has a row's probabilities again: exp2((score + start) c + shift).  Without a bias one number
-// does, the products begin at it.  With one the reference can be so large - a row all of whose pairs carry a mask's
-// -1e9 - that the sum's logarithm would be lost beside it.  -infinity for a row without pairs and for rows that do
-// not exist.
-template <bool BIAS>
+// How the backward pass has a row's probabilities again: exp2((score + start) c) * factor.  16-bit types without a bias
+// begin their products at a start that holds the logarithm of the factor too, and save the product.  With a bias that
+// would be lost beside a large reference - a row all of whose pairs carry a mask's -1e9 - and for fp32 the rounding of
+// the larger exponent would be the largest error of all: there the exponentials are the forward pass's, bit for bit.
+// start -infinity or factor 0 for a row without pairs and for rows that do not exist.
+template <typename T, bool BIAS>
 struct RowWeight {
-    float start, shift;
+    static constexpr bool FOLDED = sizeof(T) == 2 && !BIAS;
+    float start, factor;
     __device__ RowWeight(float ref, float inv, float c) {
-        shift = __log2f(inv);
-        start = BIAS ? -ref : shift / c - ref;
+        start = FOLDED ? __log2f(inv) / c - ref : BIAS ? -ref : -(ref * c);
+        factor = inv;
     }
-    __device__ float of(float score, float c) const {          // BIAS: c = 1
-        return exp2_fast(BIAS ? (score + start) + shift : (score + start) * c);
+    // what the product begins at, and the weight from what it ends at or, with a bias, from the score
+    __device__ float begin() const { return FOLDED ? start : 0.f; }
+    __device__ static float weight(float x, float start, float factor, float c) {
+        if (FOLDED) return exp2_fast(x * c);
+        return exp2_fast(BIAS ? x + start : fmaf(x, c, start)) * factor;
     }
+    __device__ float of(float score, float c) const { return weight(score + begin(), start, factor, c); }
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -640,7 +654,7 @@ __device__ inline void exact_forward(const RwkAttnArgs &p, const Place &at, floa
 
 template <typename T, bool BIAS>
 __device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end,
-                                const RowWeight<BIAS> &weight, float delta, float c, bool mine) {
+                                const RowWeight<T, BIAS> &weight, float delta, float c, bool mine) {
     const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
     const long long row = at.base + min(q, at.n - 1);
     const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
@@ -693,7 +707,7 @@ __device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int part
                 const T *o_row = row_of<T>(p.a.d_out, at.base + q, p.a.do_row, head, p.a.do_head);
                 const long long st = head * p.a.rows + at.base + q;
                 const float x = pair_score<BIAS>(p, at, table, q, k, row_product(k_row, q_row, h, dim));
-                const float w = RowWeight<BIAS>(p.a.stats[2 * st], p.a.stats[2 * st + 1], c).of(x, c);
+                const float w = RowWeight<T, BIAS>(p.a.stats[2 * st], p.a.stats[2 * st + 1], c).of(x, c);
                 add_row(gv, w, o_row, d, dim);
                 add_row(gk, weigh(w, row_product(v_row, o_row, h, dim) - p.a.delta[st]), q_row, d, dim);
             }
@@ -726,8 +740,12 @@ template <typename T, int NW> constexpr int tile_rows() { return sizeof(T) == 2 
 // the probabilities inside fp16's) range.
 constexpr float kSlack = 8.f;
 
-template <typename T, int KS, int NW, bool BIAS, bool ASYNC>
-__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && ASYNC) || KS == 1 ? 2 : 1)
+// FINE (16-bit types): a weight meets the values as two numbers of the type, the second what the rounding to the first
+// left over.  The weights' rounding counts most where few of them are added up and, through delta, which comes from the
+// output, in the query gradients of narrow heads.  Half as many products more, and the registers of a wavefront per
+// SIMD: 48 prompts of up to 1500 rows, 64 elements, 193 us against 149; so wide heads have it for short segments only.
+template <typename T, int KS, int NW, bool BIAS, bool FINE, bool ASYNC>
+__global__ void __launch_bounds__(64 * NW, (sizeof(T) == 2 && ASYNC && !(FINE && KS == 8)) || KS == 1 ? 2 : 1)
 attention_forward_kernel(const RwkAttnArgs p) {
     using S = Shape<T, KS>;
     constexpr int NT = 64 * NW, DT = S::DT, BN = tile_rows<T, NW>(), TN = BN / 32;
@@ -831,7 +849,19 @@ attention_forward_kernel(const RwkAttnArgs p) {
 #pragma unroll
             for (int t = 0; t < TN; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) acc.add(v_tile, 32 * t + 16 * u, pack<T>(s[t], u), lane);
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> f = pack<T>(s[t], u);
+                    if constexpr (sizeof(T) == 2) {
+                        if (FINE) {
+                            Frag<T> rest;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) rest.v[e] = (T)(s[t][8 * u + e] - (float)f.v[e]);
+                            acc.add(v_tile, 32 * t + 16 * u, f, rest, lane);
+                            continue;
+                        }
+                    }
+                    acc.add(v_tile, 32 * t + 16 * u, f, lane);
+                }
         }
         keys.commit(next);
         values.commit(next + BN * S::W);
@@ -878,12 +908,19 @@ attention_dq_kernel(const RwkAttnArgs p) {
     const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
     const T *q_row = (const T *)p.a.q + (at.base + qc) * p.a.q_row + at.head * p.a.q_head;
     const T *do_row = (const T *)p.a.d_out + (at.base + qc) * p.a.do_row + at.head * p.a.do_head;
+    // fp32: delta by the instructions that give d_out . v, as the diagonal of a product, so that a row that one pair
+    // takes nearly whole has the difference of two equal sums
     float delta = 0.f;
+    f32x16 deltas = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         qf[ks] = load_global<T>(q_row, 16 * ks + 8 * h, dim);
         of[ks] = load_global<T>(do_row, 16 * ks + 8 * h, dim);
         const Frag<T> o = load_global<T>((const T *)p.a.out + o_at, 16 * ks + 8 * h, dim);
+        if constexpr (sizeof(T) == 4) {
+            deltas = mma(o, of[ks], deltas);
+            continue;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf((float)of[ks].v[e], (float)o.v[e], delta);
         if (sizeof(T) == 2 && p.a.out_low != nullptr) {
@@ -892,13 +929,17 @@ attention_dq_kernel(const RwkAttnArgs p) {
             for (int e = 0; e < 8; ++e) delta = fmaf((float)of[ks].v[e], (float)low.v[e], delta);
         }
     }
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) delta = reg_row(i, h) == (lane & 31) ? deltas[i] : delta;
+    }
     delta += __shfl_xor(delta, 32, 64);
     const long long row_at = at.head * p.a.rows + at.base + qc;
     if (q < n && h == 0) p.a.delta[row_at] = delta;
     const Codes code_tiles(BIAS ? p.a.codes + p.a.code_start[at.seg] : nullptr, at.first, n);
     if (BIAS) code_tiles.issue(0, codes);
     const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale;
-    const RowWeight<BIAS> weight(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
+    const RowWeight<T, BIAS> weight(p.a.stats[2 * row_at], p.a.stats[2 * row_at + 1], c);
 
     Result<T, KS> acc;
     acc.clear();
@@ -919,12 +960,12 @@ attention_dq_kernel(const RwkAttnArgs p) {
         for (int t = 0; t < TN; ++t) {
             const int kt = k0 + 32 * t;
             if (q0 >= n || kt >= n || (causal && kt > q0 + 31)) break;
-            // the products begin at the row's reference and at minus its delta
+            // the products begin at the row's reference and, 16-bit types, at minus its delta
             f32x16 sx, dx;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                sx[i] = BIAS ? 0.f : weight.start;
-                dx[i] = -delta;
+                sx[i] = weight.begin();
+                dx[i] = sizeof(T) == 2 ? -delta : 0.f;
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -934,6 +975,8 @@ attention_dq_kernel(const RwkAttnArgs p) {
             float s[16], d[16];
             unpack(sx, s);
             unpack(dx, d);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) d[i] -= sizeof(T) == 2 ? 0.f : delta;
             uint32_t four[4];
             if (BIAS) {
 #pragma unroll
@@ -942,7 +985,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int b = code_of(four[g], e, nb);
-                        const float x = (fmaf(s[4 * g + e], scale, look_up(table, b)) + weight.start) + weight.shift;
+                        const float x = fmaf(s[4 * g + e], scale, look_up(table, b));
                         s[4 * g + e] = b < nb ? x : -INFINITY;
                     }
                 }
@@ -953,7 +996,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 for (int i = 0; i < 16; ++i) s[i] = kt + reg_row(i, h) <= last ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = weigh(exp2_fast(BIAS ? s[i] : s[i] * c), d[i]);
+            for (int i = 0; i < 16; ++i) s[i] = weigh(weight.weight(s[i], weight.start, weight.factor, c), d[i]);
             if (BIAS && q < n) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) buckets.add(four[g], s + 4 * g);
@@ -986,7 +1029,7 @@ template <typename T, int KS, int NW> constexpr int dkv_rows() {
     return values_in_lds<T, KS>() ? 32 : tile_rows<T, NW>();
 }
 template <typename T, int KS, int NW, bool BIAS> constexpr int dkv_lds() {
-    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + (BIAS ? 6 : 4) * dkv_rows<T, KS, NW>() * (int)sizeof(float) +
+    return tiles_bytes<T, KS, dkv_rows<T, KS, NW>()>() + (BIAS || sizeof(T) == 4 ? 6 : 4) * dkv_rows<T, KS, NW>() * (int)sizeof(float) +
            (BIAS ? code_bytes<NW, dkv_rows<T, KS, NW>()>() : 0) +
            (values_in_lds<T, KS>() ? tile_bytes<T, KS, 32 * NW>() : 0);
 }
@@ -999,8 +1042,8 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     constexpr bool VL = values_in_lds<T, KS>();
     extern __shared__ __attribute__((aligned(16))) char attn_lds[];
     T *tiles = (T *)attn_lds;                                       // buffer b: q at 2 b, d_out at 2 b + 1
-    // per buffer and row: the start of its scores, - delta, with a bias the shift of its weights
-    constexpr int NS = BIAS ? 3 : 2;
+    typedef RowWeight<T, BIAS> Weight;
+    constexpr int NS = Weight::FOLDED ? 2 : 3;                      // per buffer and row: start, - delta, factor
     float *stats = (float *)(attn_lds + tiles_bytes<T, KS, BQ>());
     uint8_t *codes = (uint8_t *)(stats + 2 * NS * BQ);
     typedef CodeLoader<32 * NW, BQ, NT> Codes;
@@ -1048,11 +1091,11 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             const int q = q0 + (int)threadIdx.x;
             if (threadIdx.x < BQ) {
                 const bool there = q < n;
-                const RowWeight<BIAS> w(there ? p.a.stats[2 * (row_at + q)] : 0.f,
-                                        there ? p.a.stats[2 * (row_at + q) + 1] : 0.f, c);
+                const Weight w(there ? p.a.stats[2 * (row_at + q)] : 0.f,
+                               there ? p.a.stats[2 * (row_at + q) + 1] : 0.f, c);
                 held[0] = w.start;
                 held[1] = there ? -p.a.delta[row_at + q] : 0.f;
-                if (BIAS) held[NS - 1] = w.shift;
+                if (!Weight::FOLDED) held[NS - 1] = w.factor;
             }
         };
         const auto finish = [&](int turn) {
@@ -1080,12 +1123,12 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                 f32x16 sx, dx;
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
-                    const f32x4 r = *(const f32x4 *)(st + 32 * t + 8 * g4 + 4 * h);
-                    const f32x4 d = *(const f32x4 *)(st + BQ + 32 * t + 8 * g4 + 4 * h);
+                    const int r = 32 * t + 8 * g4 + 4 * h;
+                    const f32x4 begins = *(const f32x4 *)(st + r), d = *(const f32x4 *)(st + BQ + r);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        sx[4 * g4 + e] = BIAS ? 0.f : r[e];
-                        dx[4 * g4 + e] = d[e];
+                        sx[4 * g4 + e] = Weight::FOLDED ? begins[e] : 0.f;
+                        dx[4 * g4 + e] = sizeof(T) == 2 ? d[e] : 0.f;
                     }
                 }
 #pragma unroll
@@ -1103,11 +1146,10 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                     for (int g4 = 0; g4 < 4; ++g4) {
                         const int r = 32 * t + 8 * g4 + 4 * h;
                         const uint32_t four = Codes::read(codes + turn * 32 * NW * BQ, k - at.first, r);
-                        const f32x4 begins = *(const f32x4 *)(st + r), shift = *(const f32x4 *)(st + 2 * BQ + r);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int b = code_of(four, e, nb);
-                            const float x = (fmaf(s[4 * g4 + e], scale, look_up(table, b)) + begins[e]) + shift[e];
+                            const float x = fmaf(s[4 * g4 + e], scale, look_up(table, b));
                             s[4 * g4 + e] = b < nb ? x : -INFINITY;
                         }
                     }
@@ -1118,7 +1160,9 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = exp2_fast(BIAS ? s[i] : s[i] * c);
+                    const int r = 32 * t + reg_row(i, h);
+                    if (sizeof(T) == 4) d[i] += st[BQ + r];
+                    s[i] = Weight::FOLDED ? Weight::weight(s[i], 0.f, 1.f, c) : Weight::weight(s[i], st[r], st[2 * BQ + r], c);
                     d[i] = weigh(s[i], d[i]);
                 }
 #pragma unroll
@@ -1160,8 +1204,14 @@ template <typename T, int KS, bool WIDE, bool BIAS, bool ASYNC>
 int launch_shape(RwkAttnPass pass, const RwkAttnArgs &p, hipStream_t stream) {
     constexpr int NW = WIDE ? 4 : 1, NT = 64 * NW, ROWS = tile_rows<T, NW>();
     constexpr int LDS = tiles_bytes<T, KS, ROWS>() + (BIAS ? code_bytes<NW, ROWS>() : 0);
-    if (pass == kRwkAttnForward)
-        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, ASYNC>, p.a.n_items * p.a.heads, NT, LDS, p, stream);
+    if (pass == kRwkAttnForward) {
+        constexpr bool NARROW = sizeof(T) == 2 && KS <= 2;
+        if (sizeof(T) == 2 && p.a.few_keys)
+            return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, sizeof(T) == 2, ASYNC>, p.a.n_items * p.a.heads,
+                                 NT, LDS, p, stream);
+        return launch_kernel(attention_forward_kernel<T, KS, NW, BIAS, NARROW, ASYNC>, p.a.n_items * p.a.heads, NT, LDS,
+                             p, stream);
+    }
     if (pass == kRwkAttnDq) {
         const int nb = (int)p.a.n_buckets, split = LDS + 4 * (nb + 1) * NT * (int)sizeof(float);
         // four sets of bucket sums where three workgroups still share a compute unit's 160 KB

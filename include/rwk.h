@@ -993,6 +993,7 @@ typedef struct {
     /* backward: workgroups that share a block of keys, each with as many of its query heads (1 .. heads / kv_heads, a
      * divisor; 0: one), and for more than one their sums, (key_parts, 2, rows, kv_heads, dim) */
     int32_t key_parts;
+    int32_t few_keys;               /* forward, 16-bit types: segments are short, keep more of the weights' bits */
     float *dkv_partials;
 } rwk_attention;
 
