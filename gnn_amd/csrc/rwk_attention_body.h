@@ -507,6 +507,15 @@ struct BucketSums {
 #pragma unroll
         for (int e = 0; e < 4; ++e) at[c[e] * NT] = v[e];
     }
+    __device__ void add_all(uint32_t codes, const float (&x)[16]) {       // of one code
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += x[i];
+        at[code_of(codes, 0, SPLIT ? nb : nb - 1) * NT] += sum;
+    }
+    __device__ void times_zero() {
+        for (int b = 0; b < slots(nb); ++b) at[b * NT] *= 0.f;
+    }
     // the lane's part of a bucket's sum over the workgroup, in a fixed order
     __device__ float part(int b) const {
         const float *from = at - threadIdx.x + (threadIdx.x & 63);
@@ -538,24 +547,48 @@ __device__ inline float look_up(float table, int bucket) {
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * bucket, __builtin_bit_cast(int, table)));
 }
 
+// Adds the bias to a lane's 16 products, `codes` their four words.  Far from each other pairs mostly share a bucket - rows
+// beyond the longest distance that has one of its own, nodes that no walk joins: where every lane of the wavefront has
+// one code for all its 16 pairs, one look-up does and the codes stay packed (64 walks of up to 1024 rows, 8 heads of 64
+// in bf16, 32 buckets by distance: 414 to 340 us).  Returns whether it was so.
+__device__ inline bool add_bias(float (&s)[16], const uint32_t (&codes)[4], float scale, float table, int nb) {
+    const uint32_t all = (codes[0] & 255u) * 0x01010101u;
+    const uint32_t differ = ((codes[0] ^ all) | (codes[1] ^ all)) | ((codes[2] ^ all) | (codes[3] ^ all));
+    if (__builtin_amdgcn_ballot_w64(differ != 0) == 0) {
+        const int b = code_of(all, 0, nb);
+        const float bias = look_up(table, b);
+        const bool on = b < nb;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = on ? fmaf(s[i], scale, bias) : -INFINITY;
+        return true;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int b = code_of(codes[i >> 2], i & 3, nb);
+        const float x = fmaf(s[i], scale, look_up(table, b));
+        s[i] = b < nb ? x : -INFINITY;
+    }
+    return false;
+}
+
 // How the backward pass has a row's probabilities again: exp2((score + start) c) * factor.  16-bit types without a bias
 // begin their products at a start that holds the logarithm of the factor too, and save the product.  With a bias that
 // would be lost beside a large reference - a row all of whose pairs carry a mask's -1e9 - and for fp32 the rounding of
 // the larger exponent would be the largest error of all: there the exponentials are the forward pass's, bit for bit.
-// start -infinity or factor 0 for a row without pairs and for rows that do not exist.
+// start -infinity for a row without pairs and for rows that do not exist.
 template <typename T, bool BIAS>
 struct RowWeight {
     static constexpr bool FOLDED = sizeof(T) == 2 && !BIAS;
     float start, factor;
     __device__ RowWeight(float ref, float inv, float c) {
-        start = FOLDED ? __log2f(inv) / c - ref : BIAS ? -ref : -(ref * c);
+        start = FOLDED ? __log2f(inv) / c - ref : inv == 0.f ? -INFINITY : -ref;
         factor = inv;
     }
     // what the product begins at, and the weight from what it ends at or, with a bias, from the score
     __device__ float begin() const { return FOLDED ? start : 0.f; }
     __device__ static float weight(float x, float start, float factor, float c) {
         if (FOLDED) return exp2_fast(x * c);
-        return exp2_fast(BIAS ? x + start : fmaf(x, c, start)) * factor;
+        return exp2_fast(BIAS ? x + start : (x + start) * c) * factor;
     }
     __device__ float of(float score, float c) const { return weight(score + begin(), start, factor, c); }
 };
@@ -803,17 +836,13 @@ attention_forward_kernel(const RwkAttnArgs p) {
             interleave<T, TN * KS>();
             if (BIAS) {
 #pragma unroll
-                for (int t = 0; t < TN; ++t)
+                for (int t = 0; t < TN; ++t) {
+                    uint32_t four[4];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const uint32_t four = Codes::read(codes + turn * 32 * NW * BN, q - at.first, 32 * t + 8 * g + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int b = code_of(four, e, nb);
-                            const float x = fmaf(s[t][4 * g + e], scale, look_up(table, b));
-                            s[t][4 * g + e] = b < nb ? x : -INFINITY;
-                        }
-                    }
+                    for (int g = 0; g < 4; ++g)
+                        four[g] = Codes::read(codes + turn * 32 * NW * BN, q - at.first, 32 * t + 8 * g + 4 * h);
+                    add_bias(s[t], four, scale, table, nb);
+                }
             }
             if (k0 + BN > n || (causal && k0 + BN - 1 > q0)) {
                 const int last = causal ? min(q, n - 1) : n - 1;
@@ -842,7 +871,10 @@ attention_forward_kernel(const RwkAttnArgs p) {
             for (int t = 0; t < TN; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[t][i] = exp2_fast(BIAS ? s[t][i] - base : fmaf(s[t][i], c, -base_c));
+                    // fp32: the difference first, which is exact near the maximum
+                    s[t][i] = exp2_fast(BIAS             ? s[t][i] - base
+                                        : sizeof(T) == 4 ? (s[t][i] - base) * c
+                                                         : fmaf(s[t][i], c, -base_c));
                     part += s[t][i];
                 }
             sum += part;
@@ -978,17 +1010,12 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) d[i] -= sizeof(T) == 2 ? 0.f : delta;
             uint32_t four[4];
+            bool alike = false;
             if (BIAS) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < 4; ++g)
                     four[g] = Codes::read(codes + turn * 32 * NW * BN, q - at.first, 32 * t + 8 * g + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int b = code_of(four[g], e, nb);
-                        const float x = fmaf(s[4 * g + e], scale, look_up(table, b));
-                        s[4 * g + e] = b < nb ? x : -INFINITY;
-                    }
-                }
+                alike = add_bias(s, four, scale, table, nb);
             }
             if (kt + 32 > n || (causal && kt + 31 > q0)) {
                 const int last = causal ? min(q, n - 1) : n - 1;
@@ -998,8 +1025,12 @@ attention_dq_kernel(const RwkAttnArgs p) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = weigh(weight.weight(s[i], weight.start, weight.factor, c), d[i]);
             if (BIAS && q < n) {
+                if (alike) {
+                    buckets.add_all(four[0], s);
+                } else {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) buckets.add(four[g], s + 4 * g);
+                    for (int g = 0; g < 4; ++g) buckets.add(four[g], s + 4 * g);
+                }
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) acc.add(k_tile, 32 * t + 16 * u, pack<T>(s, u), lane);
@@ -1009,9 +1040,13 @@ attention_dq_kernel(const RwkAttnArgs p) {
     }
     acc.finish();
     const bool again = q < n && not_finite<KS>(acc.a);
-    if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc.a, p.a.scale);
+    // A row's only pair has weight 1 whatever its score: no gradient, where d_out . v and delta, summed in different
+    // orders, differ by a rounding.  (Times 0: what is not a number stays.)
+    const float some = n == 1 || (causal && q == 0) ? 0.f : 1.f;
+    if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc.a, p.a.scale * some);
     if (any_lane(again)) exact_dq<T, BIAS>(p, at, table, q, end, weight, delta, c, again);
     if (BIAS) {
+        if (some == 0.f) buckets.times_zero();
         __syncthreads();
         for (int b = threadIdx.x >> 6; b < nb; b += NW) {                  // a wavefront per bucket
             const float v = rwk_wave_sum(buckets.part(b));
@@ -1142,17 +1177,11 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                 unpack(sx, s);
                 unpack(dx, d);
                 if (BIAS) {
+                    uint32_t four[4];
 #pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        const int r = 32 * t + 8 * g4 + 4 * h;
-                        const uint32_t four = Codes::read(codes + turn * 32 * NW * BQ, k - at.first, r);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int b = code_of(four, e, nb);
-                            const float x = fmaf(s[4 * g4 + e], scale, look_up(table, b));
-                            s[4 * g4 + e] = b < nb ? x : -INFINITY;
-                        }
-                    }
+                    for (int g4 = 0; g4 < 4; ++g4)
+                        four[g4] = Codes::read(codes + turn * 32 * NW * BQ, k - at.first, 32 * t + 8 * g4 + 4 * h);
+                    add_bias(s, four, scale, table, nb);
                 }
                 if (causal && qt < k0 + 31) {
 #pragma unroll
@@ -1179,11 +1208,12 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     dk.finish();
     dv.finish();
     const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a), again = k < n && (bad_k || bad_v);
+    const float by = n == 1 ? 0.f * p.a.scale : p.a.scale;        // as in dQ: a segment of one row has one pair
     if (k < n && !again && p.parts > 1) {
-        store_rows<false, float, DT>(out.dk + to, dim, h, dk.a, p.a.scale);
+        store_rows<false, float, DT>(out.dk + to, dim, h, dk.a, by);
         store_rows<false, float, DT>(out.dv + to, dim, h, dv.a, 1.f);
     } else if (k < n && !again) {
-        store_rows<false, T, DT>((T *)p.a.dk + out.at + to, dim, h, dk.a, p.a.scale);
+        store_rows<false, T, DT>((T *)p.a.dk + out.at + to, dim, h, dk.a, by);
         store_rows<false, T, DT>((T *)p.a.dv + out.at + to, dim, h, dv.a, 1.f);
     }
     if (any_lane(again)) exact_dkv<T, BIAS>(p, at, part, k, begin, c, again);

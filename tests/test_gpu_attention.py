@@ -462,6 +462,47 @@ def test_rows_gigabytes_apart(dev, dim, heads):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim,buckets", [(16, 4), (64, 4), (64, 32), (128, 9)])
+def test_blocks_of_pairs_with_one_code(dev, dtype, causal, dim, buckets):
+    """Codes that are alike over whole tiles: a far bucket, a mask over 64 columns (whose keys hold anything), one code
+    everywhere; different ones per row."""
+    lengths = [300, 77, 160]
+    q, k, v, do, bias, codes = make(dev, dtype, lengths, 4, 2, dim, seed=buckets, buckets=buckets)
+    i = torch.arange(300, device=dev)
+    far = (i[:, None] - i[None, :]).abs()
+    codes[0] = torch.where(far < 40, far % buckets, buckets - 1).to(torch.uint8)
+    codes[0][:, 192:256] = 255
+    codes[1].fill_(buckets - 2)
+    codes[2] = (i[:160] % buckets)[:, None].expand(160, 160).contiguous().to(torch.uint8)
+    want, err = truth(q, k, v, do, lengths, causal, bias=bias, codes=codes)
+    check(run(q, k, v, do, lengths, causal, bias=bias, codes=codes), want, err)
+    clean = run(q, k, v, do, lengths, causal, bias=bias, codes=codes)
+    k[200], v[201] = math.nan, math.inf
+    got = run(q, k, v, do, lengths, causal, bias=bias, codes=codes)
+    rows = torch.ones(537, dtype=torch.bool, device=dev)
+    rows[192:256] = False
+    for a, b in zip(got[1:], clean[1:]):
+        a, b = (t[rows] if t.shape[0] == 537 else t for t in (a, b))
+        assert torch.allclose(a.double(), b.double(), rtol=0.02, atol=0.02 * float(b.abs().max()))
+    check([got[0]], want[:1], err[:1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,buckets", [(53, 0), (53, 8), (16, 8), (128, 3)])
+def test_rows_of_one_pair_have_no_gradient(dev, dtype, dim, buckets):
+    """Segments of one row, and the first row under a causal mask: softmax of one score is 1 whatever the score."""
+    q, k, v, do, bias, codes = make(dev, dtype, [1] * 11, 6, 2, dim, buckets=buckets)
+    got = run(q, k, v, do, [1] * 11, False, bias=bias, codes=codes)
+    for t in got[1:3] + got[4:]:
+        assert not t.any()
+    assert torch.equal(got[0].view(11, 2, 3, dim), v[:, :, None].expand(11, 2, 3, dim))
+    q, k, v, do, bias, codes = make(dev, dtype, [40, 140], 6, 2, dim, buckets=buckets)
+    got = run(q, k, v, do, [40, 140], True, bias=bias, codes=codes)
+    assert not got[1][0].any() and not got[1][40].any() and got[1][1:40].any()
+
+
 def test_dense_and_relative_codes(dev):
     from gnn_amd import packed_segments, pair_buckets, relative_buckets
     lengths = [3, 0, 64, 131, 1]
