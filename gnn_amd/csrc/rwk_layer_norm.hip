@@ -9,6 +9,10 @@
 // fp32, one rounding to the element type at the store.
 #include "rwk_vec.h"
 
+// Every product and sum is rounded by itself, as the formula is written: the gradient of rows of two elements is what
+// is left of equal terms, and a fused step on one side only would be most of it.
+#pragma clang fp contract(off)
+
 namespace {
 
 constexpr int kBlock = 256;
@@ -118,12 +122,12 @@ norm_forward_kernel(const T *__restrict__ x, long long x_stride, const W *__rest
 #pragma unroll
         for (int i = 0; i < IT * V; ++i) {
             v[i] = (t + i / V * TPR) * V + i % V < width ? v[i] - mean : 0.f;
-            q = fmaf(v[i], v[i], q);
+            q += v[i] * v[i];
         }
         const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / (float)width + eps);
 #pragma unroll
         for (int i = 0; i < IT * V; ++i)
-            v[i] = bias != nullptr ? fmaf(v[i] * rstd, w.at(i), b.at(i)) : v[i] * rstd * w.at(i);
+            v[i] = bias != nullptr ? v[i] * rstd * w.at(i) + b.at(i) : v[i] * rstd * w.at(i);
         if (!there) continue;
         store_row<T, TPR, V, IT>(y + r * width, width, t, v);
         if (t == 0 && mean_out != nullptr) {
@@ -173,12 +177,12 @@ norm_backward_kernel(const T *__restrict__ x, long long x_stride, const T *__res
             h[i] = (xr.at(i) - mean) * rstd;              // beyond the row: dy = 0 and w = 0 take it out
             g[i] = gr.at(i);
             if (there) {
-                dw[i] = fmaf(g[i], h[i], dw[i]);
+                dw[i] += g[i] * h[i];
                 db[i] += g[i];
             }
             g[i] *= w.at(i);
             a += g[i];
-            c = fmaf(g[i], h[i], c);
+            c += g[i] * h[i];
         }
         row_sums<TPR>(a, c, red[turn]);
         a *= inv;
@@ -227,12 +231,11 @@ norm_forward_wide_kernel(const T *__restrict__ x, long long x_stride, const W *_
     float q = 0.f;
     for (int c = threadIdx.x; c < width; c += kBlock) {
         const float d = (float)row[c] - mean;
-        q = fmaf(d, d, q);
+        q += d * d;
     }
     const float rstd = 1.f / sqrtf(row_sum<kBlock>(q, red[1]) / (float)width + eps);
     for (int c = threadIdx.x; c < width; c += kBlock)
-        y[r * width + c] = (T)fmaf(((float)row[c] - mean) * rstd, (float)weight[c],
-                                   bias != nullptr ? (float)bias[c] : 0.f);
+        y[r * width + c] = (T)(((float)row[c] - mean) * rstd * (float)weight[c] + (bias != nullptr ? (float)bias[c] : 0.f));
     if (threadIdx.x == 0 && mean_out != nullptr) {
         mean_out[r] = mean;
         rstd_out[r] = rstd;
@@ -252,7 +255,7 @@ norm_backward_wide_kernel(const T *__restrict__ x, long long x_stride, const T *
     for (int i = threadIdx.x; i < width; i += kBlock) {
         const float t = (float)grad[i] * (float)weight[i];
         a += t;
-        c = fmaf(t, ((float)row[i] - mean) * rstd, c);
+        c += t * (((float)row[i] - mean) * rstd);
     }
     a = row_sum<kBlock>(a, red[0]) / (float)width;
     c = row_sum<kBlock>(c, red[1]) / (float)width;
@@ -271,7 +274,7 @@ norm_weight_wide_kernel(const T *__restrict__ x, long long x_stride, const T *__
     float dw = 0.f, db = 0.f;
     for (long long r = blockIdx.y; r < rows; r += gridDim.y) {
         const float g = (float)dy[r * dy_stride + c];
-        dw = fmaf(g, ((float)x[r * x_stride + c] - mean_in[r]) * rstd_in[r], dw);
+        dw += g * (((float)x[r * x_stride + c] - mean_in[r]) * rstd_in[r]);
         db += g;
     }
     float *out = partials + (long long)blockIdx.y * 2 * width;

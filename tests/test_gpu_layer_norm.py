@@ -242,3 +242,20 @@ def test_one_derivative(dev):
     assert all(torch.equal(p, a) and torch.equal(p, g) for p, a, g in zip(plain, again, graph))
     with pytest.raises(RuntimeError, match="once"):
         graph[0].sum().backward()
+
+
+def test_rows_of_two_elements(dev):
+    """What is left of equal terms: the same numbers as the formula's steps in fp32, each rounded by itself."""
+    from gnn_amd import layer_norm
+    x, w, b, dy = make(dev, 200, 2, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    dx = torch.autograd.grad(y, leaves, dy)[0]
+    with torch.no_grad():
+        centred = x - (x[:, :1] + x[:, 1:]) / 2
+        square = centred * centred
+        rstd = 1.0 / torch.sqrt((square[:, :1] + square[:, 1:]) / 2 + 1e-5)
+        hat, t = centred * rstd, dy * w
+        th = t * hat
+        want = rstd * (t - (t[:, :1] + t[:, 1:]) / 2 - hat * ((th[:, :1] + th[:, 1:]) / 2))
+        assert torch.equal(y, hat * w + b) and torch.equal(dx, want)
