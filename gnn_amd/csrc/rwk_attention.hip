@@ -144,39 +144,48 @@ __device__ inline CodeBlock code_block(const int *items, const int *seg_ptr, con
     return b;
 }
 
+// four codes of a row of n at j, 255 from n on
+__device__ inline uint32_t four_codes(const uint8_t *row, int j, int n) {
+    uint32_t v = 0xFFFFFFFFu;
+    if (j + 4 <= n) {
+        __builtin_memcpy(&v, row + j, 4);
+    } else {
+        for (int e = 0; e < 4; ++e)
+            if (j + e < n) v = (v & ~(255u << (8 * e))) | ((uint32_t)row[j + e] << (8 * e));
+    }
+    return v;
+}
+
 // Rows of n bytes at any address to rows of a multiple of 32, four bytes a lane, a wavefront per row; and, by 64 x 64
-// tiles through LDS, to the same with a row per key.
+// tiles through LDS, to the same with a row per key.  kDenseSplit workgroups share a block of rows.
+constexpr int kDenseSplit = 8;
 __global__ void __launch_bounds__(kBlock)
 pair_dense_kernel(const uint8_t *__restrict__ dense, const int64_t *__restrict__ pair_start,
                   const int *__restrict__ seg_ptr, const int64_t *__restrict__ code_start,
                   const int *__restrict__ items, int block_rows, uint8_t *__restrict__ codes,
                   uint8_t *__restrict__ codes_by_key) {
-    __shared__ uint8_t tile[64][68];
+    __shared__ __attribute__((aligned(4))) uint8_t tile[64][68];
     const CodeBlock b = code_block(items, seg_ptr, code_start, block_rows);
     const uint8_t *in = dense + pair_start[b.g];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = wave; r < b.rows; r += kBlock / 64) {
-        const uint8_t *row = in + (long long)(b.first + r) * b.n;
-        for (int j = 4 * lane; j < b.padded; j += 256) {
-            uint32_t v = 0xFFFFFFFFu;
-            if (j + 4 <= b.n) {
-                __builtin_memcpy(&v, row + j, 4);
-            } else {
-                for (int e = 0; e < 4; ++e)
-                    if (j + e < b.n) v = (v & ~(255u << (8 * e))) | ((uint32_t)row[j + e] << (8 * e));
-            }
-            *(uint32_t *)(codes + b.start + (long long)(b.first + r) * b.padded + j) = v;
-        }
-    }
+    const int lane = threadIdx.x & 63, share = blockIdx.y;
+    for (int r = (threadIdx.x >> 6) + share * (kBlock / 64); r < b.rows; r += kDenseSplit * (kBlock / 64))
+        for (int j = 4 * lane; j < b.padded; j += 256)
+            *(uint32_t *)(codes + b.start + (long long)(b.first + r) * b.padded + j) =
+                four_codes(in + (long long)(b.first + r) * b.n, j, b.n);
+    const int i = threadIdx.x >> 4, four = 4 * (threadIdx.x & 15);       // row of sixteen, first of four columns
     for (int k0 = b.first; k0 < b.first + b.rows; k0 += 64)
-        for (int q0 = 0; q0 < b.padded; q0 += 64) {
+        for (int q0 = 64 * share; q0 < b.padded; q0 += 64 * kDenseSplit) {
             __syncthreads();
-            for (int i = wave; i < 64; i += kBlock / 64)
-                tile[i][lane] = q0 + i < b.n && k0 + lane < b.n ? in[(long long)(q0 + i) * b.n + k0 + lane] : 255;
+            for (int r = i; r < 64; r += 16)
+                *(uint32_t *)&tile[r][four] = q0 + r < b.n ? four_codes(in + (long long)(q0 + r) * b.n, k0 + four, b.n)
+                                                           : 0xFFFFFFFFu;
             __syncthreads();
-            for (int i = wave; i < 64; i += kBlock / 64)
-                if (k0 + i < b.first + b.rows && q0 + lane < b.padded)
-                    codes_by_key[b.start + (long long)(k0 + i) * b.padded + q0 + lane] = tile[lane][i];
+            for (int k = i; k < 64; k += 16)
+                if (k0 + k < b.first + b.rows && q0 + four < b.padded) {
+                    uint32_t v = 0;
+                    for (int e = 0; e < 4; ++e) v |= (uint32_t)tile[four + e][k] << (8 * e);
+                    *(uint32_t *)(codes_by_key + b.start + (long long)(k0 + k) * b.padded + q0 + four) = v;
+                }
         }
 }
 
@@ -268,7 +277,7 @@ int rwk_pair_buckets_dense(const uint8_t *dense, const int64_t *pair_start, cons
     if (code != RWK_OK || n_items == 0) return code;
     RWK_REQUIRE_PTR(dense);
     RWK_REQUIRE_PTR(pair_start);
-    hipLaunchKernelGGL(pair_dense_kernel, dim3((unsigned)n_items), dim3(kBlock), 0, (hipStream_t)stream, dense,
+    hipLaunchKernelGGL(pair_dense_kernel, dim3((unsigned)n_items, kDenseSplit), dim3(kBlock), 0, (hipStream_t)stream, dense,
                        pair_start, seg_ptr, code_start, items, block_rows, codes, codes_by_key);
     RWK_LAUNCH_CHECK();
     return RWK_OK;

@@ -8,18 +8,27 @@
 //   dk_j = scale sum_i ds_ij q_i,  d_table[h][b] = sum over pairs with code b of ds_ij
 //
 // One pass over the keys with the running maximum and sum of the softmax; scores never leave the registers.  All
-// products are 32x32 matrix instructions (16-bit types: 16 products deep, fp32: 2 deep, eight in a row), all sums,
-// maxima and exponentials fp32.  A wavefront owns 32 rows and computes scores TRANSPOSED to what it owns as columns:
-// lane l holds row (or key) l % 32 of its own and 16 of the other index, which is the operand layout of the next
-// product up to a permutation of the summed index, so probabilities go from one product to the next without leaving
-// their lane.  They are rounded to the element type there (the matrix instructions take nothing wider); the sums l_i,
-// delta and d_table use the unrounded fp32 values.
+// products are 32x32 matrix instructions (16-bit types: 16 products deep, fp32: 2 deep, eight in a row; fp32 heads of
+// up to 16 elements have 16x16 second products), all sums, maxima and exponentials fp32.  A wavefront owns 32 rows and
+// computes scores TRANSPOSED to what it owns as columns: lane l holds row (or key) l % 32 of its own and 16 of the other
+// index, which is the operand layout of the next product up to a permutation of the summed index, so probabilities go
+// from one product to the next without leaving their lane.  They are rounded to the element type there (the matrix
+// instructions take nothing wider; the forward pass keeps what that leaves over where it counts most, see FINE); the
+// sums l_i, delta and d_table use the unrounded fp32 values.  16-bit outputs leave what their own rounding left over
+// (out_low) for delta, whose error all of a row's ds share.
+//
+// The forward pass needs 2 products of a pair's rows, dQ 3 and dK/dV 4, and between them per pair an exponential (the
+// time of four other instructions) and four to eight more.  At 128 elements of 16 bits the matrix unit bounds all three,
+// at 64 the vector unit does; fp32 matrix instructions stop the vector unit, so there the two times add up.  4 prompts
+// of up to 8192 rows, 32 heads of 128 in bf16 over 8 of keys, causal: 917 us forward (0.81 of a large product's rate),
+// 1236 dQ (0.90), 2036 + 60 dK/dV (0.71); 48 of up to 1500, 16 heads of 64 in fp16 over 4: 146, 229, 245 us; 1024 graphs
+// of 100 to 500 nodes, 4 heads of 16 in fp32, a bias of 8 buckets: 481, 756, 787 us.
 //
 // Summed index of the second product: slot e of lane half h (h = lane / 32) of step s is row 16 s + 4 h + e for
 // e < 4 and 16 s + 8 + 4 h + (e - 4) otherwise, the registers 8 s + e of a 32x32 result.
 //
 // Tiles of the other operand lie in LDS row by row, the 16-byte chunks of a row permuted by the row's number
-// (chunk ^ row) so that both kinds of reads - eight consecutive elements of a row per lane, and columns of four rows -
+// (swizzle()) so that both kinds of reads - eight consecutive elements of a row per lane, and columns of four rows -
 // spread over the banks.
 #pragma once
 
@@ -550,7 +559,7 @@ __device__ inline float look_up(float table, int bucket) {
 // Adds the bias to a lane's 16 products, `codes` their four words.  Far from each other pairs mostly share a bucket - rows
 // beyond the longest distance that has one of its own, nodes that no walk joins: where every lane of the wavefront has
 // one code for all its 16 pairs, one look-up does and the codes stay packed (64 walks of up to 1024 rows, 8 heads of 64
-// in bf16, 32 buckets by distance: 414 to 340 us).  Returns whether it was so.
+// in bf16, 32 buckets by distance: 418 to 380 us).  Returns whether it was so.
 __device__ inline bool add_bias(float (&s)[16], const uint32_t (&codes)[4], float scale, float table, int nb) {
     const uint32_t all = (codes[0] & 255u) * 0x01010101u;
     const uint32_t differ = ((codes[0] ^ all) | (codes[1] ^ all)) | ((codes[2] ^ all) | (codes[3] ^ all));
