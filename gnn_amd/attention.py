@@ -66,10 +66,13 @@ class PackedSegments:
         self._key_work = [(int(w.max(initial=0)), int(w.sum()) / 512) for w in (n, n - first)]
         packed = torch.from_numpy(np.ascontiguousarray(np.concatenate(
             [starts] + [x.reshape(-1) for x in lists]), dtype=np.int32)).to(device)
-        self._arrays = packed
+        self._arrays, self._stream = packed, _lib.current_stream(device)
         at = packed.data_ptr()
         self._seg_ptr = at
         self._items, self._q_causal, self._k_causal = (at + 4 * (starts.size + 2 * i * self.n_items) for i in range(3))
+
+    def __reduce__(self):                                 # a copy has lists of its own
+        return PackedSegments, (self.lengths, self.device)
 
     def key_parts(self, heads: int, kv_heads: int, causal: bool) -> int:
         """Workgroups that share a block of keys in the backward pass, each with its part of the query heads.  Whole,
@@ -134,6 +137,7 @@ class PairBuckets:
         self._start = torch.from_numpy(np.concatenate([[0], np.cumsum(sizes)])).to(segments.device)
         self._codes = torch.empty(int(sizes.sum()), dtype=torch.uint8, device=segments.device)
         self._by_key = self._codes if symmetric else torch.empty_like(self._codes)
+        self._stream = _lib.current_stream(segments.device)
 
     def dense(self, segment: int) -> torch.Tensor:
         """Codes of one segment, (n, n): query row, key row."""
@@ -211,6 +215,16 @@ def hop_buckets(adj: torch.Tensor, graph_indicator: torch.Tensor, max_distance: 
                  st.max_distance + 1 if far == "bucket" else 255, symmetric=True)
 
 
+def _used_here(segments: PackedSegments, buckets, stream: int):
+    """Lists and codes that were made on another stream: their memory is not handed out again before this stream's
+    work on them is done."""
+    if segments._stream != stream:
+        segments._arrays.record_stream(torch.cuda.current_stream(segments.device))
+    if buckets is not None and buckets._stream != stream:
+        for t in (buckets._codes, buckets._by_key, buckets._start):
+            t.record_stream(torch.cuda.current_stream(segments.device))
+
+
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """The elements of a head have to be adjacent; rows and heads may lie anywhere."""
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
@@ -250,9 +264,10 @@ def _forward(q, k, v, segments, causal, scale, table, buckets, stats):
             low = torch.empty_like(out)
             a.out_low = low.data_ptr()
     dev = segments.device
+    stream = _lib.current_stream(dev)
+    _used_here(segments, buckets, stream)
     with _lib.device_guard(dev):
-        _lib.check(_lib.load().rwk_attention_forward(ctypes.addressof(a), _lib.current_stream(dev)),
-                   "rwk_attention_forward")
+        _lib.check(_lib.load().rwk_attention_forward(ctypes.addressof(a), stream), "rwk_attention_forward")
     return out, st, low
 
 
@@ -294,9 +309,10 @@ class _PackedAttention(torch.autograd.Function):
             d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
             partials = torch.empty(table.numel() * segments.n_items, dtype=torch.float32, device=dev)
             a.d_table, a.d_table_partials = d_table.data_ptr(), partials.data_ptr()
+        stream = _lib.current_stream(dev)
+        _used_here(segments, buckets, stream)
         with _lib.device_guard(dev):
-            _lib.check(_lib.load().rwk_attention_backward(ctypes.addressof(a), _lib.current_stream(dev)),
-                       "rwk_attention_backward")
+            _lib.check(_lib.load().rwk_attention_backward(ctypes.addressof(a), stream), "rwk_attention_backward")
         return dq, dk, dv, d_table, None, None, None, None
 
 

@@ -503,6 +503,33 @@ def test_rows_of_one_pair_have_no_gradient(dev, dtype, dim, buckets):
     assert not got[1][0].any() and not got[1][40].any() and got[1][1:40].any()
 
 
+def test_lists_that_outlive_or_leave_their_stream(dev):
+    """Deep copies have memory of their own; lists made on one stream, used on another and dropped at once."""
+    import copy
+    from gnn_amd import packed_attention, packed_segments, relative_buckets
+    q, k, v, do, bias, _ = make(dev, torch.float32, [300, 5, 90], 4, 2, 16, buckets=8)
+    bias.requires_grad_()
+
+    def once(buckets):
+        out = packed_attention(q, k, v, buckets.segments, bias=bias, buckets=buckets)
+        return [out, *torch.autograd.grad(out, [bias], do)]
+    made = relative_buckets(packed_segments([300, 5, 90], dev), 8, 100)
+    want = once(made)
+    twin = copy.deepcopy(made)
+    assert twin.segments is not made.segments and twin.segments._seg_ptr != made.segments._seg_ptr
+    del made
+    torch.zeros(1 << 20, dtype=torch.int32, device=dev)
+    assert all(torch.equal(a, b) for a, b in zip(once(twin), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = once(twin)
+    del twin
+    junk = [torch.zeros(1 << n, dtype=torch.int32, device=dev) for n in range(4, 20)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and junk
+
+
 def test_dense_and_relative_codes(dev):
     from gnn_amd import packed_segments, pair_buckets, relative_buckets
     lengths = [3, 0, 64, 131, 1]
