@@ -7,8 +7,8 @@ the weights are learned: ``softmax_j(scale * q_i . k_j + bias[h, bucket_ij]) v_j
 trainable number per head and bucket of the pair - its hop distance (:func:`hop_buckets`), the rows' distance in a walk
 (:func:`relative_buckets`) or any other code (:func:`pair_buckets`).
 
-One launch forward and two backward (``csrc/rwk_attention_body.h``; one more for the bias gradient); scores never reach
-memory and all sums run in a fixed order, so results are bitwise reproducible.  HIP devices only.
+One launch forward and two backward (``csrc/rwk_attention_body.h``; one more for the bias gradient, and one where the
+query heads of long blocks of keys are shared out); scores never reach memory and all sums run in a fixed order, so results are bitwise reproducible.  HIP devices only.
 """
 from __future__ import annotations
 
@@ -328,7 +328,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
 
     Returns (N, H, D), contiguous.  A row that attends to nothing gives zeros.  Differentiable once with respect to
     q, k, v and bias.  Sums, softmax statistics and the bias gradient are fp32; for the 16-bit types probabilities are
-    rounded to the type before they meet ``v``.  What a pair's rows hold counts for nothing where the pair does not
+    rounded to the type before they meet ``v`` (to two numbers of it for heads of up to 32 elements and in batches whose
+    longest segment has at most 256 rows).  What a pair's rows hold counts for nothing where the pair does not
     attend, values that are not finite included (blocks of rows whose result is not finite take much longer)."""
     if not q.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
