@@ -8,7 +8,8 @@ trainable number per head and bucket of the pair - its hop distance (:func:`hop_
 (:func:`relative_buckets`) or any other code (:func:`pair_buckets`).
 
 One launch forward and two backward (``csrc/rwk_attention_body.h``; one more for the bias gradient, and one where the
-query heads of long blocks of keys are shared out); scores never reach memory and all sums run in a fixed order, so results are bitwise reproducible.  HIP devices only.
+query heads of long blocks of keys are shared out); scores never reach memory and all sums run in a fixed order, so
+results are bitwise reproducible.  HIP devices only.
 """
 from __future__ import annotations
 
