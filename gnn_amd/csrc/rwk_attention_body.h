@@ -13,8 +13,8 @@
 // computes scores TRANSPOSED to what it owns as columns: lane l holds row (or key) l % 32 of its own and 16 of the other
 // index, which is the operand layout of the next product up to a permutation of the summed index, so probabilities go
 // from one product to the next without leaving their lane.  They are rounded to the element type there (the matrix
-// instructions take nothing wider; the forward pass keeps what that leaves over where it counts most, see FINE); the
-// sums l_i, delta and d_table use the unrounded fp32 values.  16-bit outputs leave what their own rounding left over
+// instructions take nothing wider; the forward pass and narrow heads' dQ keep what that leaves over where it counts most,
+// see FINE); the sums l_i, delta and d_table use the unrounded fp32 values.  16-bit outputs leave what their own rounding left over
 // (out_low) for delta, whose error all of a row's ds share.
 //
 // The forward pass needs 2 products of a pair's rows, dQ 3 and dK/dV 4, and between them per pair an exponential (the
@@ -67,6 +67,15 @@ __device__ inline Frag<T> pack(const float (&x)[16], int s) {
     Frag<T> f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f.v[e] = (T)x[8 * s + e];
+    return f;
+}
+
+// what pack's rounding left over
+template <typename T>
+__device__ inline Frag<T> left_over(const float (&x)[16], const Frag<T> &packed, int s) {
+    Frag<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = (T)(x[8 * s + e] - (float)packed.v[e]);
     return f;
 }
 
@@ -892,16 +901,10 @@ attention_forward_kernel(const RwkAttnArgs p) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const Frag<T> f = pack<T>(s[t], u);
-                    if constexpr (sizeof(T) == 2) {
-                        if (FINE) {
-                            Frag<T> rest;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) rest.v[e] = (T)(s[t][8 * u + e] - (float)f.v[e]);
-                            acc.add(v_tile, 32 * t + 16 * u, f, rest, lane);
-                            continue;
-                        }
-                    }
-                    acc.add(v_tile, 32 * t + 16 * u, f, lane);
+                    if constexpr (sizeof(T) == 2 && FINE)
+                        acc.add(v_tile, 32 * t + 16 * u, f, left_over<T>(s[t], f, u), lane);
+                    else
+                        acc.add(v_tile, 32 * t + 16 * u, f, lane);
                 }
         }
         keys.commit(next);
@@ -1042,7 +1045,13 @@ attention_dq_kernel(const RwkAttnArgs p) {
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) acc.add(k_tile, 32 * t + 16 * u, pack<T>(s, u), lane);
+            for (int u = 0; u < 2; ++u) {
+                const Frag<T> f = pack<T>(s, u);
+                // narrow heads: keys that a row weighs lie in its query's direction, and what they have in common drops
+                // out of the gradient (ds adds up to 0) but not out of its roundings
+                if constexpr (sizeof(T) == 2 && KS <= 2) acc.add(k_tile, 32 * t + 16 * u, f, left_over<T>(s, f, u), lane);
+                else acc.add(k_tile, 32 * t + 16 * u, f, lane);
+            }
         }
         keys.commit(next);
         values.commit(next + BN * S::W);
