@@ -258,6 +258,7 @@ adamw_kernel(const rwk_adamw_chunk *__restrict__ chunks, int tensor_base, AdamwG
         update<T, STATE8, kPerWave, true>(p, g, chunk, step, lr_ptr, hyper);
     else
         update<T, STATE8, kPerWave, false>(p, g, chunk, step, lr_ptr, hyper);
+    __syncthreads();                              // every wavefront has read the count
     if (threadIdx.x == 0) chunk_steps[blockIdx.x] = step;
 }
 

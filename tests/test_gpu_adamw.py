@@ -334,3 +334,23 @@ def test_a_refused_step_changes_nothing(dev):
     with pytest.raises(RuntimeError, match="sparse"):
         opt.step()
     assert torch.equal(a, before) and int(opt.state_dict()["state"][0]["step"]) == 1
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_all_of_a_chunk_takes_one_step_count(dev, bits):
+    """Elements that are alike stay alike, in every chunk of more than fit the device at once and in every quarter of
+    one: no wavefront takes the count that another has advanced.  (With 8-bit states the same element of each tensor has
+    bits of its own, so a twin with the same seed is compared instead.)"""
+    from gnn_amd import AdamW
+    n = 6 << 20
+    params = [torch.nn.Parameter(torch.full((n,), 0.5, device=dev)) for _ in range(2)]
+    opts = [AdamW([p], **HYPER, state_bits=bits, seed=3) for p in params]
+    for t in range(40):
+        for p, o in zip(params, opts):
+            p.grad = torch.full((n,), (-0.9) ** t, device=dev)
+            o.step()
+    assert torch.equal(*params)
+    if bits == 32:
+        assert (params[0] == params[0][0]).all()
+    counts = opts[0]._tables[0].steps
+    assert counts.numel() == n // 4096 and (counts == 40).all()
