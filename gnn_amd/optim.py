@@ -8,6 +8,9 @@ device, so the update can be captured in a HIP graph and a scheduler can change 
 """
 from __future__ import annotations
 
+from itertools import chain
+from operator import is_
+
 import numpy as np
 import torch
 
@@ -315,6 +318,40 @@ class StepTail:
         self.done = True
 
 
+# looks at a tensor that map() takes at the interpreter's own speed: a step has one for every tensor it holds
+_address, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_size, _version = torch.Tensor.numel, torch.Tensor._version.__get__
+
+
+class _Snapshot:
+    """What the tables of an optimiser were made from.  A caller may replace or clear any of it - parameters, states,
+    groups - and the addresses in the tables would be those of memory given back.  Holds what launches write."""
+
+    def __init__(self, opt: "AdamW"):
+        self.groups = list(opt.param_groups)
+        self.params = [p for g in self.groups for p in g["params"]]
+        self.keys, self.states = list(opt.state.keys()), list(opt.state.values())
+        own = [opt.state[p] for p in self.params]
+        self.values = [st.values() for st in own]                 # these follow their states
+        self.tensors = list(chain.from_iterable(self.values))
+        self.steps = [st["step"] for st in own]
+        self.written = self.params + [t for st in own for n, t in st.items() if n.startswith("exp_avg")]
+        self.matrices = [p for p in self.params if p.dim() > 1]   # others of the same size and address lie the same way
+        self.seen = self._seen()
+
+    def _seen(self):
+        """What may change in a tensor that stays the same object.  (A step count changes by what a caller does to it:
+        the device counts by itself.)"""
+        return list(map(_address, self.written)), list(map(_size, self.params)), list(map(_version, self.steps))
+
+    def stands(self, opt: "AdamW"):
+        params = list(chain.from_iterable([g["params"] for g in opt.param_groups]))
+        pairs = ((opt.param_groups, self.groups), (params, self.params), (opt.state.keys(), self.keys),
+                 (opt.state.values(), self.states), (list(chain.from_iterable(self.values)), self.tensors))
+        return (all([len(now) == len(then) and all(map(is_, now, then)) for now, then in pairs])
+                and self._seen() == self.seen and all(map(_contiguous, self.matrices)))
+
+
 class _AdamWTable:
     """Device tables of one launch shape: the parameters of one group with one type on one device."""
 
@@ -339,7 +376,9 @@ class _AdamWTable:
         self.chunks, self.steps = packed.split([chunks.size, len(chunks)])             # one copy to the device
         self.lr = torch.tensor([float(group["lr"])], dtype=torch.float64, device=self.device)
         self.lr_on_device = float(group["lr"])
-        self.pointers = [p.data_ptr() for p in params]
+        self.states = [opt.state[p] for p in params]
+        self.counts = [(st["step"], st["step"]._version) for st in self.states]
+        self.sizes = [p.numel() for p in params]
 
     def push_lr(self):
         lr = float(self.group["lr"])
@@ -355,13 +394,15 @@ class _AdamWTable:
         """Addresses of the gradients, checked; keeps what they belong to, for the launches read it asynchronously."""
         keep, grads = [], []
         dtype, device, strided = self.dtype, self.device, torch.strided
-        for p in self.params:
+        for p, size in zip(self.params, self.sizes):
             g = p.grad
             if g is not None:
                 if g.layout is not strided:
                     raise RuntimeError("gnn_amd.AdamW does not take sparse gradients")
                 if g.dtype is not dtype or g.device != device:
                     raise TypeError("a gradient must have its parameter's type and device")
+                if g.numel() != size:
+                    raise ValueError("a gradient must have its parameter's shape")
                 if not g.is_contiguous():
                     g = g.contiguous()
                 keep.append(g)
@@ -390,9 +431,12 @@ class _AdamWTable:
 
     def read_steps(self, opt: "AdamW"):
         steps = self.steps.tolist()
-        for p, lo, hi in zip(self.params, self.first_chunk, self.first_chunk[1:]):
-            if hi > lo:                                   # a tensor without elements has no chunk to count in
-                opt.state[p]["step"] = torch.tensor(float(steps[lo]), dtype=torch.float32)
+        for i, (p, lo, hi) in enumerate(zip(self.params, self.first_chunk, self.first_chunk[1:])):
+            st, (count, version) = self.states[i], self.counts[i]
+            # a tensor without elements has no chunk to count in; a count that a caller replaced is the caller's
+            if hi > lo and opt.state.get(p) is st and st.get("step") is count and count._version == version:
+                st["step"] = count = torch.tensor(float(steps[lo]), dtype=torch.float32)
+                self.counts[i] = count, count._version
 
 
 class AdamW(torch.optim.Optimizer):
@@ -419,7 +463,7 @@ class AdamW(torch.optim.Optimizer):
         if not 0 <= int(seed) < 2 ** 64:
             raise ValueError("seed must be in 0 .. 2^64 - 1")
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._tables = None
+        self._tables = self._made_from = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group):
@@ -460,12 +504,47 @@ class AdamW(torch.optim.Optimizer):
                 st[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
         return st
 
-    def _drop_tables(self):
-        """The tables describe other tensors from here on: their step counts move to the state."""
+    def _check_state(self, p):
+        """The parameter's state as the kernels can use it: made anew if it was cleared, refused if it does not fit."""
+        st = self.state.get(p)
+        if not st:
+            st = self.state[p] = self._new_state(p)
+        if not isinstance(st.get("step"), torch.Tensor):
+            st["step"] = torch.tensor(float(st.get("step", 0)), dtype=torch.float32)
+        n, device = p.numel(), p.device
+        blocks = (n + 255) // 256
+        for name in ("exp_avg", "exp_avg_sq"):
+            wanted = [(name, p.shape, torch.float32)]
+            if self.state_bits == 8:
+                wanted = [(name, p.shape, torch.float8_e4m3fn), (name + "_scale", (blocks,), torch.float32)]
+            for key, shape, dtype in wanted:
+                t = st.get(key)
+                if t is None:
+                    raise ValueError(f"the state of a parameter has no {key}")
+                if t.device != device:
+                    raise RuntimeError("a parameter or its state moved to another device after the optimiser was built")
+                if t.dtype != dtype or t.shape != shape:
+                    raise ValueError(f"{key} is {t.dtype} of shape {tuple(t.shape)} for a parameter of shape "
+                                     f"{tuple(p.shape)}, not {dtype} of shape {tuple(shape)}")
+                room = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+                if key == name and self.state_bits == 8 and (t.data_ptr() % 4 or room < 256 * blocks or not t.is_contiguous()):
+                    st[key] = self._new_state(p)[key].copy_(t)       # the kernel reads and writes whole blocks
+                elif not t.is_contiguous():
+                    st[key] = t.contiguous()
+
+    def _read_steps(self):
+        """The step counts live on the device; the states get them when somebody looks."""
         if self._tables is not None:
+            stood = self._made_from.stands(self)
             for t in self._tables:
                 t.read_steps(self)
-        self._tables = None
+            if stood:
+                self._made_from = _Snapshot(self)         # with the counts just written
+
+    def _drop_tables(self):
+        """The tables describe other tensors from here on: their step counts move to the state."""
+        self._read_steps()
+        self._tables = self._made_from = None
 
     def _build_tables(self):
         if torch.cuda.is_current_stream_capturing():
@@ -478,8 +557,7 @@ class AdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 if not p.is_cuda or p.layout != torch.strided or not p.is_contiguous():
                     raise ValueError("gnn_amd.AdamW takes contiguous parameters on HIP devices")
-                if any(s.device != p.device for k, s in self.state[p].items() if k != "step"):
-                    raise RuntimeError("a parameter moved to another device after the optimiser was built")
+                self._check_state(p)
                 kinds.setdefault((p.dtype, p.device), ([], []))
                 kinds[p.dtype, p.device][0].append(p)
                 kinds[p.dtype, p.device][1].append(pid)
@@ -487,7 +565,7 @@ class AdamW(torch.optim.Optimizer):
             for params, ids in kinds.values():
                 with _lib.device_guard(params[0].device):
                     tables.append(_AdamWTable(self, group, params, ids))
-        self._tables = tables
+        self._tables, self._made_from = tables, _Snapshot(self)
 
     def push_lr(self):
         """Hand changed learning rates to the device (``step`` does it by itself; replays of a captured step do not)."""
@@ -500,7 +578,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._tables is None or any([p.data_ptr() for p in t.params] != t.pointers for t in self._tables):
+        if self._tables is None or not self._made_from.stands(self):
             self._build_tables()
         lib = _lib.load()
         grads = [t.gather() for t in self._tables]        # all are checked before anything changes
@@ -509,17 +587,15 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def __getstate__(self):                               # copy.deepcopy, pickle: tables are built anew
-        for t in self._tables or ():
-            t.read_steps(self)
+        self._read_steps()
         return super().__getstate__() | {"state_bits": self.state_bits, "seed": self.seed}
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._tables = None
+        self._tables = self._made_from = None
 
     def state_dict(self):
-        for t in self._tables or ():                      # the step counts live on the device
-            t.read_steps(self)
+        self._read_steps()
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
@@ -545,6 +621,6 @@ class AdamW(torch.optim.Optimizer):
                 st["step"] = torch.tensor(float(src["step"]), dtype=torch.float32)
             new[p] = st
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        self._tables = None
+        self._tables = self._made_from = None
         for p, st in new.items():
             self.state[p] = st

@@ -354,3 +354,111 @@ def test_all_of_a_chunk_takes_one_step_count(dev, bits):
         assert (params[0] == params[0][0]).all()
     counts = opts[0]._tables[0].steps
     assert counts.numel() == n // 4096 and (counts == 40).all()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_that_a_caller_clears_or_replaces(dev, bits):
+    """Cleared states begin anew, replaced ones are taken, and what was replaced is not written any more."""
+    from collections import defaultdict
+    from gnn_amd import AdamW
+    for reset in ("clear", "replace", "assign", "count"):
+        params, grads = make(dev, torch.float32, [700, 5000], seed=8)
+        opt = AdamW(params, **HYPER, state_bits=bits, seed=4)
+
+        def go(o, ps, gs):
+            for p, g in zip(ps, gs):
+                p.grad = g.clone()
+            o.step()
+        go(opt, params, grads[0])
+        go(opt, params, grads[1])
+        old = [dict(opt.state[p]) for p in params]
+        before = [{n: t.clone() for n, t in st.items()} for st in old]
+        fresh = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        other = AdamW(fresh, **HYPER, state_bits=bits, seed=4)
+        if reset == "clear":
+            opt.state.clear()
+        elif reset == "assign":
+            opt.state = defaultdict(dict)
+        else:
+            saved = copy.deepcopy(opt.state_dict())
+            for p, s in zip(params, saved["state"].values()):
+                if reset == "replace":                   # as after keeping them elsewhere for a while
+                    for name, t in opt.state[p].items():
+                        if name != "step":
+                            opt.state[p][name] = t.cpu().to(dev)
+                else:
+                    opt.state[p]["step"] = torch.tensor(7.0)
+                    s["step"] = torch.tensor(7.0)
+            other.load_state_dict(saved)
+        for gs in grads[2:]:
+            go(opt, params, gs)
+            go(other, fresh, gs)
+        assert all(torch.equal(a, b) for a, b in zip(params, fresh)), reset
+        a, b = (o.state_dict()["state"] for o in (opt, other))
+        assert [float(s["step"]) for s in a.values()] == [float(s["step"]) for s in b.values()], reset
+        if reset != "count":
+            for was, now in zip(before, old):
+                for name in was:
+                    if name != "step":
+                        assert torch.equal(was[name].view(torch.uint8), now[name].view(torch.uint8)), (reset, name)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_and_states_that_no_longer_fit(dev, bits):
+    """Same address, other elements: refused, with the step counts as they were."""
+    from gnn_amd import AdamW
+
+    def moved(change, kind, match):
+        p = torch.nn.Parameter(torch.ones(32, 32, device=dev))
+        opt = AdamW([p], state_bits=bits)
+        p.grad = torch.ones_like(p)
+        opt.step()
+        change(p, opt)
+        before = p.detach().clone()
+        with pytest.raises(kind, match=match):
+            opt.step()
+        assert torch.equal(p, before) and int(opt.state_dict()["state"][0]["step"]) == 1
+
+    def shrink(p, opt):
+        p.grad = None
+        p.data = p.data[:3]
+        p.grad = torch.ones_like(p)
+
+    def transpose(p, opt):
+        p.data = p.data.t()
+
+    def widen(p, opt):
+        p.grad = None
+        p.data = torch.ones(64, 64, device=dev)
+        p.grad = torch.ones_like(p)
+
+    def offload(p, opt):
+        opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"].cpu()
+
+    def lose(p, opt):
+        del opt.state[p]["exp_avg_sq"]
+
+    def halve(p, opt):
+        opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"].half()
+    moved(shrink, ValueError, "shape")
+    moved(widen, ValueError, "shape")
+    moved(transpose, ValueError, "contiguous")
+    moved(offload, RuntimeError, "device")
+    moved(lose, ValueError, "exp_avg_sq")
+    moved(halve, ValueError, "float16")
+
+
+def test_groups_that_a_caller_changes(dev):
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.float32, [300, 40, 9], seed=2)
+    opt = AdamW(params[:2], lr=0.1, weight_decay=0.0)
+    for p, g in zip(params, grads[0]):
+        p.grad = g
+    opt.step()
+    kept = params[1].detach().clone()
+    opt.param_groups[0]["params"] = [params[0], params[2]]
+    before = params[2].detach().clone()
+    opt.step()
+    assert torch.equal(params[1], kept) and not torch.equal(params[2], before)
+    assert float(opt.state.pop(params[1])["step"]) == 1.0            # torch saves no state of a parameter of no group
+    assert [float(s["step"]) for s in opt.state_dict()["state"].values()] == [2.0, 1.0]
