@@ -391,8 +391,10 @@ class _AdamWTable:
             self.lr_on_device = lr
 
     def gather(self):
-        """Addresses of the gradients, checked; keeps what they belong to, for the launches read it asynchronously."""
-        keep, grads = [], []
+        """Addresses of the gradients, checked, and the copies among them.  Whoever launches on them holds the copies
+        until then (memory given back is handed out again behind the launch, on its stream); the others are their
+        owner's to free, at once if it likes."""
+        copies, grads = [], []
         dtype, device, strided = self.dtype, self.device, torch.strided
         for p, size in zip(self.params, self.sizes):
             g = p.grad
@@ -405,11 +407,10 @@ class _AdamWTable:
                     raise ValueError("a gradient must have its parameter's shape")
                 if not g.is_contiguous():
                     g = g.contiguous()
-                keep.append(g)
+                    copies.append(g)
                 g = g.data_ptr()
             grads.append(g)
-        self._keep = keep
-        return grads
+        return grads, copies
 
     def step(self, lib, opt: "AdamW", grads):
         import ctypes
@@ -582,8 +583,8 @@ class AdamW(torch.optim.Optimizer):
             self._build_tables()
         lib = _lib.load()
         grads = [t.gather() for t in self._tables]        # all are checked before anything changes
-        for t, g in zip(self._tables, grads):
-            t.step(lib, self, g)
+        for t, (addresses, _) in zip(self._tables, grads):
+            t.step(lib, self, addresses)
         return loss
 
     def __getstate__(self):                               # copy.deepcopy, pickle: tables are built anew

@@ -462,3 +462,22 @@ def test_groups_that_a_caller_changes(dev):
     assert torch.equal(params[1], kept) and not torch.equal(params[2], before)
     assert float(opt.state.pop(params[1])["step"]) == 1.0            # torch saves no state of a parameter of no group
     assert [float(s["step"]) for s in opt.state_dict()["state"].values()] == [2.0, 1.0]
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradients_are_freed_when_their_owner_frees_them(dev, strided):
+    """Neither the gradients nor the copies of strided ones outlive the step."""
+    from gnn_amd import AdamW
+    n = 2048
+    p = torch.nn.Parameter(torch.zeros(n, n, device=dev))
+    opt = AdamW([p])
+    for _ in range(3):
+        before = torch.cuda.memory_allocated(dev)
+        g = torch.ones(n, n, device=dev)
+        p.grad = g.t() if strided else g
+        del g
+        opt.step()
+        opt.zero_grad(set_to_none=True)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated(dev) < before + 4 * n * n // 2
+    assert (p == p[0, 0]).all() and float(p[0, 0]) < 0
