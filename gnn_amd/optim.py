@@ -373,6 +373,7 @@ class _AdamWTable:
         chunks = np.repeat(np.array(rows, dtype=np.int64), n_chunks, axis=0)
         chunks[:, 6] = (np.arange(len(chunks)) - np.repeat(ends - n_chunks, n_chunks)) * size
         packed = torch.from_numpy(np.concatenate([chunks.reshape(-1), np.repeat(steps, n_chunks)])).to(self.device)
+        self.packed, self.stream = packed, _lib.current_stream(self.device)
         self.chunks, self.steps = packed.split([chunks.size, len(chunks)])             # one copy to the device
         self.lr = torch.tensor([float(group["lr"])], dtype=torch.float64, device=self.device)
         self.lr_on_device = float(group["lr"])
@@ -416,6 +417,9 @@ class _AdamWTable:
         import ctypes
         self.push_lr()
         group, stream = self.group, _lib.current_stream(self.device)
+        if stream != self.stream:                         # the tables' memory waits for this stream, too
+            for t in (self.packed, self.lr):
+                t.record_stream(torch.cuda.current_stream(self.device))
         limit = 256                                       # RWK_ADAMW_TENSORS: gradient addresses of one launch
         with _lib.device_guard(self.device):
             for base in range(0, len(grads), limit):
@@ -449,7 +453,8 @@ class AdamW(torch.optim.Optimizer):
     devices and stay where they are (:class:`Adam` moves them into one flat fp32 buffer).  The update is computed in
     fp32 and rounded to the parameter's type once; a parameter whose ``.grad`` is ``None`` is skipped and does not
     age.  The step counts and the learning rate live on the device, so a captured step replays correctly;
-    :meth:`push_lr` hands a changed rate to replays.
+    :meth:`push_lr` hands a changed rate to replays.  Replays go on with the states of the capture: after
+    ``load_state_dict``, new groups or states of a caller's own, capture again.
 
     ``state_bits=32``: ``exp_avg`` and ``exp_avg_sq`` are float32, in torch's layout.  ``state_bits=8``: they are
     float8 (e4m3) tensors with one fp32 scale per 256 consecutive elements (``exp_avg_scale``, ``exp_avg_sq_scale``;
@@ -465,6 +470,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("seed must be in 0 .. 2^64 - 1")
         self.state_bits, self.seed = int(state_bits), int(seed)
         self._tables = self._made_from = None
+        self._captured = []                               # what replays of captured steps read and write
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group):
@@ -583,6 +589,8 @@ class AdamW(torch.optim.Optimizer):
             self._build_tables()
         lib = _lib.load()
         grads = [t.gather() for t in self._tables]        # all are checked before anything changes
+        if torch.cuda.is_current_stream_capturing():
+            self._captured.append((self._tables, self._made_from))
         for t, (addresses, _) in zip(self._tables, grads):
             t.step(lib, self, addresses)
         return loss
@@ -594,6 +602,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._tables = self._made_from = None
+        self.__dict__.setdefault("_captured", [])
 
     def state_dict(self):
         self._read_steps()

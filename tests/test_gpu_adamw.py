@@ -481,3 +481,50 @@ def test_gradients_are_freed_when_their_owner_frees_them(dev, strided):
         torch.cuda.synchronize()
         assert torch.cuda.memory_allocated(dev) < before + 4 * n * n // 2
     assert (p == p[0, 0]).all() and float(p[0, 0]) < 0
+
+
+def test_a_captured_step_outlives_its_tables(dev):
+    """Replays after the states were loaded anew read and write what the capture did, which is still there."""
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.float32, [5000, 77], seed=6)
+    opt = AdamW(params)
+    for p, g in zip(params, grads[0]):
+        p.grad = g.clone()
+    opt.step()
+    moments = [opt.state[p]["exp_avg"] for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    opt.load_state_dict(saved)
+    at = [m.data_ptr() for m in moments]
+    tables = [t.packed.data_ptr() for tables, _ in opt._captured for t in tables]
+    del moments
+    taken = [torch.empty(n, device=dev) for n in (5000, 77) for _ in range(40)]          # of the sizes given back
+    assert not set(at) & {t.data_ptr() for t in taken} and len(tables) == 1
+    for t in taken:
+        t.zero_()
+    new = [opt.state[p]["exp_avg"].clone() for p in params]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(not t.any() for t in taken)
+    assert all(torch.equal(opt.state[p]["exp_avg"], n) for p, n in zip(params, new))
+    assert int(opt.state_dict()["state"][0]["step"]) == 1
+
+
+def test_tables_built_on_one_stream_and_dropped_on_another(dev):
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.float32, [5000, 77], seed=6)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = AdamW(params), AdamW(twin)
+    side = torch.cuda.Stream()
+    for gs in grads:
+        for p, q, g in zip(params, twin, gs):
+            p.grad, q.grad = g.clone(), g.clone()
+        b.step()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            a.step()
+        torch.cuda.current_stream().wait_stream(side)
+    a._drop_tables()
+    assert all(torch.equal(p, q) for p, q in zip(params, twin)) and int(a.state[params[0]]["step"]) == 4
