@@ -477,14 +477,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         group = self.param_groups[-1]
         try:
-            if not float(group["lr"]) >= 0.0:
-                raise ValueError("lr must not be negative")
-            if not float(group["eps"]) >= 0.0:
-                raise ValueError("eps must not be negative")
-            if not float(group["weight_decay"]) >= 0.0:
-                raise ValueError("weight_decay must not be negative")
-            if not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
-                raise ValueError("betas must be in [0, 1)")
+            self._check_options(group)
             for p in group["params"]:
                 if not p.is_cuda:
                     raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
@@ -497,6 +490,22 @@ class AdamW(torch.optim.Optimizer):
         for p in group["params"]:
             self.state[p] = self._new_state(p)
         self._drop_tables()
+
+    @staticmethod
+    def _check_options(group):
+        if not float(group["lr"]) >= 0.0:
+            raise ValueError("lr must not be negative")
+        if not float(group["eps"]) >= 0.0:
+            raise ValueError("eps must not be negative")
+        if not float(group["weight_decay"]) >= 0.0:
+            raise ValueError("weight_decay must not be negative")
+        if not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
+            raise ValueError("betas must be in [0, 1)")
+        for name in ("amsgrad", "maximize", "differentiable"):        # torch's, also out of its checkpoints
+            if group.get(name):
+                raise ValueError(f"gnn_amd.AdamW has no {name}")
+        if not group.get("decoupled_weight_decay", True) and float(group["weight_decay"]):
+            raise ValueError("gnn_amd.AdamW decouples the weight decay")
 
     def _new_state(self, p):
         st = {"step": torch.zeros((), dtype=torch.float32)}
@@ -612,6 +621,8 @@ class AdamW(torch.optim.Optimizer):
         names = ["exp_avg", "exp_avg_sq"]
         if self.state_bits == 8:
             names += ["exp_avg_scale", "exp_avg_sq_scale"]
+        for group in state_dict["param_groups"]:
+            self._check_options(group)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         new = {}

@@ -528,3 +528,26 @@ def test_tables_built_on_one_stream_and_dropped_on_another(dev):
         torch.cuda.current_stream().wait_stream(side)
     a._drop_tables()
     assert all(torch.equal(p, q) for p, q in zip(params, twin)) and int(a.state[params[0]]["step"]) == 4
+
+
+def test_options_that_would_be_another_optimiser(dev):
+    """torch's checkpoints load where the steps are the same ones, and are refused, unchanged, where they are not."""
+    from gnn_amd import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(40, device=dev)) for _ in range(2))
+    for kind, options, good in ((torch.optim.AdamW, {}, True), (torch.optim.Adam, dict(weight_decay=0.0), True),
+                                (torch.optim.AdamW, dict(amsgrad=True), False), (torch.optim.AdamW, dict(maximize=True), False),
+                                (torch.optim.Adam, dict(weight_decay=0.1), False)):
+        theirs = kind([q], lr=0.01, **options)
+        q.grad = torch.ones_like(q)
+        theirs.step()
+        mine = AdamW([p], lr=0.5)
+        if good:
+            mine.load_state_dict(theirs.state_dict())
+            assert torch.equal(mine.state[p]["exp_avg"], theirs.state[q]["exp_avg"]) and mine.param_groups[0]["lr"] == 0.01
+        else:
+            with pytest.raises(ValueError, match="gnn_amd.AdamW"):
+                mine.load_state_dict(theirs.state_dict())
+            assert mine.param_groups[0]["lr"] == 0.5 and not mine.state[p]["exp_avg"].any()
+            if "weight_decay" not in options:
+                with pytest.raises(ValueError, match="gnn_amd.AdamW"):
+                    AdamW([dict(params=[p], **options)])
