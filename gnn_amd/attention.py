@@ -285,7 +285,9 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, table, out, stats, low = ctx.saved_tensors
+        q, k, v, *rest = ctx.saved_tensors
+        q, k, v = _heads(q), _heads(k), _heads(v)         # hooks of saved tensors may have laid them anew
+        table, out, stats, low = (None if t is None else t.contiguous() for t in rest)
         segments, causal, scale, buckets = ctx.rest
         dev = q.device
         d_out = _heads(d_out)

@@ -101,6 +101,8 @@ class _LayerNorm(torch.autograd.Function):
         # little is done here: the engine's thread has just woken up, and everything in it takes twice its time
         rows, weight, stats = ctx.saved_tensors
         a, dev = _Args.from_buffer_copy(ctx.args), dy.device          # a copy: a graph may be walked by two threads
+        rows, a.x_stride = _rows(rows)                    # hooks of saved tensors may have laid them anew
+        weight, stats = weight.contiguous(), stats.contiguous()
         dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
         dw, db = torch.empty((2, a.width), dtype=weight.dtype, device=dev).unbind(0)
         if a.rows == 0:

@@ -634,3 +634,29 @@ def test_a_graph_attention_block_trains(dev, bits):
         loss().backward()
         opt.step()
     assert all(p.isfinite().all() for p in params)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_that_were_laid_anew(dev, dtype):
+    """Hooks of saved tensors hand back the same values in a layout of their own."""
+    from gnn_amd import packed_attention, packed_segments, pair_buckets
+    lengths = [70, 33]
+    n = sum(lengths)
+    q, k, v, do, bias, codes = make(dev, dtype, lengths, 4, 2, 24, buckets=3)
+    want = run(q, k, v, do, lengths, True, bias=bias, codes=codes)
+    seg = packed_segments(lengths, dev)
+    buckets = pair_buckets(seg, torch.cat([c.reshape(-1) for c in codes]))
+
+    def apart(t):                                   # elements of a row far apart
+        wide = torch.zeros(*t.shape, 3, dtype=t.dtype, device=t.device)
+        wide[..., 1] = t
+        return wide[..., 1]
+    packed = torch.empty(n, 8, 24, device=dev, dtype=dtype)
+    for part, t in zip(packed.split([4, 2, 2], 1), (q, k, v)):
+        part.copy_(t)
+    for hook in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, apart)):
+        leaves = [t.detach().requires_grad_() for t in (*packed.split([4, 2, 2], 1), bias)]
+        with hook:
+            out = packed_attention(*leaves[:3], seg, causal=True, bias=leaves[3], buckets=buckets)
+        got = [out, *torch.autograd.grad(out, leaves, do)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

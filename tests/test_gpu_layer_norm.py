@@ -259,3 +259,26 @@ def test_rows_of_two_elements(dev):
         th = t * hat
         want = rstd * (t - (t[:, :1] + t[:, 1:]) / 2 - hat * ((th[:, :1] + th[:, 1:]) / 2))
         assert torch.equal(y, hat * w + b) and torch.equal(dx, want)
+
+
+def test_saved_rows_that_were_laid_anew(dev):
+    """Hooks of saved tensors hand back the same values in a layout of their own: a strided slice comes back packed,
+    from host memory too, and the backward pass goes by the rows as they are."""
+    from gnn_amd import layer_norm
+    wide, w, b, dy = make(dev, 60, 96, torch.float32)
+    w, b, dy = w[:64], b[:64], dy[:, :64]
+    plain = run(wide[:, 7:71], w, b, dy)[1]
+
+    def apart(t):                                                 # and packed rows come back strided
+        if t.dim() != 2 or t.shape[1] != 64:
+            return t
+        return torch.nn.functional.pad(t, (3, 5))[:, 3:67]
+    hooks = (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, apart),
+             torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.contiguous()))
+    for hook in hooks:
+        for x in (wide[:, 7:71], wide[:, 7:71].contiguous()):
+            leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+            with hook:
+                y = layer_norm(*leaves)
+            grads = torch.autograd.grad(y, leaves, dy)
+            assert all(torch.equal(g, p) for g, p in zip(grads, plain))
