@@ -11,6 +11,7 @@ import os
 from ctypes import c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librwk.so")
@@ -197,6 +198,18 @@ def element_type(dtype):
     if code is None:
         raise TypeError("expected float32, float16 or bfloat16, got %s" % dtype)
     return code
+
+
+def forward_mode():
+    """Whether tensors may carry tangents (``torch.autograd.forward_ad``).  The kernels see values only, so a call that
+    needs no graph goes through its autograd function all the same then, which refuses them."""
+    return forward_ad._current_level >= 0
+
+
+def refuse_tangent(grad):
+    """For a backward pass, which torch does not ask: an incoming gradient with a tangent."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(grad).tangent is not None:
+        raise RuntimeError("gnn_amd has no forward-mode derivatives of its gradients")
 
 
 def ptr(t):

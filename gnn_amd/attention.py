@@ -285,6 +285,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
+        _lib.refuse_tangent(d_out)
         q, k, v, *rest = ctx.saved_tensors
         q, k, v = _heads(q), _heads(k), _heads(v)         # hooks of saved tensors may have laid them anew
         table, out, stats, low = (None if t is None else t.contiguous() for t in rest)
@@ -370,7 +371,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
         if buckets.segments is not segments:
             raise ValueError("the buckets were made for other segments")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (
-            bias is not None and bias.requires_grad)):
+            bias is not None and bias.requires_grad)) or _lib.forward_mode():
         return _PackedAttention.apply(q, k, v, bias, segments, bool(causal), scale, buckets)
     return _forward(_heads(q), _heads(k), _heads(v), segments, bool(causal), scale,
                     None if bias is None else bias.contiguous(), buckets, False)[0]

@@ -99,6 +99,7 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         # little is done here: the engine's thread has just woken up, and everything in it takes twice its time
+        _lib.refuse_tangent(dy)
         rows, weight, stats = ctx.saved_tensors
         a, dev = _Args.from_buffer_copy(ctx.args), dy.device          # a copy: a graph may be walked by two threads
         rows, a.x_stride = _rows(rows)                    # hooks of saved tensors may have laid them anew
@@ -128,7 +129,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None,
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and
-                                                                               bias.requires_grad)):
+                                                                               bias.requires_grad)) or _lib.forward_mode():
         return _LayerNorm.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, False)[0]
 
