@@ -152,6 +152,7 @@ class PairBuckets:
 def _fill(segments: PackedSegments, entry: str, *args, symmetric: bool = False) -> PairBuckets:
     buckets = PairBuckets(segments, symmetric)
     out = (buckets._codes.data_ptr(),) if symmetric else (buckets._codes.data_ptr(), buckets._by_key.data_ptr())
+    _used_here(segments, None, buckets._stream)
     with _lib.device_guard(segments.device):
         _lib.check(getattr(_lib.load(), entry)(
             *args, segments._seg_ptr, buckets._start.data_ptr(), segments._items, segments.n_items,

@@ -48,3 +48,29 @@ def test_forward_mode_derivatives_are_refused(dev):
             torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, leaves, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_codes_made_on_another_stream_than_their_segments(dev):
+    """Lists dropped while a stream that was not theirs still lays out codes from them: their memory stays."""
+    from gnn_amd import packed_segments, pair_buckets, relative_buckets
+    lengths = [700, 3, 90]
+    flat = torch.randint(0, 9, (sum(n * n for n in lengths),), device=dev).to(torch.uint8)
+    make = (lambda seg: pair_buckets(seg, flat), lambda seg: relative_buckets(seg, 8, 100))
+    side = torch.cuda.Stream()
+    for one in make:
+        want = one(packed_segments(lengths, dev))
+        seg = packed_segments(lengths, dev)
+        at, size = seg._arrays.data_ptr(), seg._arrays.numel()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            busy = torch.randn(2048, 2048, device=dev)
+            for _ in range(20):
+                busy = busy @ busy * 1e-2
+            got = one(seg)
+        got.segments = want.segments
+        del seg
+        taken = [torch.empty(size, dtype=torch.int32, device=dev) for _ in range(20)]
+        still = not side.query()
+        assert not (still and at in [t.data_ptr() for t in taken])
+        torch.cuda.synchronize()
+        assert torch.equal(got._codes, want._codes) and torch.equal(got._by_key, want._by_key)
