@@ -208,6 +208,8 @@ def hop_buckets(adj: torch.Tensor, graph_indicator: torch.Tensor, max_distance: 
     from .distance_bias import distance_bias_structure
     if far not in ("bucket", "mask"):
         raise ValueError('far must be "bucket" or "mask"')
+    if segments is not None and segments.device != adj.device:
+        raise RuntimeError("the matrix and segments must be on the same device")
     st = distance_bias_structure(adj, graph_indicator, max_distance=max_distance)
     if segments is None:
         segments = packed_segments(st.base)

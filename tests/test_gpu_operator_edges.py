@@ -74,3 +74,12 @@ def test_codes_made_on_another_stream_than_their_segments(dev):
         assert not (still and at in [t.data_ptr() for t in taken])
         torch.cuda.synchronize()
         assert torch.equal(got._codes, want._codes) and torch.equal(got._by_key, want._by_key)
+
+
+def test_hop_codes_of_segments_on_another_device(dev):
+    from gnn_amd import hop_buckets, packed_segments
+    seg = packed_segments([2], dev)
+    seg.device = torch.device("cuda", 7)                          # stands for lists made there
+    adj = torch.sparse_coo_tensor(torch.tensor([[0, 1], [1, 0]]), torch.ones(2), (2, 2)).to(dev)
+    with pytest.raises(RuntimeError, match="same device"):
+        hop_buckets(adj, torch.zeros(2, dtype=torch.long, device=dev), segments=seg)
