@@ -5,8 +5,10 @@
 //
 // Both passes are bound by memory: the forward reads and writes each element once, the backward reads x and dy and
 // writes dx.  A row stays in the registers of the lanes that share it between its statistics and its output (the
-// variance is the mean of squared distances from the mean, not a difference of two large sums).  All arithmetic is
-// fp32, one rounding to the element type at the store.
+// variance is the mean of squared distances from the mean, not a difference of two large sums).  The sum of a row is
+// rounded on its way, so that its mean is off by a few roundings of x, which the distances of a row of nearly equal
+// values do not forgive; the sum of these distances says by how much, and comes with the sum of their squares.  All
+// arithmetic is fp32, one rounding to the element type at the store.
 #include "rwk_vec.h"
 
 // Every product and sum is rounded by itself, as the formula is written: the gradient of rows of two elements is what
@@ -91,12 +93,22 @@ __device__ inline void store_row(T *__restrict__ row, int width, int t, const fl
     }
 }
 
+// What is left of a row's mean and its variance from the sums of the distances from the mean and of their squares.  Equal
+// values: distances of a small whole number of x's roundings, whose sums are exact, so both come out exact too.  Up to
+// two elements the mean itself is rounded once only, and the distances are all there is.
+struct Spread { float shift, var; };
+__device__ inline Spread spread(float sum, float squares, int width) {
+    const float shift = width > 2 ? sum / (float)width : 0.f, rest = squares - sum * shift;
+    return {shift, (rest < 0.f ? 0.f : rest) / (float)width};
+}
+
 template <typename T, typename W, int TPR, int V, int IT>
 __global__ void __launch_bounds__(kBlock)
 norm_forward_kernel(const T *__restrict__ x, long long x_stride, const W *__restrict__ weight,
                     const W *__restrict__ bias, long long rows, int width, float eps, T *__restrict__ y,
                     float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float red[2][kWaves];
+    __shared__ float red[kWaves];
+    __shared__ float2 red2[kWaves];
     constexpr int kRows = kBlock / TPR;
     const int t = threadIdx.x % TPR;
     const long long step = (long long)gridDim.x * kRows;
@@ -117,21 +129,27 @@ norm_forward_kernel(const T *__restrict__ x, long long x_stride, const W *__rest
         }
         if (r + step - threadIdx.x / TPR < rows)
             load_row<TPR>(x + (r + step < rows ? r + step : rows - 1) * x_stride, width, t, next);
-        const float mean = row_sum<TPR>(s, red[0]) / (float)width;    // exact for constant rows
+        const float mean = row_sum<TPR>(s, red) / (float)width;
         float q = 0.f;
+        s = 0.f;
 #pragma unroll
         for (int i = 0; i < IT * V; ++i) {
             v[i] = (t + i / V * TPR) * V + i % V < width ? v[i] - mean : 0.f;
+            s += v[i];
             q += v[i] * v[i];
         }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / (float)width + eps);
+        row_sums<TPR>(s, q, red2);
+        const Spread by = spread(s, q, width);
+        const float rstd = 1.f / sqrtf(by.var + eps);
 #pragma unroll
-        for (int i = 0; i < IT * V; ++i)
-            v[i] = bias != nullptr ? v[i] * rstd * w.at(i) + b.at(i) : v[i] * rstd * w.at(i);
+        for (int i = 0; i < IT * V; ++i) {
+            v[i] = (v[i] - by.shift) * rstd * w.at(i);
+            if (bias != nullptr) v[i] += b.at(i);
+        }
         if (!there) continue;
         store_row<T, TPR, V, IT>(y + r * width, width, t, v);
         if (t == 0 && mean_out != nullptr) {
-            mean_out[r] = mean;
+            mean_out[r] = mean + by.shift;
             rstd_out[r] = rstd;
         }
     }
@@ -222,22 +240,27 @@ __global__ void __launch_bounds__(kBlock)
 norm_forward_wide_kernel(const T *__restrict__ x, long long x_stride, const W *__restrict__ weight,
                          const W *__restrict__ bias, int width, float eps, T *__restrict__ y,
                          float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float red[2][kWaves];
+    __shared__ float red[kWaves];
+    __shared__ float2 red2[kWaves];
     const long long r = blockIdx.x;
     const T *row = x + r * x_stride;
     float s = 0.f;
     for (int c = threadIdx.x; c < width; c += kBlock) s += (float)row[c];
-    const float mean = row_sum<kBlock>(s, red[0]) / (float)width;
+    const float mean = row_sum<kBlock>(s, red) / (float)width;
     float q = 0.f;
+    s = 0.f;
     for (int c = threadIdx.x; c < width; c += kBlock) {
         const float d = (float)row[c] - mean;
+        s += d;
         q += d * d;
     }
-    const float rstd = 1.f / sqrtf(row_sum<kBlock>(q, red[1]) / (float)width + eps);
+    row_sums<kBlock>(s, q, red2);
+    const Spread by = spread(s, q, width);
+    const float rstd = 1.f / sqrtf(by.var + eps);
     for (int c = threadIdx.x; c < width; c += kBlock)
-        y[r * width + c] = (T)(((float)row[c] - mean) * rstd * (float)weight[c] + (bias != nullptr ? (float)bias[c] : 0.f));
+        y[r * width + c] = (T)(((float)row[c] - mean - by.shift) * rstd * (float)weight[c] + (bias != nullptr ? (float)bias[c] : 0.f));
     if (threadIdx.x == 0 && mean_out != nullptr) {
-        mean_out[r] = mean;
+        mean_out[r] = mean + by.shift;
         rstd_out[r] = rstd;
     }
 }

@@ -1,4 +1,4 @@
-"""Calls of layer norm and packed attention at the edge of what they promise: other kinds of derivatives."""
+"""Calls of layer norm and packed attention at the edge of what they promise."""
 import pytest
 import torch
 
@@ -83,3 +83,40 @@ def test_hop_codes_of_segments_on_another_device(dev):
     adj = torch.sparse_coo_tensor(torch.tensor([[0, 1], [1, 0]]), torch.ones(2), (2, 2)).to(dev)
     with pytest.raises(RuntimeError, match="same device"):
         hop_buckets(adj, torch.zeros(2, dtype=torch.long, device=dev), segments=seg)
+
+
+@pytest.mark.parametrize("width", [2, 3, 7, 96, 130, 333, 1000, 2049, 4096, 8191, 8193, 20001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_of_constant_rows(dev, dtype, width):
+    """Equal values have no distance from their mean, whatever the rounding of their sum: the result is the bias, and
+    what the backward pass makes of the rows is dy's sum in db and nothing in dw."""
+    from gnn_amd import layer_norm
+    values = torch.tensor([0.1, 1000.1, 12345.678, -7.3e-5, 3.0, 1e20], device=dev)
+    x = values[:, None].expand(-1, width).to(dtype).contiguous().requires_grad_()
+    w = torch.linspace(0.5, 2, width, device=dev).to(dtype).requires_grad_()
+    b = torch.linspace(-1, 1, width, device=dev).to(dtype).requires_grad_()
+    y = layer_norm(x, w, b)
+    assert torch.equal(y, b.expand_as(y))
+    dw = torch.autograd.grad(y, w, torch.ones_like(y))[0]
+    assert not dw.any()
+
+
+@pytest.mark.parametrize("width", [64, 333, 4097, 9001])
+def test_layer_norm_of_rows_with_one_large_element(dev, width):
+    """An element a million times the others, wherever it lies: its neighbours keep their digits relative to the row's
+    deviation, a few fp32 roundings of the largest normalised value's share of the mean."""
+    from gnn_amd import layer_norm
+    g = torch.Generator(device=dev)
+    g.manual_seed(width)
+    x = torch.randn(8, width, generator=g, device=dev)
+    x[torch.arange(8), torch.tensor([0, 1, 2, width // 2, width - 1, 0, 5, 9])] = 1e6
+    ones = torch.ones(width, device=dev)
+    d = x.double()
+    mean, var = d.mean(1, keepdim=True), d.var(1, keepdim=True, unbiased=False)
+    rstd = (var + 1e-5) ** -0.5
+    want = (d - mean) * rstd
+    # mean: the sum's roundings of at most a dozen partial sums that hold the large element, over the width, and one of
+    # the mean; every distance one rounding; the deviation's own half a dozen
+    chain = width / 64 + 80
+    bound = 2.0 ** -24 * ((12e6 / width + mean.abs() + (d - mean).abs()) * rstd + (chain + 8) * want.abs())
+    assert ((layer_norm(x, ones).double() - want).abs() <= bound).all()
