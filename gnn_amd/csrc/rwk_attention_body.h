@@ -593,14 +593,14 @@ __device__ inline bool add_bias(float (&s)[16], const uint32_t (&codes)[4], floa
 // begin their products at a start that holds the logarithm of the factor too, and save the product.  With a bias that
 // would be lost beside a large reference - a row all of whose pairs carry a mask's -1e9 - and for fp32 the rounding of
 // the larger exponent would be the largest error of all: there the exponentials are the forward pass's, bit for bit.
-// start -infinity for a row without pairs and for rows that do not exist.
+// start -infinity for a row without pairs and for rows that do not exist.  `up`: the weights times 2^up.
 template <typename T, bool BIAS>
 struct RowWeight {
     static constexpr bool FOLDED = sizeof(T) == 2 && !BIAS;
     float start, factor;
-    __device__ RowWeight(float ref, float inv, float c) {
-        start = FOLDED ? __log2f(inv) / c - ref : inv == 0.f ? -INFINITY : -ref;
-        factor = inv;
+    __device__ RowWeight(float ref, float inv, float c, int up = 0) {
+        start = FOLDED ? (__log2f(inv) + (float)up) / c - ref : inv == 0.f ? -INFINITY : -ref;
+        factor = ldexpf(inv, up);
     }
     // what the product begins at, and the weight from what it ends at or, with a bias, from the score
     __device__ float begin() const { return FOLDED ? start : 0.f; }
@@ -609,6 +609,44 @@ struct RowWeight {
         return exp2_fast(BIAS ? x + start : (x + start) * c) * factor;
     }
     __device__ float of(float score, float c) const { return weight(score + begin(), start, factor, c); }
+};
+
+// fp16 in the backward pass: its normal numbers end at 2^-14, and weights of many keys and gradients of scores - a weight
+// times a gradient - lie below that long before the results do (d_out of 1e-4, 4096 keys: a fifth of all ds would round to
+// 0).  dK/dV takes the weights times 2^kWeightUp, normal down to 2^-26 and far from the largest number, as no weight
+// exceeds 1 by more than its exponent's rounding.  The ds have no such bound: a wavefront multiplies them by a power of two
+// of its own for each of its rows (dQ) or keys (dK), which begins large and shrinks when a ds would pass 2^15, to where
+// that one is below 2^13; the sums shrink with it and are divided by it at the end.  Eight maxima of three and a branch per
+// 32 x 32 pairs: 48 prompts of up to 1500 rows, 64 elements, forward and backward 559 to 591 us.
+template <typename T> constexpr bool kNarrowRange = sizeof(T) == 2 && (T)1e-30f == (T)0.f;
+template <typename T> constexpr int kWeightUp = kNarrowRange<T> ? 12 : 0;
+template <typename T>
+struct GradientScale {
+    static constexpr float TOP = 0x1p15f;
+    float by = kNarrowRange<T> ? 0x1p60f : 1.f, limit = TOP / 0x1p60f;
+    // makes room for these ds in `acc`, the sums of the ones before, and multiplies them
+    template <typename R>
+    __device__ void apply(float (&x)[16], R &acc) {
+        if constexpr (kNarrowRange<T>) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(x[i]));
+            if (__builtin_amdgcn_ballot_w64(most > limit) != 0) {
+                most = fmaxf(most, __shfl_xor(most, 32, 64));          // both halves of a row or key
+                const float now = most > limit ? fminf(by, ldexpf(1.f, 13 - __builtin_amdgcn_frexp_expf(most))) : by;
+                acc.scale(now / by);
+                by = now;
+                limit = TOP / now;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= by;
+        }
+    }
+    // the sums as they are
+    template <typename R>
+    __device__ void undo(R &acc, int up) const {
+        if constexpr (kNarrowRange<T>) acc.scale(ldexpf(1.f / by, -up));
+    }
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -987,6 +1025,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
 
     Result<T, KS> acc;
     acc.clear();
+    GradientScale<T> scaled;
     const int end = causal && at.first + 32 * NW < n ? at.first + 32 * NW : n;
     keys.commit(tiles);
     values.commit(tiles + BN * S::W);
@@ -1044,6 +1083,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
                     for (int g = 0; g < 4; ++g) buckets.add(four[g], s + 4 * g);
                 }
             }
+            scaled.apply(s, acc);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> f = pack<T>(s, u);
@@ -1058,6 +1098,7 @@ attention_dq_kernel(const RwkAttnArgs p) {
     }
     acc.finish();
     const bool again = q < n && not_finite<KS>(acc.a);
+    scaled.undo(acc, 0);
     // A row's only pair has weight 1 whatever its score: no gradient, where d_out . v and delta, summed in different
     // orders, differ by a rounding.  (Times 0: what is not a number stays.)
     const float some = n == 1 || (causal && q == 0) ? 0.f : 1.f;
@@ -1128,6 +1169,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     Result<T, KS> dk, dv;
     dk.clear();
     dv.clear();
+    GradientScale<T> scaled;
     const int begin = causal ? at.first : 0;
     for (int g = 0; g < p.part_heads; ++g) {
         const int head = at.head + g;
@@ -1145,7 +1187,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
             if (threadIdx.x < BQ) {
                 const bool there = q < n;
                 const Weight w(there ? p.a.stats[2 * (row_at + q)] : 0.f,
-                               there ? p.a.stats[2 * (row_at + q) + 1] : 0.f, c);
+                               there ? p.a.stats[2 * (row_at + q) + 1] : 0.f, c, kWeightUp<T>);
                 held[0] = w.start;
                 held[1] = there ? -p.a.delta[row_at + q] : 0.f;
                 if (!Weight::FOLDED) held[NS - 1] = w.factor;
@@ -1212,6 +1254,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
                     s[i] = Weight::FOLDED ? Weight::weight(s[i], 0.f, 1.f, c) : Weight::weight(s[i], st[r], st[2 * BQ + r], c);
                     d[i] = weigh(s[i], d[i]);
                 }
+                scaled.apply(d, dk);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     dv.add(o_tile, 32 * t + 16 * u, pack<T>(s, u), lane);
@@ -1227,12 +1270,14 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     dv.finish();
     const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a), again = k < n && (bad_k || bad_v);
     const float by = n == 1 ? 0.f * p.a.scale : p.a.scale;        // as in dQ: a segment of one row has one pair
+    constexpr float dv_by = 1.f / (1 << kWeightUp<T>);
+    scaled.undo(dk, kWeightUp<T>);
     if (k < n && !again && p.parts > 1) {
         store_rows<false, float, DT>(out.dk + to, dim, h, dk.a, by);
-        store_rows<false, float, DT>(out.dv + to, dim, h, dv.a, 1.f);
+        store_rows<false, float, DT>(out.dv + to, dim, h, dv.a, dv_by);
     } else if (k < n && !again) {
         store_rows<false, T, DT>((T *)p.a.dk + out.at + to, dim, h, dk.a, by);
-        store_rows<false, T, DT>((T *)p.a.dv + out.at + to, dim, h, dv.a, 1.f);
+        store_rows<false, T, DT>((T *)p.a.dv + out.at + to, dim, h, dv.a, dv_by);
     }
     if (any_lane(again)) exact_dkv<T, BIAS>(p, at, part, k, begin, c, again);
 }

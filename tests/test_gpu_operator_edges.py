@@ -120,3 +120,87 @@ def test_layer_norm_of_rows_with_one_large_element(dev, width):
     chain = width / 64 + 80
     bound = 2.0 ** -24 * ((12e6 / width + mean.abs() + (d - mean).abs()) * rstd + (chain + 8) * want.abs())
     assert ((layer_norm(x, ones).double() - want).abs() <= bound).all()
+
+
+def gradients(q, k, v, do, bias=None, code=None):
+    """64-bit gradients of causal attention of one segment, and what the roundings of p and ds to the element type do to
+    them: the errors of a sum's terms are independent and at most half a step each, so the error's standard deviation is
+    at most half a step of the root of the terms' squares."""
+    n, heads, dim = q.shape
+    group = heads // k.shape[1]
+    u = torch.finfo(q.dtype).eps / 2
+    a, b, c, d = (t.double().transpose(0, 1) for t in (q, k, v, do))
+    b, c = b.repeat_interleave(group, 0), c.repeat_interleave(group, 0)
+    s = a @ b.transpose(1, 2) * dim ** -0.5
+    off = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1)
+    if bias is not None:
+        s = s + bias.double()[:, code.long()]
+    p = torch.softmax(s.masked_fill(off, -torch.inf), 2)
+    dp = d @ c.transpose(1, 2)
+    ds = p * (dp - (p * dp).sum(2, keepdim=True)) * dim ** -0.5
+    ds[:, 0] = 0                                                  # a row of one pair
+    pt, dst = p.transpose(1, 2), ds.transpose(1, 2)
+    want = [ds @ b, dst @ a, pt @ d]
+    noise = [u * (x.square() @ y.square()).sqrt() for x, y in ((ds, b), (dst, a), (pt, d))]
+
+    def shared(x):
+        return x.view(-1, group, n, dim).sum(1).transpose(0, 1)
+    want = [want[0].transpose(0, 1), shared(want[1]), shared(want[2])]
+    noise = [noise[0].transpose(0, 1), *(shared(x.square()).sqrt() for x in noise[1:])]
+    return want, noise
+
+
+def check_roundings(got, want, noise, dtype):
+    for x, t, e, name in zip(got, want, noise, ("dq", "dk", "dv")):
+        once = (t.to(dtype).double() - t).norm()                  # one rounding of the result
+        # twice the noise: delta and the products' fp32 sums take part, too
+        assert float((x.double() - t).norm()) <= float(1.1 * once + 2 * e.norm()), name
+
+
+@pytest.mark.parametrize("size", [3e-5, 1e-4, 1e-3, 1.0, 2e3, "mixed"])
+@pytest.mark.parametrize("dim,buckets", [(16, 0), (64, 0), (128, 0), (64, 4), (16, 4)])
+def test_fp16_gradients_of_small_and_large_upstream_gradients(dev, size, dim, buckets):
+    """The roundings of p and ds are relative to them, however small the upstream gradient and however many the keys."""
+    from gnn_amd import packed_attention, packed_segments, pair_buckets
+    g = torch.Generator(device=dev)
+    g.manual_seed(dim + buckets)
+    n = 1500
+    q, k, v, do = (torch.randn(n, h, dim, generator=g, device=dev).half() for h in (4, 2, 2, 4))
+    if size == "mixed":
+        do = do * 10.0 ** torch.randint(-4, 3, (n, 1, 1), generator=g, device=dev)
+    else:
+        do = do * size
+    do = do.half()
+    seg = packed_segments([n], dev)
+    leaves, kw, bias, code = [t.requires_grad_() for t in (q, k, v)], {}, None, None
+    if buckets:
+        bias = torch.randn(4, buckets, generator=g, device=dev).half()
+        code = torch.randint(0, buckets, (n, n), generator=g, device=dev).to(torch.uint8)
+        kw = dict(bias=bias, buckets=pair_buckets(seg, code))
+    got = torch.autograd.grad(packed_attention(*leaves, seg, causal=True, **kw), leaves, do)
+    want, noise = gradients(*(t.detach() for t in (q, k, v)), do, bias, code)
+    check_roundings(got, want, noise, torch.float16)
+
+
+@pytest.mark.parametrize("dim", [16, 64])
+def test_fp16_weights_of_very_many_keys(dev, dim):
+    """All scores alike: every weight is 1 / n, below the smallest normal number of fp16, and so is every ds."""
+    from gnn_amd import packed_attention, packed_segments
+    n = 40000
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    v = torch.randn(n, 1, dim, generator=g, device=dev).half().requires_grad_()
+    do = torch.randn(n, 1, dim, generator=g, device=dev).half()
+    zero = torch.zeros(n, 1, dim, device=dev, dtype=torch.float16)
+    k = torch.randn(n, 1, dim, generator=g, device=dev).half()
+    q = zero.clone().requires_grad_()
+    dq, dv = torch.autograd.grad(packed_attention(q, k, v, packed_segments([n], dev)), (q, v), do)
+    vd, dd, kd = (t.detach().double()[:, 0] for t in (v, do, k))
+    want_v = dd.mean(0)                                           # the same for all keys
+    want_q = dim ** -0.5 * (dd @ (vd.t() @ kd) / n - (dd @ vd.mean(0))[:, None] * kd.mean(0))
+    u = 2.0 ** -11
+    # 40000 equal weights share their rounding's relative error, if it is no subnormal one; the result's own rounding
+    assert float((dv[:, 0].double() - want_v).abs().max()) <= float((2.5 * u * want_v.abs()).max()) + 1e-6
+    noise = u * dim ** -0.5 / n * (n ** 0.5) * float((dd @ vd.t()[:, :2000]).std() * kd.std())
+    once = (want_q.half().double() - want_q).norm() / want_q.numel() ** 0.5
+    assert float((dq[:, 0].double() - want_q).norm() / want_q.numel() ** 0.5) <= float(1.1 * once) + 2 * noise
