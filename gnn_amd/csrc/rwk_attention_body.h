@@ -825,9 +825,11 @@ template <int NW, int COLS> constexpr int code_bytes() { return 2 * 32 * NW * CO
 template <typename T, int NW> constexpr int tile_rows() { return sizeof(T) == 2 && NW > 1 ? 64 : 32; }
 
 // Scores below the reference by this much or less (in powers of two) leave it as it is: the sums and the output are
-// rescaled only when a row's maximum has grown by a factor of 2^8 in its exponential, and stay far inside fp32's (and
-// the probabilities inside fp16's) range.
-constexpr float kSlack = 8.f;
+// rescaled only when a row's maximum has grown by that factor in its exponential, and stay far inside fp32's range.
+// fp16: the weights are 2^6 times the exponentials and so at most 2^13 - 2^15 where a large bias leaves the reference no
+// digits for the 6 - and keys that a row hardly looks at count down to 2^-31 of its largest weight, by thousands of them.
+template <typename T> constexpr float kSlack = kNarrowRange<T> ? 7.f : 8.f;
+template <typename T> constexpr int kExpUp = kNarrowRange<T> ? 6 : 0;
 
 // FINE (16-bit types): a weight meets the values as two numbers of the type, the second what the rounding to the first
 // left over.  The weights' rounding counts most where few of them are added up and, through delta, which comes from the
@@ -862,7 +864,7 @@ attention_forward_kernel(const RwkAttnArgs p) {
 
     // without a bias the maximum is taken over q . k and the scale meets it in the exponent; with one the scores are
     // the sum, in units of log2(e) (load_table)
-    const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale, slack = kSlack / c;
+    const float scale = p.a.scale * kLog2e, c = BIAS ? 1.f : scale, slack = kSlack<T> / c;
     Result<T, KS> acc;
     acc.clear();
     float ref = -INFINITY, sum = 0.f;           // ref: what the exponentials are taken relative to
@@ -921,7 +923,7 @@ attention_forward_kernel(const RwkAttnArgs p) {
                 sum *= shrink;
                 acc.scale(shrink);
             }
-            const float base = ref == -INFINITY ? 0.f : ref, base_c = base * c;
+            const float base = (ref == -INFINITY ? 0.f : ref) - (BIAS ? kExpUp<T> : 0), base_c = base * c - kExpUp<T>;
             float part = 0.f;
 #pragma unroll
             for (int t = 0; t < TN; ++t)
@@ -951,17 +953,19 @@ attention_forward_kernel(const RwkAttnArgs p) {
     acc.finish();
     sum += __shfl_xor(sum, 32, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;      // a row without pairs: zeros
+    // what pairs' weights follow from: exp2((score - base) c) * factor
+    const float base = (ref == -INFINITY ? 0.f : ref) - (BIAS ? kExpUp<T> : 0), factor = BIAS ? inv : ldexpf(inv, kExpUp<T>);
     const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
     const bool again = q < n && not_finite<KS>(acc.a);
     if (q < n && !again) {
         store_rows<false, T, DT>((T *)p.a.out + o_at, dim, h, acc.a, inv);
         if (p.a.out_low != nullptr) store_rows<true, T, DT>((T *)p.a.out_low + o_at, dim, h, acc.a, inv);
     }
-    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, ref == -INFINITY ? 0.f : ref, inv, c, again);
+    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, base, factor, c, again);
     if (q < n && p.a.stats != nullptr && h == 0) {
         float *st = p.a.stats + 2 * (at.head * p.a.rows + at.base + q);
-        st[0] = ref == -INFINITY ? 0.f : ref;
-        st[1] = inv;
+        st[0] = base;
+        st[1] = factor;
     }
 }
 

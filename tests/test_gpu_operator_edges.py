@@ -1,4 +1,6 @@
 """Calls of layer norm and packed attention at the edge of what they promise."""
+import math
+
 import pytest
 import torch
 
@@ -204,3 +206,30 @@ def test_fp16_weights_of_very_many_keys(dev, dim):
     noise = u * dim ** -0.5 / n * (n ** 0.5) * float((dd @ vd.t()[:, :2000]).std() * kd.std())
     once = (want_q.half().double() - want_q).norm() / want_q.numel() ** 0.5
     assert float((dq[:, 0].double() - want_q).norm() / want_q.numel() ** 0.5) <= float(1.1 * once) + 2 * noise
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,buckets", [(16, 0), (64, 0), (128, 0), (16, 2), (64, 2)])
+def test_thousands_of_keys_that_a_row_hardly_looks_at(dev, dtype, dim, buckets):
+    """One key takes nearly all of every row's weight and has a value of zeros; what 4095 others of 2^-25.6 each add up to
+    is the whole result.  fp16: half a step of its smallest numbers, 2^-25, against a weight of 2^-19.6; the others half
+    a step of the type; besides a few fp32 roundings of the score."""
+    from gnn_amd import packed_attention, packed_segments, pair_buckets
+    n, high = 4096, 17.75
+    q, k, v = (torch.zeros(n, 1, dim, device=dev, dtype=dtype) for _ in range(3))
+    v[1:] = 100
+    seg, kw = packed_segments([n], dev), {}
+    if buckets:
+        code = torch.ones(n, n, dtype=torch.uint8, device=dev)
+        code[:, 0] = 0
+        kw = dict(bias=torch.tensor([[high - 5, -5.0]], device=dev, dtype=dtype), buckets=pair_buckets(seg, code))
+    else:
+        q[:, 0, 3] = 1
+        k[0, 0, 3] = high
+    out = packed_attention(q, k, v, seg, scale=1.0, **kw)
+    if buckets:
+        high = float(kw["bias"][0, 0] - kw["bias"][0, 1])
+    small = math.exp(-high) if dtype != torch.bfloat16 else math.exp(-float(torch.tensor(high).to(dtype)))
+    want = 100 * 4095 * small / (1 + 4095 * small)
+    tol = {torch.float16: 2.0 ** (-25 + 19.7), torch.bfloat16: 2.0 ** -7, torch.float32: 1e-4}[dtype]
+    assert float((out.double() / want - 1).abs().max()) <= tol
