@@ -340,7 +340,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
     scores before their products (to two numbers before ``k`` for heads of up to 32 elements).  Errors are then up to 1.5
     times those of rounding the results once.  fp16: these factors are scaled to the type's range first, so that small
     upstream gradients and many keys cost no digits.  What a pair's rows hold counts for nothing where the pair does not
-    attend, values that are not finite included (blocks of rows whose result is not finite take much longer)."""
+    attend, values that are not finite included: blocks of rows that such a value may have reached are computed a second
+    time, which takes up to some twenty times as long (2 prompts of 2048 rows, 32 heads of 128: forward 0.1 ms, 1.9 with
+    infinities all over ``v``).  Where it does attend, the elements it reaches are not finite, infinite or NaN."""
     if not q.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
     shape, k_shape, dtype, device = q.shape, k.shape, q.dtype, q.device          # every look costs a small call time

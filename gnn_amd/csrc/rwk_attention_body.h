@@ -651,10 +651,13 @@ struct GradientScale {
 
 // ---------------------------------------------------------------------------------------------------------------
 // A pair that does not attend counts for nothing whatever its rows hold, but a matrix instruction adds 0 times what it
-// finds: not a number where that is not finite.  So rows whose result is not finite are computed again, pair by pair and
-// without matrix instructions, leaving out the pairs whose weight is zero.  Slow, and only ever run for such rows.
-// Lanes l and l + 32 share a row, eight elements each of every sixteen.  Elements are taken sixteen at a time, each time
-// with all the row's products over again: few registers, so that the code costs the kernels' loops none.
+// finds: not a number where that is not finite.  So rows whose result is not finite are computed again - if pairs that do
+// not attend can be the reason: there are such pairs (a causal mask: in the tiles on the diagonal only) and one of their
+// rows does hold something that is not finite.  An overflow in d_out, say, is none for dQ, whose products take keys.  The
+// second time what is not finite is taken out of the operands and counted where it is weighed: elements whose sum would
+// have had any come out as NaN, the others as they should.  The operands come from memory, 32 elements of a result in a
+// pass with all of its scores over again, which needs few registers, so that the code costs the kernels' loops none; a
+// pass ends early once nothing is left that could be finite.
 // ---------------------------------------------------------------------------------------------------------------
 // whether the lane's row is not finite
 template <int KS, int DT>
@@ -670,34 +673,74 @@ __device__ inline bool not_finite(const f32x16 (&acc)[DT]) {
 }
 __device__ inline bool any_lane(bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; }
 
+// whether rows lo .. hi - 1 of a head, `base` its first, hold anything that is not finite: the wavefront together
 template <typename T>
-__device__ inline float row_product(const T *a, const T *b, int h, int dim) {
-    float sum = 0.f;
+__device__ inline bool holds_not_finite(const T *base, long long stride, int lo, int hi, int dim) {
+    float t = 0.f;
 #pragma unroll 1
-    for (int d = 8 * h; d < dim + 8 * h; d += 16) {            // both halves in the same rounds
-        const Frag<T> x = load_global<T>(a, d, dim), y = load_global<T>(b, d, dim);
+    for (int r = lo + (int)(threadIdx.x & 63); r < hi; r += 64)
+#pragma unroll 1
+        for (int d = 0; d < dim; d += 8) {
+            const Frag<T> x = load_global<T>(base + r * stride, d, dim);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf((float)x.v[e], (float)y.v[e], sum);
-    }
-    return sum + __shfl_xor(sum, 32, 64);
+            for (int e = 0; e < 8; ++e) t = fmaf((float)x.v[e], 0.f, t);
+        }
+    return any_lane(t != t);
 }
 
+// products of the lane's row with 32 rows of a head, from `first` (the last of n for those behind it): a transposed result
 template <typename T>
-__device__ inline void add_row(float (&acc)[8], float weight, const T *row, int d, int dim) {
-    if (weight == 0.f) return;
-    const Frag<T> x = load_global<T>(row, d, dim);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(weight, (float)x.v[e], acc[e]);
+__device__ inline f32x16 row_products(const T *base, long long stride, int first, int n, const T *row, int dim) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const T *other = base + min(first + (lane & 31), n - 1) * stride;
+    f32x16 x = f32x16{};
+#pragma unroll 1
+    for (int d = 8 * h; d < dim + 8 * h; d += 16)              // both halves in the same rounds
+        x = mma(load_global<T>(other, d, dim), load_global<T>(row, d, dim), x);
+    return x;
 }
 
-template <bool LOW, typename T>
-__device__ inline void store_eight(T *row, const float (&acc)[8], float scale, int d, int dim) {
+// 32 elements, from `d`, of a sum over rows of a head: what is finite, and how often anything else was weighed
+template <typename T>
+struct FiniteSum {
+    f32x16 sum = f32x16{}, spoilt = f32x16{};
+    // eight weights of the lane's row, for the rows first .. first + 15 of n as column_operand has them
+    __device__ void add(const T *base, long long stride, int first, int n, int d, int dim, const float (&weight)[16], int s) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, col = d + (lane & 31);
+        Frag<T> x, other, on;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float x = acc[e] * scale;
-        if (d + e < dim) row[d + e] = LOW ? (T)(x - (float)(T)x) : (T)x;
+        for (int e = 0; e < 8; ++e) {
+            const int row = first + 8 * (e >> 2) + 4 * h + (e & 3);
+            const float v = (float)base[min(row, n - 1) * stride + min(col, dim - 1)];      // no branches
+            const bool there = row < n && col < dim, finite = fabsf(v) <= 3.402823466e38f;
+            x.v[e] = (T)(there && finite ? v : 0.f);
+            other.v[e] = (T)(there && !finite ? 1.f : 0.f);
+            on.v[e] = (T)(weight[8 * s + e] == 0.f ? 0.f : 1.f);
+        }
+        const Frag<T> f = pack<T>(weight, s);
+        sum = mma(x, f, sum);
+        if constexpr (sizeof(T) == 2) sum = mma(x, left_over<T>(weight, f, s), sum);
+        spoilt = mma(other, on, spoilt);
     }
-}
+    // whether no element of any of the wavefront's rows that count can be finite any more
+    __device__ bool lost(int d, int dim, bool mine) const {
+        const int h = (int)(threadIdx.x >> 5) & 1;
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) all = all && (d + reg_row(i, h) >= dim || sum[i] != sum[i] || spoilt[i] > 0.f);
+        return !any_lane(mine && !all);
+    }
+    // LOW: what the rounding to R left over
+    template <bool LOW, typename R>
+    __device__ void store(R *row, int d, int dim, float undo, float scale) const {
+        const int h = (int)(threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = spoilt[i] > 0.f ? __builtin_nanf("") : sum[i] * undo * scale;
+            if (d + reg_row(i, h) < dim) row[d + reg_row(i, h)] = LOW ? (R)(x - (float)(R)x) : (R)x;
+        }
+    }
+};
 
 // exponent (less the reference's part) of pair (q, k) from its product, -infinity if it does not attend
 template <bool BIAS>
@@ -706,60 +749,82 @@ __device__ inline float pair_score(const RwkAttnArgs &p, const Place &at, float 
     float x = product;
     if (BIAS) {
         const int nb = (int)p.a.n_buckets;
-        int b = nb;
-        if (on) b = min((int)p.a.codes[p.a.code_start[at.seg] + (long long)q * ((at.n + 31) / 32 * 32) + k], nb);
+        const int b = min((int)p.a.codes[p.a.code_start[at.seg] + (long long)min(q, at.n - 1) * ((at.n + 31) / 32 * 32) +
+                                         min(k, at.n - 1)], nb);
         x = fmaf(product, p.a.scale * kLog2e, look_up(table, b));
         on = on && b < nb;
     }
     return on ? x : -INFINITY;
 }
 
-// The lane's row of the operands, at `row` (clamped to the segment) of head or kv_head.
+// row `row` of a head; 0 for the first of the segment
 template <typename T>
-__device__ inline const T *row_of(const void *base, long long row, long long stride, long long head, long long head_stride) {
-    return (const T *)base + row * stride + head * head_stride;
+__device__ inline const T *row_of(const void *base, const Place &at, int row, long long stride, long long head, long long head_stride) {
+    return (const T *)base + (at.base + row) * stride + head * head_stride;
+}
+
+// Whether pairs of the wavefront's rows from q0 that do not attend may be why a result is not finite: `base` holds what
+// is weighed, the keys or the values.
+template <typename T, bool BIAS>
+__device__ inline bool masked_may_spoil(const RwkAttnArgs &p, const Place &at, const T *base, long long stride, int q0, int end) {
+    if (!BIAS && p.a.causal == 0) return false;
+    // causal: tiles of at most 64 keys, the last of which begins no later than the wavefront's last row
+    return holds_not_finite(base, stride, BIAS ? 0 : q0, min(at.n, BIAS ? end + 32 : q0 + 64 + 32), (int)p.a.dim);
 }
 
 template <typename T, bool BIAS>
-__device__ inline void exact_forward(const RwkAttnArgs &p, const Place &at, float table, int q, int end, float base,
-                                     float inv, float c, bool mine) {
-    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
-    const long long row = at.base + min(q, at.n - 1);
-    const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
+__device__ inline void again_forward(const RwkAttnArgs &p, const Place &at, float table, int q, int end, float base,
+                                     float factor, float c, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim, qc = min(q, at.n - 1);
+    const T *q_row = row_of<T>(p.a.q, at, qc, p.a.q_row, at.head, p.a.q_head);
+    const T *keys = row_of<T>(p.a.k, at, 0, p.a.k_row, at.kv_head, p.a.k_head);
+    const T *values = row_of<T>(p.a.v, at, 0, p.a.v_row, at.kv_head, p.a.v_head);
+    const long long to = ((at.base + qc) * p.a.heads + at.head) * dim;
 #pragma unroll 1
-    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
-        float o[8] = {};
+    for (int d = 0; d < dim; d += 32) {
+        FiniteSum<T> o;
 #pragma unroll 1
-        for (int k = 0; k < end; ++k) {
-            const T *k_row = row_of<T>(p.a.k, at.base + k, p.a.k_row, at.kv_head, p.a.k_head);
-            const float x = pair_score<BIAS>(p, at, table, q, k, row_product(q_row, k_row, h, dim));
-            add_row(o, exp2_fast((x - base) * c), row_of<T>(p.a.v, at.base + k, p.a.v_row, at.kv_head, p.a.v_head), d, dim);
+        for (int k0 = 0; k0 < end; k0 += 32) {
+            float s[16];
+            unpack(row_products(keys, p.a.k_row, k0, at.n, q_row, dim), s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = exp2_fast((pair_score<BIAS>(p, at, table, q, k0 + reg_row(i, h), s[i]) - base) * c);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) o.add(values, p.a.v_row, k0 + 16 * u, at.n, d, dim, s, u);
+            if (o.lost(d, dim, mine)) break;
         }
-        const long long to = (row * p.a.heads + at.head) * dim;
-        if (mine) store_eight<false>((T *)p.a.out + to, o, inv, d, dim);
-        if (mine && p.a.out_low != nullptr) store_eight<true>((T *)p.a.out_low + to, o, inv, d, dim);
+        if (mine) o.template store<false>((T *)p.a.out + to, d, dim, 1.f, factor);
+        if (mine && p.a.out_low != nullptr) o.template store<true>((T *)p.a.out_low + to, d, dim, 1.f, factor);
     }
 }
 
 template <typename T, bool BIAS>
-__device__ inline void exact_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end,
-                                const RowWeight<T, BIAS> &weight, float delta, float c, bool mine) {
-    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
-    const long long row = at.base + min(q, at.n - 1);
-    const T *q_row = row_of<T>(p.a.q, row, p.a.q_row, at.head, p.a.q_head);
-    const T *o_row = row_of<T>(p.a.d_out, row, p.a.do_row, at.head, p.a.do_head);
+__device__ inline void again_dq(const RwkAttnArgs &p, const Place &at, float table, int q, int end,
+                                const RowWeight<T, BIAS> &weight, float delta, float c, float by, float scale, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim, qc = min(q, at.n - 1);
+    const T *q_row = row_of<T>(p.a.q, at, qc, p.a.q_row, at.head, p.a.q_head);
+    const T *o_row = row_of<T>(p.a.d_out, at, qc, p.a.do_row, at.head, p.a.do_head);
+    const T *keys = row_of<T>(p.a.k, at, 0, p.a.k_row, at.kv_head, p.a.k_head);
+    const T *values = row_of<T>(p.a.v, at, 0, p.a.v_row, at.kv_head, p.a.v_head);
 #pragma unroll 1
-    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
-        float g[8] = {};
+    for (int d = 0; d < dim; d += 32) {
+        FiniteSum<T> g;
 #pragma unroll 1
-        for (int k = 0; k < end; ++k) {
-            const T *k_row = row_of<T>(p.a.k, at.base + k, p.a.k_row, at.kv_head, p.a.k_head);
-            const T *v_row = row_of<T>(p.a.v, at.base + k, p.a.v_row, at.kv_head, p.a.v_head);
-            const float x = pair_score<BIAS>(p, at, table, q, k, row_product(q_row, k_row, h, dim));
-            const float w = weigh(weight.of(x, c), row_product(o_row, v_row, h, dim) - delta);
-            add_row(g, w, k_row, d, dim);
+        for (int k0 = 0; k0 < end; k0 += 32) {
+            float s[16], dp[16];
+            unpack(row_products(keys, p.a.k_row, k0, at.n, q_row, dim), s);
+            unpack(row_products(values, p.a.v_row, k0, at.n, o_row, dim), dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = pair_score<BIAS>(p, at, table, q, k0 + reg_row(i, h), s[i]);
+                s[i] = weigh(weight.of(x, c), dp[i] - delta) * by;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) g.add(keys, p.a.k_row, k0 + 16 * u, at.n, d, dim, s, u);
+            if (g.lost(d, dim, mine)) break;
         }
-        if (mine) store_eight<false>((T *)p.a.dq + (row * p.a.heads + at.head) * dim, g, p.a.scale, d, dim);
+        if (mine) g.template store<false>((T *)p.a.dq + ((at.base + qc) * p.a.heads + at.head) * dim, d, dim, 1.f / by, scale);
     }
 }
 
@@ -778,37 +843,65 @@ struct KeyGradients {
     }
 };
 
+// as masked_may_spoil, for the wavefront's keys from k0: queries and d_out
 template <typename T, bool BIAS>
-__device__ inline void exact_dkv(const RwkAttnArgs &p, const Place &at, int part, int k, int begin, float c, bool mine) {
-    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim;
-    const long long row = at.base + min(k, at.n - 1);
-    const T *k_row = row_of<T>(p.a.k, row, p.a.k_row, at.kv_head, p.a.k_head);
-    const T *v_row = row_of<T>(p.a.v, row, p.a.v_row, at.kv_head, p.a.v_head);
+__device__ inline bool masked_may_spoil_keys(const RwkAttnArgs &p, const Place &at, int k0, int begin) {
+    if (!BIAS && p.a.causal == 0) return false;
+    const int lo = BIAS ? begin : k0, hi = BIAS ? at.n : min(at.n, k0 + 64);
+    bool any = false;
 #pragma unroll 1
-    for (int d = 8 * h; d < dim + 8 * h; d += 16) {
-        float gk[8] = {}, gv[8] = {};
+    for (int head = at.head; head < at.head + p.part_heads && !any; ++head)
+        any = holds_not_finite(row_of<T>(p.a.q, at, 0, p.a.q_row, head, p.a.q_head), p.a.q_row, lo, hi, (int)p.a.dim) ||
+              holds_not_finite(row_of<T>(p.a.d_out, at, 0, p.a.do_row, head, p.a.do_head), p.a.do_row, lo, hi, (int)p.a.dim);
+    return any;
+}
+
+template <typename T, bool BIAS>
+__device__ inline void again_dkv(const RwkAttnArgs &p, const Place &at, int part, int k, int begin, float c, float by,
+                                 float dk_scale, bool mine) {
+    const int h = (int)(threadIdx.x >> 5) & 1, dim = (int)p.a.dim, kc = min(k, at.n - 1);
+    const T *k_row = row_of<T>(p.a.k, at, kc, p.a.k_row, at.kv_head, p.a.k_head);
+    const T *v_row = row_of<T>(p.a.v, at, kc, p.a.v_row, at.kv_head, p.a.v_head);
+    const KeyGradients out(p, at, part);
+    const long long to = kc * p.a.kv_heads * dim;
 #pragma unroll 1
-        for (int head = at.head; head < at.head + p.part_heads; ++head) {
-            const float table = BIAS ? load_table<T>(p, head) : 0.f;
+    for (int pass = 0; pass < 2; ++pass) {                     // dK, then dV
+        const float times = ldexpf(pass == 0 ? by : 1.f, kWeightUp<T>), scale = pass == 0 ? dk_scale : 1.f;
+        float *sums = pass == 0 ? out.dk : out.dv;
+        T *result = (pass == 0 ? (T *)p.a.dk : (T *)p.a.dv) + out.at;
 #pragma unroll 1
-            for (int q = begin; q < at.n; ++q) {
-                const T *q_row = row_of<T>(p.a.q, at.base + q, p.a.q_row, head, p.a.q_head);
-                const T *o_row = row_of<T>(p.a.d_out, at.base + q, p.a.do_row, head, p.a.do_head);
-                const long long st = head * p.a.rows + at.base + q;
-                const float x = pair_score<BIAS>(p, at, table, q, k, row_product(k_row, q_row, h, dim));
-                const float w = RowWeight<T, BIAS>(p.a.stats[2 * st], p.a.stats[2 * st + 1], c).of(x, c);
-                add_row(gv, w, o_row, d, dim);
-                add_row(gk, weigh(w, row_product(v_row, o_row, h, dim) - p.a.delta[st]), q_row, d, dim);
+        for (int d = 0; d < dim; d += 32) {
+            FiniteSum<T> g;
+            bool lost = false;
+#pragma unroll 1
+            for (int head = at.head; head < at.head + p.part_heads && !lost; ++head) {
+                const float table = BIAS ? load_table<T>(p, head) : 0.f;
+                const T *queries = row_of<T>(p.a.q, at, 0, p.a.q_row, head, p.a.q_head);
+                const T *grads = row_of<T>(p.a.d_out, at, 0, p.a.do_row, head, p.a.do_head);
+#pragma unroll 1
+                for (int q0 = begin; q0 < at.n && !lost; q0 += 32) {
+                    float s[16], dp[16];
+                    unpack(row_products(queries, p.a.q_row, q0, at.n, k_row, dim), s);
+                    f32x16 x = f32x16{};
+                    if (pass == 0) x = row_products(grads, p.a.do_row, q0, at.n, v_row, dim);
+                    unpack(x, dp);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int q = q0 + reg_row(i, h);
+                        const long long st = head * p.a.rows + at.base + min(q, at.n - 1);
+                        const RowWeight<T, BIAS> weight(p.a.stats[2 * st], p.a.stats[2 * st + 1], c);
+                        const float w = weight.of(pair_score<BIAS>(p, at, table, q, k, s[i]), c);
+                        s[i] = (pass == 0 ? weigh(w, dp[i] - p.a.delta[st]) : w) * times;
+                    }
+                    const T *from = pass == 0 ? queries : grads;
+                    const long long stride = pass == 0 ? p.a.q_row : p.a.do_row;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) g.add(from, stride, q0 + 16 * u, at.n, d, dim, s, u);
+                    lost = g.lost(d, dim, mine);
+                }
             }
-        }
-        const KeyGradients out(p, at, part);
-        const long long to = (row - at.base) * p.a.kv_heads * dim;
-        if (mine && p.parts > 1) {
-            store_eight<false>(out.dk + to, gk, p.a.scale, d, dim);
-            store_eight<false>(out.dv + to, gv, 1.f, d, dim);
-        } else if (mine) {
-            store_eight<false>((T *)p.a.dk + out.at + to, gk, p.a.scale, d, dim);
-            store_eight<false>((T *)p.a.dv + out.at + to, gv, 1.f, d, dim);
+            if (mine && p.parts > 1) g.template store<false>(sums + to, d, dim, 1.f / times, scale);
+            else if (mine) g.template store<false>(result + to, d, dim, 1.f / times, scale);
         }
     }
 }
@@ -956,12 +1049,13 @@ attention_forward_kernel(const RwkAttnArgs p) {
     // what pairs' weights follow from: exp2((score - base) c) * factor
     const float base = (ref == -INFINITY ? 0.f : ref) - (BIAS ? kExpUp<T> : 0), factor = BIAS ? inv : ldexpf(inv, kExpUp<T>);
     const long long o_at = ((at.base + qc) * p.a.heads + at.head) * dim;
-    const bool again = q < n && not_finite<KS>(acc.a);
+    bool again = q < n && not_finite<KS>(acc.a);
+    if (any_lane(again) && !masked_may_spoil<T, BIAS>(p, at, values.base, p.a.v_row, q0, end)) again = false;
     if (q < n && !again) {
         store_rows<false, T, DT>((T *)p.a.out + o_at, dim, h, acc.a, inv);
         if (p.a.out_low != nullptr) store_rows<true, T, DT>((T *)p.a.out_low + o_at, dim, h, acc.a, inv);
     }
-    if (any_lane(again)) exact_forward<T, BIAS>(p, at, table, q, end, base, factor, c, again);
+    if (any_lane(again)) again_forward<T, BIAS>(p, at, table, q, end, base, factor, c, again);
     if (q < n && p.a.stats != nullptr && h == 0) {
         float *st = p.a.stats + 2 * (at.head * p.a.rows + at.base + q);
         st[0] = base;
@@ -1101,13 +1195,14 @@ attention_dq_kernel(const RwkAttnArgs p) {
         values.commit(next + BN * S::W);
     }
     acc.finish();
-    const bool again = q < n && not_finite<KS>(acc.a);
+    bool again = q < n && not_finite<KS>(acc.a);
+    if (any_lane(again) && !masked_may_spoil<T, BIAS>(p, at, keys.base, p.a.k_row, q0, end)) again = false;
     scaled.undo(acc, 0);
     // A row's only pair has weight 1 whatever its score: no gradient, where d_out . v and delta, summed in different
     // orders, differ by a rounding.  (Times 0: what is not a number stays.)
     const float some = n == 1 || (causal && q == 0) ? 0.f : 1.f;
     if (q < n && !again) store_rows<false, T, DT>((T *)p.a.dq + o_at, dim, h, acc.a, p.a.scale * some);
-    if (any_lane(again)) exact_dq<T, BIAS>(p, at, table, q, end, weight, delta, c, again);
+    if (any_lane(again)) again_dq<T, BIAS>(p, at, table, q, end, weight, delta, c, scaled.by, p.a.scale * some, again);
     if (BIAS) {
         if (some == 0.f) buckets.times_zero();
         __syncthreads();
@@ -1272,7 +1367,9 @@ attention_dkv_kernel(const RwkAttnArgs p) {
     const long long to = kc * p.a.kv_heads * dim;
     dk.finish();
     dv.finish();
-    const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a), again = k < n && (bad_k || bad_v);
+    const bool bad_k = not_finite<KS>(dk.a), bad_v = not_finite<KS>(dv.a);
+    bool again = k < n && (bad_k || bad_v);
+    if (any_lane(again) && !masked_may_spoil_keys<T, BIAS>(p, at, k0, begin)) again = false;
     const float by = n == 1 ? 0.f * p.a.scale : p.a.scale;        // as in dQ: a segment of one row has one pair
     constexpr float dv_by = 1.f / (1 << kWeightUp<T>);
     scaled.undo(dk, kWeightUp<T>);
@@ -1283,7 +1380,7 @@ attention_dkv_kernel(const RwkAttnArgs p) {
         store_rows<false, T, DT>((T *)p.a.dk + out.at + to, dim, h, dk.a, by);
         store_rows<false, T, DT>((T *)p.a.dv + out.at + to, dim, h, dv.a, dv_by);
     }
-    if (any_lane(again)) exact_dkv<T, BIAS>(p, at, part, k, begin, c, again);
+    if (any_lane(again)) again_dkv<T, BIAS>(p, at, part, k, begin, c, scaled.by, by, again);
 }
 
 template <typename K>

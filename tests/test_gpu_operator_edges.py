@@ -233,3 +233,127 @@ def test_thousands_of_keys_that_a_row_hardly_looks_at(dev, dtype, dim, buckets):
     want = 100 * 4095 * small / (1 + 4095 * small)
     tol = {torch.float16: 2.0 ** (-25 + 19.7), torch.bfloat16: 2.0 ** -7, torch.float32: 1e-4}[dtype]
     assert float((out.double() / want - 1).abs().max()) <= tol
+
+
+def reference(q, k, v, do, lengths, causal, bias=None, codes=None):
+    """64-bit (out, dq, dk, dv), segment by segment; bias and codes as pair_buckets takes them, 255 masks."""
+    group, dim, lo, at = q.shape[1] // k.shape[1], q.shape[2], 0, 0
+    leaves = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    outs = []
+    for n in lengths:
+        a, b, c = (t[lo:lo + n].transpose(0, 1) for t in leaves)
+        s = a @ b.repeat_interleave(group, 0).transpose(1, 2) * dim ** -0.5
+        on = torch.ones(n, n, dtype=torch.bool, device=q.device)
+        on = on.tril() if causal else on
+        if bias is not None:
+            code = codes[at:at + n * n].view(n, n).long()
+            on = on & (code < bias.shape[1])
+            s = s + bias.double()[:, code.clamp(max=bias.shape[1] - 1)]
+        p = torch.softmax(s.masked_fill(~on, -torch.inf), 2).masked_fill(~on, 0.0)
+        outs.append((p @ c.repeat_interleave(group, 0)).transpose(0, 1))
+        lo, at = lo + n, at + n * n
+    out = torch.cat(outs)
+    return [out.detach(), *torch.autograd.grad(out, leaves, do.double())]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,buckets", [(16, 0), (24, 5), (64, 0), (64, 5), (128, 0), (100, 5)])
+@pytest.mark.parametrize("parts", [1, 3])
+def test_what_is_not_finite_reaches_what_attends_to_it_only(dev, dtype, dim, buckets, parts, monkeypatch):
+    """Single elements of v and of d_out that are not finite, in causal segments, with masked pairs if there is a bias:
+    the elements that weigh them are not finite, every other one is the result with zeros in their place."""
+    from gnn_amd import packed_attention, packed_segments, pair_buckets
+    from gnn_amd.attention import PackedSegments
+    monkeypatch.setattr(PackedSegments, "key_parts", lambda *a: parts)
+    g = torch.Generator(device=dev)
+    g.manual_seed(dim)
+    lengths, heads, kv = [300, 1, 77], 6, 2
+    total = sum(lengths)
+    q, k, v, do = (torch.randn(total, h, dim, generator=g, device=dev).to(dtype) for h in (heads, kv, kv, heads))
+    bias = codes = None
+    kw = {}
+    seg = packed_segments(lengths, dev)
+    if buckets:
+        bias = torch.randn(heads, buckets, generator=g, device=dev).to(dtype)
+        codes = torch.randint(0, buckets, (sum(n * n for n in lengths),), generator=g, device=dev).to(torch.uint8)
+        codes[torch.rand(codes.shape, generator=g, device=dev) < 0.3] = 255
+        codes[0] = 0                                              # row 0 attends to itself
+        kw = dict(bias=bias, buckets=pair_buckets(seg, codes))
+    on = torch.zeros(total, total, dtype=torch.bool, device=dev)
+    lo = at = 0
+    for n in lengths:
+        part = torch.ones(n, n, dtype=torch.bool, device=dev).tril()
+        if buckets:
+            part &= codes[at:at + n * n].view(n, n) < buckets
+        on[lo:lo + n, lo:lo + n] = part
+        lo, at = lo + n, at + n * n
+    tol = {torch.float32: 2e-5, torch.float16: 6e-3, torch.bfloat16: 5e-2}[dtype]
+
+    def check(got, want, spoilt, what):
+        """What is spoilt is not finite; the rest is within a few roundings of terms as large as the largest."""
+        assert not got[spoilt].isfinite().any(), what
+        rest = ~spoilt
+        assert got[rest].isfinite().all(), what
+        assert float((got.double() - want)[rest].abs().max()) <= tol * float(want.abs().max()), what
+
+    # values
+    bad = torch.zeros_like(v, dtype=torch.bool)
+    for row, head, d, x in ((5, 0, 3, math.inf), (64, 1, 0, math.nan), (150, 0, dim - 1, -math.inf), (151, 0, 1, math.inf),
+                            (299, 1, 2, math.nan), (340, 1, 7, math.inf)):
+        v[row, head, d], bad[row, head, d] = x, True
+    clean = torch.where(bad, 0.0, v).to(dtype)
+    want = reference(q, k, clean, do, lengths, True, bias, codes)
+    out = packed_attention(q, k, v, seg, causal=True, **kw)
+    spoilt = torch.einsum("ij,jhd->ihd", on.float(), bad.float()).repeat_interleave(heads // kv, 1) > 0
+    check(out, want[0], spoilt, "out")
+    # upstream gradients
+    bad = torch.zeros_like(do, dtype=torch.bool)
+    for row, head, d, x in ((0, 0, 3, math.inf), (40, 4, 0, math.nan), (41, 1, dim - 1, -math.inf), (290, 5, 1, math.inf),
+                            (376, 2, 2, math.inf)):
+        do[row, head, d], bad[row, head, d] = x, True
+    leaves = [t.clone().requires_grad_() for t in (q, k, clean)]
+    dq, dk, dv = torch.autograd.grad(packed_attention(*leaves, seg, causal=True, **kw), leaves, do)
+    want = reference(q, k, clean, torch.where(bad, 0.0, do).to(dtype), lengths, True, bias, codes)
+    rows = bad.any(2) & (on.sum(1) > 0)[:, None]                  # (row, head): delta is not finite
+    spoilt = rows[..., None].expand_as(dq)
+    check(dq, want[1], spoilt, "dq")
+    reach = torch.einsum("ij,ih->jh", on.float(), rows.float())   # (key, query head)
+    shared = reach.view(total, kv, -1).sum(2)[..., None].expand_as(dk) > 0
+    check(dk, want[2], shared, "dk")
+    some = torch.einsum("ij,ihd->jhd", on.float(), bad.float()).view(total, kv, -1, dim).sum(2) > 0
+    check(dv, want[3], some, "dv")
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,buckets", [(torch.float16, 16, 4, 64, 0), (torch.bfloat16, 16, 4, 128, 0),
+                                                      (torch.float16, 8, 8, 64, 32)])
+def test_time_of_what_is_not_finite(dev, dtype, heads, kv, dim, buckets):
+    """An overflowed step takes a bounded multiple of an ordinary one: twenty times as long at most where measured, several
+    hundred if the pairs were taken one by one."""
+    from gnn_amd import packed_attention, packed_segments, relative_buckets
+    lengths = [1500] * 6
+    n = sum(lengths)
+    seg = packed_segments(lengths, dev)
+    q, k, v, do = (torch.randn(n, h, dim, device=dev).to(dtype) for h in (heads, kv, kv, heads))
+    kw = {}
+    if buckets:
+        kw = dict(bias=torch.randn(heads, buckets, device=dev).to(dtype), buckets=relative_buckets(seg, buckets, 128))
+    places = torch.rand(n, device=dev) < 0.3
+
+    def times(v, do):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        ends = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        for _ in range(2):                                        # the second counts
+            ends[0].record()
+            out = packed_attention(*leaves, seg, causal=True, **kw)
+            ends[1].record()
+            torch.autograd.grad(out, leaves, do)
+            ends[2].record()
+        torch.cuda.synchronize()
+        return ends[0].elapsed_time(ends[1]), ends[1].elapsed_time(ends[2])
+    usual = times(v, do)
+    bad_v, bad_do, nan = v.clone(), do.clone(), torch.full_like(do, math.nan)
+    bad_v[places, :, 3] = math.inf
+    bad_do[places, :, 3] = math.inf
+    for got in (times(bad_v, do), times(v, bad_do), times(v, nan)):
+        for a, b in zip(got, usual):
+            assert a <= 60 * b + 1
