@@ -19,10 +19,11 @@
 //
 // The forward pass needs 2 products of a pair's rows, dQ 3 and dK/dV 4, and between them per pair an exponential (the
 // time of four other instructions) and four to eight more.  At 128 elements of 16 bits the matrix unit bounds all three,
-// at 64 the vector unit does; fp32 matrix instructions stop the vector unit, so there the two times add up.  4 prompts
-// of up to 8192 rows, 32 heads of 128 in bf16 over 8 of keys, causal: 917 us forward (0.81 of a large product's rate),
-// 1236 dQ (0.90), 2036 + 60 dK/dV (0.71); 48 of up to 1500, 16 heads of 64 in fp16 over 4: 146, 229, 245 us; 1024 graphs
-// of 100 to 500 nodes, 4 heads of 16 in fp32, a bias of 8 buckets: 481, 756, 787 us.
+// at 64 none of the units is busy all the time - a wavefront's
+// scores, exponentials and second products follow each other - with the vector unit the busiest; fp32 matrix instructions stop the vector unit, so there the two times add up.  4 prompts
+// of up to 8192 rows, 32 heads of 128 in bf16 over 8 of keys, causal: 907 us forward (0.82 of a large product's rate),
+// 1250 dQ (0.89), 1994 + 60 dK/dV (0.73); 48 of up to 1500, 16 heads of 64 in fp16 over 4: 148, 248, 280 us; 1024 graphs
+// of 100 to 500 nodes, 4 heads of 16 in fp32, a bias of 8 buckets: 495, 757, 789 us.
 //
 // Summed index of the second product: slot e of lane half h (h = lane / 32) of step s is row 16 s + 4 h + e for
 // e < 4 and 16 s + 8 + 4 h + (e - 4) otherwise, the registers 8 s + e of a 32x32 result.
@@ -496,7 +497,7 @@ __device__ inline int code_of(uint32_t codes, int e, int nb) { return min((int)(
 // LDS float atomic works through its lanes one by one: 180 cycles for a wavefront's 64 separate places, measured.)
 // SPLIT: four sets of them, one per place among four neighbouring pairs, each with a slot for the pairs that have no
 // bucket, so that four values are read, added and written without a look at each other's codes (fp32, 8 buckets, 1024
-// protein-sized graphs: 715 us for 809).  Otherwise all four
+// protein-sized graphs: dQ in seven eighths of the time).  Otherwise all four
 // sums are read before the first is written, and an equal code before takes the place of what was read.
 template <int NT, bool SPLIT>
 struct BucketSums {
@@ -1215,8 +1216,8 @@ attention_dq_kernel(const RwkAttnArgs p) {
 
 // dK and dV of 32 keys per wavefront.  Two wavefronts per SIMD hide each other's exponentials and LDS reads, which
 // leaves 256 registers each: at 128 elements of 16 bits the sums take 128 and the keys 32 of them, and the values stay
-// in LDS.  fp32 of up to 16 elements needs half of that, and four hide more (1024 protein-sized graphs: 791 us, 829 by
-// three).
+// in LDS.  fp32 of up to 16 elements needs half of that, and four hide more (1024 protein-sized graphs: 789 us; by
+// three 5 % more).
 template <typename T, int KS> constexpr bool values_in_lds() { return sizeof(T) == 2 && KS == 8; }
 template <typename T, int KS, int NW> constexpr int dkv_rows() {
     return values_in_lds<T, KS>() ? 32 : tile_rows<T, NW>();

@@ -333,8 +333,8 @@ norm_weight_sum_kernel(const float *__restrict__ partials, int n_partials, int w
 // Launch shapes.  Threads per row: as few as hold the row in one vector each up to a wavefront, so that narrow rows
 // (node features of a few channels) still fill every lane; wider rows give each lane of a wavefront, then of a
 // workgroup, more vectors.  A wavefront alone needs no barrier: up to 256 vectors it is at least as fast as a workgroup
-// (65536 x 1024 bf16 forward 45 us = 6.0 TB/s; 40000 x 2048 fp16 53), at 512 its registers leave too few rows in flight
-// (32768 x 4096 bf16: 148 us, by workgroups 96 = 5.6 TB/s).  The backward pass keeps two column sums per element besides
+// (65536 x 1024 bf16 forward 44 us = 6.1 TB/s; 40000 x 2048 fp16 58), at 512 its registers leave too few rows in flight
+// (32768 x 4096 bf16: 148 us, by workgroups 98 = 5.5 TB/s).  The backward pass keeps two column sums per element besides
 // the row and turns to the workgroup at 128.  A large copy runs at 5.1 TB/s on the same card.
 // Workgroups are few enough to stay resident and walk over the rows.  In the backward pass each also leaves a row of
 // partial sums: 512 of them are faster than 1024 for workgroup-wide rows (32768 x 4096 bf16: 150 + 5 us against

@@ -598,7 +598,7 @@ class AdamW(torch.optim.Optimizer):
             self._build_tables()
         lib = _lib.load()
         grads = [t.gather() for t in self._tables]        # all are checked before anything changes
-        if torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing() and all(t is not self._tables for t, _ in self._captured):
             self._captured.append((self._tables, self._made_from))
         for t, (addresses, _) in zip(self._tables, grads):
             t.step(lib, self, addresses)
