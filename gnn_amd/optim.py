@@ -542,11 +542,11 @@ class AdamW(torch.optim.Optimizer):
                 if t.dtype != dtype or t.shape != shape:
                     raise ValueError(f"{key} is {t.dtype} of shape {tuple(t.shape)} for a parameter of shape "
                                      f"{tuple(p.shape)}, not {dtype} of shape {tuple(shape)}")
-                room = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
-                if key == name and self.state_bits == 8 and (t.data_ptr() % 4 or room < 256 * blocks or not t.is_contiguous()):
-                    st[key] = self._new_state(p)[key].copy_(t)       # the kernel reads and writes whole blocks
-                elif not t.is_contiguous():
-                    st[key] = t.contiguous()
+                if not t.is_contiguous():
+                    st[key] = t = t.contiguous()
+                # the kernel reads and writes whole blocks, so the last one's rest has to be the tensor's own
+                if dtype == torch.float8_e4m3fn and (t.storage_offset() or t.untyped_storage().nbytes() != 256 * blocks):
+                    st[key] = self._new_state(p)[key].copy_(t)
 
     def _read_steps(self):
         """The step counts live on the device; the states get them when somebody looks."""

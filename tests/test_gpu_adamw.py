@@ -551,3 +551,34 @@ def test_options_that_would_be_another_optimiser(dev):
             if "weight_decay" not in options:
                 with pytest.raises(ValueError, match="gnn_amd.AdamW"):
                     AdamW([dict(params=[p], **options)])
+
+
+def test_8_bit_states_that_lie_in_one_buffer(dev):
+    """A caller keeps the states packed, one behind the other: nothing is written behind a state's last element."""
+    from gnn_amd import AdamW
+    params, grads = make(dev, torch.float32, [300, 77, 512], seed=3)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = AdamW(params, state_bits=8, seed=1), AdamW(twin, state_bits=8, seed=1)
+
+    def go():
+        for q in (params, twin):
+            for p, g in zip(q, grads[0]):
+                p.grad = g.clone()
+        a.step()
+        b.step()
+    go()
+    for name in ("exp_avg", "exp_avg_sq"):
+        buffer, at = torch.full((4096,), 17, dtype=torch.uint8, device=dev), 0
+        for p in params:
+            view = buffer[at:at + p.numel()].view(torch.float8_e4m3fn)
+            view.copy_(a.state[p][name])
+            a.state[p][name] = view
+            at += p.numel()
+        kept = buffer.clone()
+        go()
+        assert torch.equal(buffer[at:], kept[at:])
+    go()
+    assert all(torch.equal(p, q) for p, q in zip(params, twin))
+    for p, q in zip(params, twin):
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a.state[p][name].view(torch.uint8), b.state[q][name].view(torch.uint8))
