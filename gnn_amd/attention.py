@@ -338,16 +338,18 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments
     ``buckets``: added to the scaled products by the pair's bucket; an entry may be ``-inf``.
 
     Returns (N, H, D), contiguous.  A row that attends to nothing gives zeros.  Differentiable once with respect to
-    q, k, v and bias.  Sums, softmax statistics and the bias gradient are fp32; for the 16-bit types probabilities are
-    rounded to the type before they meet ``v`` (to two numbers of it for heads of up to 32 elements and in batches whose
-    longest segment has at most 256 rows), and so are, in the backward pass, probabilities and the gradients of the
-    scores before their products (to two numbers before ``k`` for heads of up to 32 elements).  Errors are then up to 1.5
-    times those of rounding the results once (1.65 in segments of one or two rows).  fp16: these factors are scaled to the type's range first, so that small
-    upstream gradients and many keys cost no digits.  Results repeat bit by bit; in another batch, whose longest segment or
-    padding asks for another launch shape, the same segment may differ within these errors.  What a pair's rows hold counts for nothing where the pair does not
-    attend, values that are not finite included: blocks of rows that such a value may have reached are computed a second
-    time, which takes up to some twenty times as long (2 prompts of 2048 rows, 32 heads of 128: forward 0.1 ms, 1.9 with
-    infinities all over ``v``).  Where it does attend, the elements it reaches are not finite, infinite or NaN."""
+    q, k, v and bias.  Sums, softmax statistics and the bias gradient are fp32; for the 16-bit types probabilities
+    are rounded to the type before they meet ``v`` (to two numbers of it for heads of up to 32 elements and in
+    batches whose longest segment has at most 256 rows), and so are, in the backward pass, probabilities and the
+    gradients of the scores before their products (to two numbers before ``k`` for heads of up to 32 elements).
+    Errors are then up to 1.5 times those of rounding the results once (1.65 in segments of one or two rows).  fp16:
+    these factors are scaled to the type's range first, so that small upstream gradients and many keys cost no
+    digits.  Results repeat bit by bit; in another batch, whose longest segment or padding asks for another launch
+    shape, the same segment may differ within these errors.  What a pair's rows hold counts for nothing where the
+    pair does not attend, values that are not finite included: blocks of rows that such a value may have reached are
+    computed a second time, which takes up to some twenty times as long (2 prompts of 2048 rows, 32 heads of 128:
+    forward 0.1 ms, 1.9 with infinities all over ``v``).  Where it does attend, the elements it reaches are not
+    finite, infinite or NaN."""
     if not q.is_cuda:
         raise RuntimeError("gnn_amd runs on HIP devices only (no CPU fallback)")
     shape, k_shape, dtype, device = q.shape, k.shape, q.dtype, q.device          # every look costs a small call time
