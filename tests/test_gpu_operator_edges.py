@@ -258,8 +258,9 @@ def reference(q, k, v, do, lengths, causal, bias=None, codes=None):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("dim,buckets", [(16, 0), (24, 5), (64, 0), (64, 5), (128, 0), (100, 5)])
-@pytest.mark.parametrize("parts", [1, 3])
-def test_what_is_not_finite_reaches_what_attends_to_it_only(dev, dtype, dim, buckets, parts, monkeypatch):
+@pytest.mark.parametrize("parts,lengths", [(1, [300, 1, 77]), (3, [300, 1, 77]), (1, [33] * 12)],
+                         ids=["whole", "parts", "short"])
+def test_what_is_not_finite_reaches_what_attends_to_it_only(dev, dtype, dim, buckets, parts, lengths, monkeypatch):
     """Single elements of v and of d_out that are not finite, in causal segments, with masked pairs if there is a bias:
     the elements that weigh them are not finite, every other one is the result with zeros in their place."""
     from gnn_amd import packed_attention, packed_segments, pair_buckets
@@ -267,12 +268,13 @@ def test_what_is_not_finite_reaches_what_attends_to_it_only(dev, dtype, dim, buc
     monkeypatch.setattr(PackedSegments, "key_parts", lambda *a: parts)
     g = torch.Generator(device=dev)
     g.manual_seed(dim)
-    lengths, heads, kv = [300, 1, 77], 6, 2
-    total = sum(lengths)
-    q, k, v, do = (torch.randn(total, h, dim, generator=g, device=dev).to(dtype) for h in (heads, kv, kv, heads))
+    heads, kv, total = 6, 2, sum(lengths)
+    rows = torch.randn(total, 2 * heads + 2 * kv, dim, generator=g, device=dev).to(dtype)
+    q, k, v, do = (t.clone() if dim == 64 else t for t in rows.split([heads, kv, kv, heads], 1))     # or slices of one
     bias = codes = None
     kw = {}
     seg = packed_segments(lengths, dev)
+    assert seg.block_rows == (32 if len(lengths) == 12 else 128)
     if buckets:
         bias = torch.randn(heads, buckets, generator=g, device=dev).to(dtype)
         codes = torch.randint(0, buckets, (sum(n * n for n in lengths),), generator=g, device=dev).to(torch.uint8)
